@@ -222,6 +222,71 @@ b200_status b200_compensated_sum(uint64_t sum, uint64_t cmp, uint64_t add, int32
 b200_status b200_log2_hist(uint64_t in, int32_t dtype, uint64_t count, uint64_t hist, int32_t nbins,
                            int32_t offset, uint64_t stream);
 
+/* ---- operators of language models
+ * Matrices travel as descriptors: the address of element (0, 0) and the element strides along the
+ * first axis (features or words) and along the second (items).  Any strides are accepted, so that
+ * both neon's order (items next to each other) and its transposed view (the features of an item
+ * next to each other) can be handed in.  Vectors of one value per feature or per item are
+ * contiguous; an address of 0 leaves an optional one out.  An output may be the input of the same
+ * shape itself where that is said; any other sharing of memory is refused (B200_ERR_INVALID).
+ * Element types of matrices: f32, f16, bf16, with fp32 arithmetic and rounding to nearest.
+ * `scratch` is 256-byte aligned device memory of at least the size the matching *_scratch_bytes
+ * function gives; it is overwritten, and calls that share it must be ordered on the GPU.
+ * `launches` (may be null) receives the number of kernels launched. */
+typedef struct b200_matrix {
+    uint64_t ptr;
+    int64_t s0, s1;
+    int32_t dtype;
+    int32_t reserved;
+} b200_matrix;
+
+/* layer normalisation of every item over its features, y = (x - mean) * rstd * gamma + beta, next to
+ * the batch normalisation entry points (neon/backends/nervanagpu.py:2463-2588).  gamma and beta
+ * (param_dtype), mean and rstd (f32, written) are optional.  y may be x. */
+b200_status b200_ln_fprop(const b200_matrix *x, const b200_matrix *y, uint64_t gamma, uint64_t beta,
+                          int32_t param_dtype, uint64_t mean, uint64_t rstd, int64_t features, int64_t items,
+                          float eps, uint64_t stream, int32_t *launches);
+/* its gradient: delta with respect to x (may be x or the error), grad_gamma and grad_beta
+ * (param_dtype, optional) summed over the items; mean and rstd as the forward call wrote them */
+uint64_t    b200_ln_bprop_scratch_bytes(int64_t features, int64_t items);
+b200_status b200_ln_bprop(const b200_matrix *delta, const b200_matrix *error, const b200_matrix *x,
+                          uint64_t mean, uint64_t rstd, uint64_t gamma, uint64_t grad_gamma, uint64_t grad_beta,
+                          int32_t param_dtype, int64_t features, int64_t items, uint64_t scratch,
+                          uint64_t scratch_bytes, uint64_t stream, int32_t *launches);
+
+/* embedding lookup, out[f, n] = scale * table[ids[n], f]; `table` is (words, features), ids int32.
+ * A word number outside the table gives zeros. */
+b200_status b200_lut_fprop(uint64_t ids, const b200_matrix *table, const b200_matrix *out, int64_t words,
+                           int64_t features, int64_t positions, float scale, uint64_t stream);
+/* its gradient, replacing compound_bprop_lut (neon/backends/nervanagpu.py): dtable[v] = beta *
+ * dtable[v] + alpha * (sum of error[:, n] over the positions n that hold v), for every row of
+ * dtable; word pad_idx (-1: none) and numbers outside the table collect nothing.  The same bits in
+ * every run. */
+uint64_t    b200_lut_bprop_scratch_bytes(int64_t words, int64_t features, int64_t positions);
+b200_status b200_lut_bprop(uint64_t ids, const b200_matrix *error, const b200_matrix *dtable, int64_t words,
+                           int64_t features, int64_t positions, int64_t pad_idx, float alpha, float beta,
+                           uint64_t scratch, uint64_t scratch_bytes, uint64_t stream, int32_t *launches);
+
+/* distillation from a teacher's `top` largest logits (any float type) at the words top_ids (int32),
+ * both (top, items): cost[n] = weights[n] T^2 KL(softmax(top_logits / T) || softmax(logits / T)), and
+ * delta its gradient with respect to the logits (optional; may be the logits).  Entries whose word
+ * lies outside the vocabulary or whose logit is -inf are left out; an item of weight 0 or without
+ * an entry has cost 0 and delta 0. */
+#define B200_DISTILL_MAX_TOP 1024
+b200_status b200_distill(const b200_matrix *logits, const b200_matrix *delta, const b200_matrix *top_ids,
+                         const b200_matrix *top_logits, uint64_t weights, uint64_t cost, int64_t words,
+                         int64_t items, int64_t top, float temperature, uint64_t stream, int32_t *launches);
+
+/* clipped policy cost: with l the log-probability of the item's word actions[n] (int32; written to
+ * logp when that is given), r = exp(l - old_logp) and d = ref_logp - l, cost[n] = weights[n] *
+ * (kl_coef * (exp(d) - d - 1) - min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)), and delta its
+ * gradient with respect to the logits (optional; may be the logits).  weights and, for kl_coef 0,
+ * ref_logp are optional.  An item whose word lies outside the vocabulary has cost, logp and delta 0. */
+b200_status b200_policy(const b200_matrix *logits, const b200_matrix *delta, uint64_t actions, uint64_t old_logp,
+                        uint64_t ref_logp, uint64_t advantages, uint64_t weights, uint64_t cost, uint64_t logp,
+                        int64_t words, int64_t items, float clip_low, float clip_high, float kl_coef,
+                        uint64_t stream, int32_t *launches);
+
 /* ---- the same reduction for callers that cannot allocate device memory
  * No counterpart in the reference.  Meant for hosts where cudaMalloc is off
  * limits when the call is made (a framework pool owns the device, a latency-

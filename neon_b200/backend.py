@@ -4,14 +4,16 @@ The ``b200`` backend: executes op-trees on one B200 through libb200ew.so.
 Stands where neon's ``NervanaGPU`` stands for the op-tree path
 (neon/backends/nervanagpu.py:694-1439, 1825-1861, 3138-3231): same constructor
 keywords as ``gen_backend`` forwards (neon/backends/__init__.py:107-114), same
-tensor factories, ``execute``, RNG state functions and timing marks.  Methods
-of the abstract backend that are not op-tree work (GEMM, convolution, pooling,
-lookup tables) raise ``NotImplementedError``.
+tensor factories, ``execute``, RNG state functions and timing marks.  Operators of
+language models (layer normalisation, lookup tables, costs on logits) are mixed in
+from ``lm.py``.  Methods of the abstract backend that are neither (GEMM, convolution,
+pooling) raise ``NotImplementedError``.
 """
 
 import numpy as np
 
 from . import runtime as rt
+from .lm import LanguageModelOps
 from .lowering import BoundPlan, MixedExtents, Planner, Statement, dtype_code, program_key
 from .optree import OpCollection, OpTreeBackend, OpTreeNode, Tensor
 from .tensor import B200Tensor
@@ -118,7 +120,7 @@ class CapturedGraph(object):
             pass
 
 
-class B200Backend(OpTreeBackend):
+class B200Backend(LanguageModelOps, OpTreeBackend):
     backend_name = "b200"
     tensor_cls = B200Tensor
 
@@ -834,7 +836,7 @@ class B200Backend(OpTreeBackend):
         return C
 
     batched_dot = conv_layer = deconv_layer = fprop_conv = bprop_conv = _off_path
-    update_conv = pool_layer = fprop_pool = bprop_pool = compound_bprop_lut = _off_path
+    update_conv = pool_layer = fprop_pool = bprop_pool = _off_path
 
 
 def gen_backend(backend="b200", rng_seed=None, datatype=np.float32, batch_size=0,

@@ -1,0 +1,143 @@
+// What the kernels of the language-model operators share (layernorm.cu, lookup.cu,
+// logit_cost.cu): matrix descriptors and their checks on the host, launches, and
+// warp / block reductions.
+#pragma once
+
+#include "b200ew.h"
+#include "optree_templates.cuh"
+
+#include <cuda_runtime.h>
+
+#include <cstdio>
+
+extern "C" void* b200_detail_stream(uint64_t stream);
+extern "C" int32_t b200_detail_fail(int32_t code, const char* message);
+extern "C" int32_t b200_detail_device(void);
+
+namespace nn {
+
+using namespace b200;
+
+// ------------------------------------------------------------------ host side
+inline bool is_float(int dt) { return dt == B200_F32 || dt == B200_F16 || dt == B200_BF16; }
+inline i64 esize(int dt) { return dt == B200_F32 || dt == B200_I32 || dt == B200_U32 ? 4 : dt == B200_I8 || dt == B200_U8 ? 1 : 2; }
+
+// First byte and one past the last byte that an (n0, n1) matrix reaches.
+inline void span(const b200_matrix& m, i64 n0, i64 n1, i64& lo, i64& hi) {
+    const i64 e = esize(m.dtype), a = (n0 - 1) * m.s0 * e, b = (n1 - 1) * m.s1 * e;
+    lo = (i64)m.ptr + (a < 0 ? a : 0) + (b < 0 ? b : 0);
+    hi = (i64)m.ptr + (a > 0 ? a : 0) + (b > 0 ? b : 0) + e;
+}
+
+// Whether two matrices can share memory.  Spans that do not meet are apart; two views with the
+// same pitch along one axis, whose extents along the other fit into the pitch side by side (the
+// halves of one buffer, say), are apart as well; everything else counts as shared.
+inline bool meet(const b200_matrix& a, i64 a0, i64 a1, const b200_matrix& b, i64 b0, i64 b1) {
+    if (a0 <= 0 || a1 <= 0 || b0 <= 0 || b1 <= 0) return false;
+    i64 alo, ahi, blo, bhi;
+    span(a, a0, a1, alo, ahi);
+    span(b, b0, b1, blo, bhi);
+    if (ahi <= blo || bhi <= alo) return false;
+    const i64 ea = esize(a.dtype), eb = esize(b.dtype);
+    const i64 pa[2] = {a.s0 * ea, a.s1 * ea}, pb[2] = {b.s0 * eb, b.s1 * eb};
+    const i64 na[2] = {a0, a1}, nb[2] = {b0, b1};
+    for (int k = 0; k < 2; ++k) {
+        const i64 pitch = pa[k], wa = pa[1 - k], wb = pb[1 - k];
+        if (pitch != pb[k] || pitch <= 0 || wa <= 0 || wb <= 0) continue;
+        const i64 la = (na[1 - k] - 1) * wa + ea, lb = (nb[1 - k] - 1) * wb + eb;      // bytes of one line
+        if (la > pitch || lb > pitch) continue;
+        i64 d = ((i64)b.ptr - (i64)a.ptr) % pitch;
+        if (d < 0) d += pitch;
+        if (d >= la && d + lb <= pitch) return false;
+    }
+    return true;
+}
+
+// element-aligned addresses; 0 stands for an argument left out
+inline bool aligned(uint64_t ptr, int dt) { return ptr % (uint64_t)esize(dt) == 0; }
+
+inline bool same(const b200_matrix& a, const b200_matrix& b) {
+    return a.ptr == b.ptr && a.s0 == b.s0 && a.s1 == b.s1 && a.dtype == b.dtype;
+}
+
+// Sets the library's device for the length of a call, whatever the calling thread's current
+// device is.
+class DeviceScope {
+public:
+    DeviceScope() {
+        const int want = b200_detail_device();
+        if (want < 0) { err_ = cudaErrorInvalidDevice; return; }
+        err_ = cudaGetDevice(&was_);
+        if (err_ == cudaSuccess && was_ != want) {
+            err_ = cudaSetDevice(want);
+            moved_ = err_ == cudaSuccess;
+        }
+    }
+    ~DeviceScope() { if (moved_) cudaSetDevice(was_); }
+    cudaError_t error() const { return err_; }
+
+private:
+    int was_ = 0;
+    bool moved_ = false;
+    cudaError_t err_ = cudaSuccess;
+};
+
+inline int32_t refuse(const char* where, const char* what, int32_t code = B200_ERR_INVALID) {
+    char msg[320];
+    snprintf(msg, sizeof msg, "%s: %s", where, what);
+    return b200_detail_fail(code, msg);
+}
+inline int32_t cuda_status(const char* where, cudaError_t e) {
+    return e == cudaSuccess ? B200_OK : refuse(where, cudaGetErrorString(e), B200_ERR_CUDA);
+}
+
+// ------------------------------------------------------------------ device side
+// one element of a floating-point array whose type is known at run time only
+DEV float ld_any(u64 base, i64 off, int dt) {
+    if (dt == F32) return *(reinterpret_cast<const float*>(base) + off);
+    const u32 w = *(reinterpret_cast<const u16*>(base) + off);
+    return dt == F16 ? h2f(w) : bf2f(w);
+}
+DEV void st_any(u64 base, i64 off, int dt, float v) {
+    if (dt == F32) *(reinterpret_cast<float*>(base) + off) = v;
+    else *(reinterpret_cast<u16*>(base) + off) = (u16)(dt == F16 ? f2h_rn(v) : f2bf_rn(v));
+}
+
+// V neighbouring elements, 16-byte aligned when V > 1
+template <int DT, int V> DEV void st_f(u64 base, i64 off, const float* v) {
+    constexpr int B = dt_size<DT>::value * V;
+    u32 w[(B + 3) / 4];
+    cvt_out<DT, V, false>(v, w, SrCtx(), nullptr);
+    st_raw<B>(reinterpret_cast<char*>(base) + off * dt_size<DT>::value, w);
+}
+
+DEV float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+DEV float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+// Sum over a block, in the same order in every run, known to every thread.  `s` holds 32 floats;
+// the first barrier keeps a previous use of it apart.
+DEV float block_sum(float v, float* s) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
+    v = warp_sum(v);
+    __syncthreads();
+    if (lane == 0) s[warp] = v;
+    __syncthreads();
+    return warp_sum(lane < warps ? s[lane] : 0.f);
+}
+DEV float block_max(float v, float* s) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
+    v = warp_max(v);
+    __syncthreads();
+    if (lane == 0) s[warp] = v;
+    __syncthreads();
+    return warp_max(lane < warps ? s[lane] : -INFINITY);
+}
+
+}  // namespace nn

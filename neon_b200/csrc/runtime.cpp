@@ -185,6 +185,7 @@ extern "C" int b200_detail_gemm(uint64_t a, int da, int64_t a_s0, int64_t a_s1, 
 
 // helpers for the other translation units of the library
 extern "C" void *b200_detail_stream(uint64_t stream) { return stream ? reinterpret_cast<void *>(stream) : g.stream; }
+extern "C" int32_t b200_detail_device(void) { return g.device; }      // -1 before b200_init
 extern "C" int32_t b200_detail_fail(int32_t code, const char *message) { return fail(code, "%s", message); }
 
 extern "C" {

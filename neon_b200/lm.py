@@ -1,0 +1,336 @@
+"""
+Operators of language models around their matrix products, as methods of the b200 backend:
+layer normalisation and its gradient, the embedding lookup and its gradient, and two costs
+on the logits (distillation from a teacher's largest logits, clipped policy cost with a KL
+term) with theirs.  They stand beside ``compound_fprop_bn`` / ``compound_bprop_bn`` and take
+their arguments in neon's way: results are written into tensors the caller owns, matrices
+have the shape (features, items), vectors of one value per feature (F, 1), vectors of one
+value per item (1, N).
+
+Both orders of memory are supported everywhere, as are other strides: neon's own, in which
+the items of one feature are neighbours, and the order in which the features of one item
+are, handed over as the transposed view of an (items, features) tensor::
+
+    h = be.empty((tokens, width), dtype=bfloat16)          # one row per token
+    be.compound_fprop_lut(ids, W, h.T, scale=width ** 0.5)
+    be.compound_fprop_ln(h.T, mean, rstd, gamma, beta, y.T)
+
+Arithmetic is fp32; results are rounded to the tensor's type once, to nearest (a tensor whose
+``rounding`` asks for stochastic rounding is refused as a result).  Work is issued on
+``be.stream`` and uses the backend's scratch, as statements do; nothing is allocated, so a
+call can be recorded with ``be.capture``.
+"""
+
+import numpy as np
+
+from . import runtime as rt
+from .lowering import dtype_code
+from .tensor import B200Tensor
+
+_NONE = rt.Matrix(0, 0, 0, rt.F32, 0)
+_FLOATS = (rt.F32, rt.F16, rt.BF16)
+
+
+class LanguageModelOps(object):
+    """Mixed into ``B200Backend``."""
+
+    # ------------------------------------------------------------------ arguments
+    @staticmethod
+    def _lm_tensor(t, name):
+        if not isinstance(t, B200Tensor):
+            if hasattr(t, "local"):
+                raise NotImplementedError("%s: sharded tensors" % name)
+            raise TypeError("%s must be a tensor of the backend, got %s" % (name, type(t).__name__))
+        if t.take_array is not None:
+            raise NotImplementedError("%s: a tensor indexed with an array" % name)
+        return t
+
+    def _lm_matrix(self, t, name, shape=None, out=False, floats=True):
+        """Descriptor of a matrix argument, after its checks."""
+        self._lm_tensor(t, name)
+        if len(t.shape) != 2 or (shape is not None and t.shape != shape):
+            raise ValueError("%s has shape %s, expected %s" % (name, t.shape, shape or "two dimensions"))
+        code = dtype_code(t.dtype)
+        if floats and code not in _FLOATS:
+            raise TypeError("%s must be float32, float16 or bfloat16, not %s" % (name, t.dtype))
+        if out:
+            self._lm_output(t, name)
+        return rt.Matrix(t.gpudata, t.strides[0], t.strides[1], code, 0)
+
+    def _lm_vector(self, t, name, size, dtype=None, out=False):
+        """Address of a contiguous vector argument of ``size`` values (0 for None)."""
+        if t is None:
+            return 0
+        self._lm_tensor(t, name)
+        if t.size != size or (size and max(t.shape) != size):
+            raise ValueError("%s has shape %s, expected %d values" % (name, t.shape, size))
+        if size > 1 and t.strides[t.shape.index(size)] != 1:
+            raise ValueError("%s must be contiguous" % name)
+        if dtype is not None and t.dtype.type is not dtype:
+            raise TypeError("%s must be %s, not %s" % (name, np.dtype(dtype).name, t.dtype))
+        if out:
+            self._lm_output(t, name)
+        return t.gpudata
+
+    @staticmethod
+    def _lm_output(t, name):
+        if t.rounding:
+            raise NotImplementedError("%s: stochastic rounding of this operator's result" % name)
+        for d, s in zip(t.shape, t.strides):
+            if d > 1 and s == 0:
+                raise ValueError("%s repeats its elements and cannot be written" % name)
+
+    @staticmethod
+    def _lm_span(t):
+        """First byte and one past the last byte that a tensor reaches."""
+        if not t.size:
+            return 0, 0
+        reach = [(d - 1) * s for d, s in zip(t.shape, t.strides)]
+        size = t.dtype.itemsize
+        return (t.gpudata + size * sum(r for r in reach if r < 0),
+                t.gpudata + size * (1 + sum(r for r in reach if r > 0)))
+
+    @staticmethod
+    def _lm_params(first, second, names):
+        """Common type code of two optional parameter vectors."""
+        for t, name in zip((first, second), names):
+            if t is not None and dtype_code(t.dtype) not in _FLOATS:
+                raise TypeError("%s must be float32, float16 or bfloat16, not %s" % (name, t.dtype))
+        if first is not None and second is not None and first.dtype != second.dtype:
+            raise TypeError("%s and %s must have one type" % names)
+        given = first if first is not None else second
+        return rt.F32 if given is None else dtype_code(given.dtype)
+
+    def _lm_scratch(self, nbytes):
+        if not nbytes:
+            return 0
+        self._scratch.reset()
+        return self._scratch(nbytes, zero=False)
+
+    def _lm_check(self, *tensors):
+        if self.check_bounds:
+            self.check_operands([t for t in tensors if t is not None])
+
+    # ------------------------------------------------------------------ layer normalisation
+    def compound_fprop_ln(self, x, mean, rstd, gamma, beta, y, eps=1e-5):
+        """
+        Layer normalisation of every item (column) of ``x`` over its features::
+
+            y = (x - mean) * rstd * gamma + beta,   rstd = 1 / sqrt(var + eps)
+
+        Arguments:
+            x, y: (features, items), float32, float16 or bfloat16, one type; y may be x
+            mean, rstd: (1, items) float32, written for the backward pass, or None
+            gamma, beta: (features, 1), one floating type, or None (1 and 0)
+            eps: added to the variance (the centred one, over all features)
+        """
+        mx = self._lm_matrix(x, "x")
+        my = self._lm_matrix(y, "y", x.shape, out=True)
+        if x.dtype != y.dtype:
+            raise TypeError("x and y must have one type")
+        f, n = x.shape
+        pdt = self._lm_params(gamma, beta, ("gamma", "beta"))
+        args = (self._lm_vector(gamma, "gamma", f), self._lm_vector(beta, "beta", f), pdt,
+                self._lm_vector(mean, "mean", n, np.float32, out=True),
+                self._lm_vector(rstd, "rstd", n, np.float32, out=True))
+        self._lm_check(x, y, gamma, beta, mean, rstd)
+        self.launches += rt.ln_fprop(mx, my, *args, f, n, float(eps), self.stream)
+        return y
+
+    def compound_bprop_ln(self, delta_out, grad_gamma, grad_beta, delta_in, x, mean, rstd, gamma):
+        """
+        Gradient of ``compound_fprop_ln``, arguments in the order of ``compound_bprop_bn``.
+
+        Arguments:
+            delta_out: (features, items), written: the error with respect to x; may be
+                delta_in or x itself
+            grad_gamma, grad_beta: (features, 1) of one floating type, written: sums over the
+                items of delta_in * (x - mean) * rstd and of delta_in; or None
+            delta_in: (features, items): the error with respect to y
+            x, mean, rstd, gamma: as given to and left by the forward pass
+        """
+        mx = self._lm_matrix(x, "x")
+        me = self._lm_matrix(delta_in, "delta_in", x.shape)
+        md = self._lm_matrix(delta_out, "delta_out", x.shape, out=True)
+        if x.dtype != delta_in.dtype or x.dtype != delta_out.dtype:
+            raise TypeError("x, delta_in and delta_out must have one type")
+        if mean is None or rstd is None:
+            raise ValueError("the backward pass needs the forward pass's mean and rstd")
+        f, n = x.shape
+        pdt = self._lm_params(grad_gamma, grad_beta, ("grad_gamma", "grad_beta"))
+        if gamma is not None:
+            gdt = self._lm_params(gamma, None, ("gamma", None))
+            if (grad_gamma is not None or grad_beta is not None) and gdt != pdt:
+                raise TypeError("gamma, grad_gamma and grad_beta must have one type")
+            pdt = gdt
+        args = (self._lm_vector(mean, "mean", n, np.float32), self._lm_vector(rstd, "rstd", n, np.float32),
+                self._lm_vector(gamma, "gamma", f), self._lm_vector(grad_gamma, "grad_gamma", f, out=True),
+                self._lm_vector(grad_beta, "grad_beta", f, out=True))
+        self._lm_check(x, delta_in, delta_out, mean, rstd, gamma, grad_gamma, grad_beta)
+        nbytes = rt.ln_bprop_scratch_bytes(f, n)
+        scratch = self._lm_scratch(nbytes)
+        self.launches += rt.ln_bprop(md, me, mx, *args, pdt, f, n, scratch, nbytes, self.stream)
+        return delta_out
+
+    # ------------------------------------------------------------------ embedding table
+    def compound_fprop_lut(self, inputs, W, outputs, scale=1.0):
+        """
+        Embedding lookup: column n of ``outputs`` becomes ``scale * W[inputs[n]]``.
+
+        Arguments:
+            inputs: int32 word numbers, contiguous, one per column of outputs; a number
+                outside the table gives a column of zeros
+            W: (vocabulary, features) table
+            outputs: (features, positions), of W's type
+            scale: factor of every value looked up
+        """
+        mw = self._lm_matrix(W, "W")
+        self._lm_tensor(outputs, "outputs")
+        mo = self._lm_matrix(outputs, "outputs", (W.shape[1], outputs.shape[-1]), out=True)
+        if W.dtype != outputs.dtype:
+            raise TypeError("W and outputs must have one type")
+        n = outputs.shape[1]
+        ids = self._lm_words(inputs, "inputs", n)
+        self._lm_check(inputs, W, outputs)
+        if n:
+            rt.lut_fprop(ids, mw, mo, W.shape[0], W.shape[1], n, float(scale), self.stream)
+            self.launches += 1
+        return outputs
+
+    def _lm_words(self, t, name, size):
+        self._lm_tensor(t, name)
+        if t.dtype.type is not np.int32:
+            raise TypeError("%s must be int32, not %s" % (name, t.dtype))
+        if t.size != size or not t.is_contiguous:
+            raise ValueError("%s must hold %d contiguous word numbers, got shape %s" % (name, size, t.shape))
+        return t.gpudata
+
+    def compound_bprop_lut(self, nin, inputs, error, error_t, dW, pad_idx=None, alpha=1.0, beta=0):
+        """
+        Gradient of the embedding table, with the arguments of neon's lookup layer::
+
+            dW[v] = beta * dW[v] + alpha * sum of error[:, n] over the positions n that hold v
+
+        for every row of dW, so dW need not be cleared first.  Deterministic: positions are
+        sorted by word and summed in order, without floating-point atomics.
+
+        Arguments:
+            nin: positions per example (the number of positions is taken from ``inputs``)
+            inputs: int32 word numbers, contiguous; numbers outside the table are skipped
+            error: (features, positions), float32, float16 or bfloat16
+            error_t: (positions, features) buffer of error's type, which receives the error
+                transposed when error's features are not neighbours already; or None (the
+                strided error is then read as it lies, which is slower)
+            dW: (vocabulary, features), any of the three types
+            pad_idx: word that takes no gradient, or None
+        """
+        me = self._lm_matrix(error, "error")
+        mw = self._lm_matrix(dW, "dW", (dW.shape[0], error.shape[0]), out=True)
+        f, n = error.shape
+        ids = self._lm_words(inputs, "inputs", n)
+        if error_t is not None:
+            self._lm_matrix(error_t, "error_t", (n, f), out=True)
+            if error_t.dtype != error.dtype:
+                raise TypeError("error and error_t must have one type")
+            for t, name in ((error, "error"), (dW, "dW"), (inputs, "inputs")):
+                lo, hi = self._lm_span(t)
+                first, last = self._lm_span(error_t)
+                if lo < last and first < hi:
+                    raise ValueError("error_t must lie apart from %s" % name)
+        self._lm_check(inputs, error, error_t, dW)
+        pad = -1 if pad_idx is None else int(pad_idx)
+        nbytes = rt.lut_bprop_scratch_bytes(dW.shape[0], f, max(n, 1))
+        scratch = self._lm_scratch(nbytes)
+        if error_t is not None and n > 1 and f > 1 and error.strides[0] != 1:
+            self.copy_transpose(error, error_t)
+            me = rt.Matrix(error_t.gpudata, error_t.strides[1], error_t.strides[0], me.dtype, 0)
+        self.launches += rt.lut_bprop(ids, me, mw, dW.shape[0], f, n, pad, float(alpha), float(beta), scratch, nbytes,
+                                      self.stream)
+        return dW
+
+    # ------------------------------------------------------------------ costs on logits
+    def compound_distill(self, logits, top_ids, top_logits, cost, delta=None, weights=None, temperature=1.0):
+        """
+        Distillation from a teacher's largest logits and, with ``delta``, its gradient::
+
+            p = softmax(top_logits / T) over an item's entries, q = softmax(logits / T)
+            cost  = weights * T^2 * sum_k p_k * (log p_k - log q[top_ids_k])
+            delta = weights * T * (q - p scattered to the vocabulary)
+
+        Arguments:
+            logits: (vocabulary, items), float32, float16 or bfloat16
+            top_ids: (K, items) int32, K <= 1024; an entry outside the vocabulary is left
+                out, a word that occurs twice collects both of its entries
+            top_logits: (K, items) teacher's logits or log-probabilities, of any of the
+                three types; an entry of -inf is left out
+            cost: (1, items) float32, written
+            delta: like logits, written; may be logits itself; None for the cost alone
+            weights: (1, items) float32 factors of cost and delta (None: 1).  An item of
+                weight 0, or without an entry, has cost and delta 0 whatever its logits hold
+            temperature: T > 0
+        """
+        mz = self._lm_matrix(logits, "logits")
+        v, n = logits.shape
+        md = self._lm_delta(delta, logits)
+        self._lm_tensor(top_ids, "top_ids")
+        if top_ids.dtype.type is not np.int32:
+            raise TypeError("top_ids must be int32, not %s" % top_ids.dtype)
+        k = top_ids.shape[0]
+        mi = self._lm_matrix(top_ids, "top_ids", (k, n), floats=False)
+        mt = self._lm_matrix(top_logits, "top_logits", (k, n))
+        if cost is None:
+            raise ValueError("cost must be a tensor")
+        args = (self._lm_vector(weights, "weights", n, np.float32), self._lm_vector(cost, "cost", n, np.float32, out=True))
+        self._lm_check(logits, delta, top_ids, top_logits, weights, cost)
+        self.launches += rt.distill(mz, md, mi, mt, *args, v, n, k, float(temperature), self.stream)
+        return cost
+
+    def _lm_delta(self, delta, logits):
+        if delta is None:
+            return _NONE
+        md = self._lm_matrix(delta, "delta", logits.shape, out=True)
+        if delta.dtype != logits.dtype:
+            raise TypeError("logits and delta must have one type")
+        return md
+
+    def compound_policy(self, logits, actions, old_logp, advantages, cost, delta=None, logp=None, ref_logp=None,
+                        weights=None, clip=0.2, kl_coef=0.0):
+        """
+        Clipped policy cost with a KL term and, with ``delta``, its gradient with respect to
+        the logits: with l the log-probability of the chosen word, r = exp(l - old_logp) and
+        d = ref_logp - l::
+
+            cost = weights * (kl_coef * (exp(d) - d - 1)
+                              - min(r * A, clip(r, 1 - low, 1 + high) * A))
+
+        Arguments:
+            logits: (vocabulary, items), float32, float16 or bfloat16
+            actions: int32, one chosen word per item, contiguous; an item whose word lies
+                outside the vocabulary (a padded position) has cost, delta and logp 0
+            old_logp, advantages: (1, items) float32
+            cost: (1, items) float32, written
+            delta: like logits, written; may be logits itself; None for the cost alone
+            logp: (1, items) float32, written: l; or None
+            ref_logp: (1, items) float32, needed when kl_coef is not 0
+            weights: (1, items) float32 factors of cost and delta (None: 1); an item of
+                weight 0 has cost and delta 0 whatever its logits hold
+            clip: one number, or (low, high)
+            kl_coef: factor of the KL term
+        """
+        mz = self._lm_matrix(logits, "logits")
+        v, n = logits.shape
+        md = self._lm_delta(delta, logits)
+        low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+        for t, name in ((old_logp, "old_logp"), (advantages, "advantages"), (cost, "cost")):
+            if t is None:
+                raise ValueError("%s must be a tensor" % name)
+        if kl_coef != 0 and ref_logp is None:
+            raise ValueError("a KL term needs ref_logp")
+        vec = self._lm_vector
+        args = (self._lm_words(actions, "actions", n), vec(old_logp, "old_logp", n, np.float32),
+                vec(ref_logp, "ref_logp", n, np.float32), vec(advantages, "advantages", n, np.float32),
+                vec(weights, "weights", n, np.float32), vec(cost, "cost", n, np.float32, out=True),
+                vec(logp, "logp", n, np.float32, out=True))
+        self._lm_check(logits, delta, actions, old_logp, ref_logp, advantages, weights, cost, logp)
+        self.launches += rt.policy(mz, md, *args, v, n, float(low), float(high), float(kl_coef), self.stream)
+        return cost

@@ -27,6 +27,11 @@ class DeviceProps(C.Structure):
                 ("total_mem", u64), ("name", C.c_char * 64)]
 
 
+class Matrix(C.Structure):
+    """A strided (features, items) matrix as the language-model operators take it."""
+    _fields_ = [("ptr", u64), ("s0", C.c_int64), ("s1", C.c_int64), ("dtype", i32), ("reserved", i32)]
+
+
 # name -> (restype, argtypes); everything include/b200ew.h declares
 SIGNATURES = {
     "b200_version": (i32, []),
@@ -80,6 +85,18 @@ SIGNATURES = {
     "b200_dimshuffle": (i32, [u64, u64, i32, i32, P(C.c_int64), P(C.c_int64), P(C.c_int64), u64]),
     "b200_compensated_sum": (i32, [u64, u64, u64, i32, u64, C.c_float, C.c_float, i32, u64]),
     "b200_log2_hist": (i32, [u64, i32, u64, u64, i32, i32, u64]),
+    "b200_ln_fprop": (i32, [P(Matrix), P(Matrix), u64, u64, i32, u64, u64, C.c_int64, C.c_int64, C.c_float, u64, P(i32)]),
+    "b200_ln_bprop_scratch_bytes": (u64, [C.c_int64, C.c_int64]),
+    "b200_ln_bprop": (i32, [P(Matrix), P(Matrix), P(Matrix), u64, u64, u64, u64, u64, i32, C.c_int64, C.c_int64,
+                            u64, u64, u64, P(i32)]),
+    "b200_lut_fprop": (i32, [u64, P(Matrix), P(Matrix), C.c_int64, C.c_int64, C.c_int64, C.c_float, u64]),
+    "b200_lut_bprop_scratch_bytes": (u64, [C.c_int64, C.c_int64, C.c_int64]),
+    "b200_lut_bprop": (i32, [u64, P(Matrix), P(Matrix), C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_float,
+                             C.c_float, u64, u64, u64, P(i32)]),
+    "b200_distill": (i32, [P(Matrix), P(Matrix), P(Matrix), P(Matrix), u64, u64, C.c_int64, C.c_int64, C.c_int64,
+                           C.c_float, u64, P(i32)]),
+    "b200_policy": (i32, [P(Matrix), P(Matrix), u64, u64, u64, u64, u64, u64, u64, C.c_int64, C.c_int64, C.c_float,
+                          C.c_float, C.c_float, u64, P(i32)]),
     "b200_reduce_full_noalloc_max_count": (u64, []),
     "b200_reduce_full_noalloc": (i32, [u64, i32, u64, i32, i32, u64, u64]),
     "b200_comm_unique_id": (i32, [P(C.c_uint8)]),
@@ -369,6 +386,55 @@ def compensated_sum(sum_ptr, cmp_ptr, add_ptr, dtype, count, cmp_scale, add_scal
 
 def log2_hist(src, dtype, count, hist, nbins, offset, stream=0):
     check(lib().b200_log2_hist(src, dtype, count, hist, nbins, offset, stream))
+
+
+def ln_fprop(x, y, gamma, beta, param_dtype, mean, rstd, features, items, eps, stream=0):
+    """Layer normalisation (matrices as ``Matrix``); returns the number of kernels launched."""
+    n = i32(0)
+    check(lib().b200_ln_fprop(x, y, gamma, beta, param_dtype, mean, rstd, features, items, eps, stream, n))
+    return n.value
+
+
+def ln_bprop_scratch_bytes(features, items):
+    return int(lib().b200_ln_bprop_scratch_bytes(features, items))
+
+
+def ln_bprop(delta, error, x, mean, rstd, gamma, grad_gamma, grad_beta, param_dtype, features, items,
+             scratch, scratch_bytes, stream=0):
+    n = i32(0)
+    check(lib().b200_ln_bprop(delta, error, x, mean, rstd, gamma, grad_gamma, grad_beta, param_dtype, features,
+                              items, scratch, scratch_bytes, stream, n))
+    return n.value
+
+
+def lut_fprop(ids, table, out, words, features, positions, scale, stream=0):
+    check(lib().b200_lut_fprop(ids, table, out, words, features, positions, scale, stream))
+
+
+def lut_bprop_scratch_bytes(words, features, positions):
+    return int(lib().b200_lut_bprop_scratch_bytes(words, features, positions))
+
+
+def lut_bprop(ids, error, dtable, words, features, positions, pad_idx, alpha, beta, scratch, scratch_bytes, stream=0):
+    n = i32(0)
+    check(lib().b200_lut_bprop(ids, error, dtable, words, features, positions, pad_idx, alpha, beta, scratch,
+                               scratch_bytes, stream, n))
+    return n.value
+
+
+def distill(logits, delta, top_ids, top_logits, weights, cost, words, items, top, temperature, stream=0):
+    n = i32(0)
+    check(lib().b200_distill(logits, delta, top_ids, top_logits, weights, cost, words, items, top, temperature,
+                             stream, n))
+    return n.value
+
+
+def policy(logits, delta, actions, old_logp, ref_logp, advantages, weights, cost, logp, words, items, clip_low,
+           clip_high, kl_coef, stream=0):
+    n = i32(0)
+    check(lib().b200_policy(logits, delta, actions, old_logp, ref_logp, advantages, weights, cost, logp, words,
+                            items, clip_low, clip_high, kl_coef, stream, n))
+    return n.value
 
 
 def reduce_full_noalloc(src, dtype, count, op, absolute, out, stream=0):

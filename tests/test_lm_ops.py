@@ -1,0 +1,190 @@
+"""
+CPU tests of the language-model operators: what the backend's methods and the C entry points
+refuse, before anything reaches a device, and the formulas of tests/lm_reference.py against
+differences.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from neon_b200 import runtime as rt
+from neon_b200.dryrun import DryRunBackend
+from tests import lm_reference as ref
+
+
+@pytest.fixture(scope="module")
+def be():
+    return DryRunBackend()
+
+
+def ln_args(be, f=8, n=6, dtype=np.float32):
+    return dict(x=be.empty((f, n), dtype), mean=be.empty((1, n)), rstd=be.empty((1, n)), gamma=be.empty((f, 1)),
+                beta=be.empty((f, 1)), y=be.empty((f, n), dtype))
+
+
+def refused(error, fn, args, match=None, **change):
+    args = dict(args, **change)
+    with pytest.raises(error, match=match):
+        fn(**args)
+
+
+def rounding(t):
+    t.rounding = 10
+    return t
+
+
+def test_layer_norm_refusals(be):
+    a, fn = ln_args(be), be.compound_fprop_ln
+    refused(ValueError, fn, a, "y has shape", y=be.empty((6, 8)))
+    refused(TypeError, fn, a, "one type", y=be.empty((8, 6), np.float16))
+    refused(TypeError, fn, a, "float32, float16 or bfloat16", x=be.empty((8, 6), np.int32))
+    refused(TypeError, fn, a, "gamma", gamma=be.empty((8, 1), np.int32))
+    refused(TypeError, fn, a, "one type", gamma=be.empty((8, 1), np.float16))
+    refused(ValueError, fn, a, "gamma has shape", gamma=be.empty((7, 1)))
+    refused(ValueError, fn, a, "beta must be contiguous", beta=be.empty((8, 3))[:, 1:2])
+    refused(TypeError, fn, a, "mean must be float32", mean=be.empty((1, 6), np.float16))
+    refused(ValueError, fn, a, "rstd has shape", rstd=be.empty((1, 8)))
+    refused(TypeError, fn, a, "tensor of the backend", x=np.zeros((8, 6), np.float32))
+    refused(ValueError, fn, a, "two dimensions", x=be.empty((2, 4, 6)))
+    refused(NotImplementedError, fn, a, "stochastic", y=rounding(be.empty((8, 6))))
+    refused(NotImplementedError, fn, a, "indexed with an array", x=be.empty((9, 6))[be.empty((8, 1), np.int32)])
+    refused(rt.B200Error, fn, a, "eps", eps=-1.0)
+    refused(rt.B200Error, fn, a, "eps", eps=float("nan"))
+    buf = be.empty((8, 13))
+    refused(rt.B200Error, fn, a, "not a shifted view", x=buf[:, :6], y=buf[:, 1:7])
+    refused(rt.B200Error, fn, a, "shares memory", mean=a["y"][0:1])
+    refused(rt.B200Error, fn, a, "share memory", rstd=a["mean"])
+    b = dict(delta_out=be.empty((8, 6)), grad_gamma=be.empty((8, 1)), grad_beta=be.empty((8, 1)),
+             delta_in=be.empty((8, 6)), x=a["x"], mean=a["mean"], rstd=a["rstd"], gamma=a["gamma"])
+    fn = be.compound_bprop_ln
+    refused(ValueError, fn, b, "mean and rstd", mean=None)
+    refused(ValueError, fn, b, "delta_in has shape", delta_in=be.empty((8, 5)))
+    refused(TypeError, fn, b, "one type", delta_out=be.empty((8, 6), np.float16))
+    refused(TypeError, fn, b, "one type", grad_beta=be.empty((8, 1), np.float16))
+    refused(TypeError, fn, b, "one type", gamma=be.empty((8, 1), np.float16))
+    refused(NotImplementedError, fn, b, "stochastic", grad_gamma=rounding(be.empty((8, 1))))
+    be._scratch = lambda nbytes, zero: be._fake(nbytes)
+    be._scratch.reset = lambda: None
+    try:
+        refused(rt.B200Error, fn, b, "shares memory", grad_gamma=b["grad_beta"])
+        refused(rt.B200Error, fn, b, "shares memory", grad_gamma=b["x"].reshape(1, 48)[:, :8])
+        refused(rt.B200Error, fn, b, "shifted view", delta_out=buf[:, :6], x=buf[:, 3:9])
+    finally:
+        be._scratch = None
+
+
+def test_lookup_refusals(be):
+    a = dict(inputs=be.empty((1, 6), np.int32), W=be.empty((10, 8)), outputs=be.empty((8, 6)))
+    fn = be.compound_fprop_lut
+    refused(TypeError, fn, a, "int32", inputs=be.empty((1, 6)))
+    refused(ValueError, fn, a, "6 contiguous", inputs=be.empty((1, 7), np.int32))
+    refused(ValueError, fn, a, "contiguous", inputs=be.empty((6, 2), np.int32)[:, 0:1])
+    refused(ValueError, fn, a, "outputs has shape", outputs=be.empty((9, 6)))
+    refused(TypeError, fn, a, "one type", outputs=be.empty((8, 6), np.float16))
+    refused(rt.B200Error, fn, a, "shares memory", outputs=a["W"].reshape(8, 10)[:, :6])
+    b = dict(nin=1, inputs=a["inputs"], error=be.empty((8, 6)), error_t=None, dW=be.empty((10, 8)))
+    fn = be.compound_bprop_lut
+    refused(ValueError, fn, b, "dW has shape", dW=be.empty((10, 7)))
+    refused(ValueError, fn, b, "error_t has shape", error_t=be.empty((8, 6)))
+    refused(TypeError, fn, b, "one type", error_t=be.empty((6, 8), np.float16))
+    refused(TypeError, fn, b, "float32, float16 or bfloat16", dW=be.empty((10, 8), np.int32))
+    refused(TypeError, fn, b, "int32", inputs=be.empty((1, 6), np.uint32))
+    refused(ValueError, fn, b, "apart", error_t=b["error"].reshape(6, 8))
+    refused(NotImplementedError, fn, b, "stochastic", dW=rounding(be.empty((10, 8))))
+
+
+def test_cost_refusals(be):
+    n, v, k = 5, 20, 3
+    row = lambda dtype=np.float32: be.empty((1, n), dtype)                          # noqa: E731
+    a = dict(logits=be.empty((v, n)), top_ids=be.empty((k, n), np.int32), top_logits=be.empty((k, n)), cost=row(),
+             delta=be.empty((v, n)), weights=row())
+    fn = be.compound_distill
+    refused(TypeError, fn, a, "int32", top_ids=be.empty((k, n)))
+    refused(ValueError, fn, a, "top_logits has shape", top_logits=be.empty((k + 1, n)))
+    refused(ValueError, fn, a, "delta has shape", delta=be.empty((n, v)))
+    refused(TypeError, fn, a, "one type", delta=be.empty((v, n), np.float16))
+    refused(ValueError, fn, a, "cost must be", cost=None)
+    refused(TypeError, fn, a, "float32", cost=row(np.float16))
+    refused(ValueError, fn, a, "weights has shape", weights=be.empty((1, n + 1)))
+    refused(NotImplementedError, fn, a, "stochastic", delta=rounding(be.empty((v, n))))
+    for t in (0.0, -1.0, float("nan"), float("inf"), 1e-45):
+        refused(rt.B200Error, fn, a, "temperature", temperature=t)
+    refused(rt.B200Error, fn, a, "1024", top_ids=be.empty((1025, n), np.int32), top_logits=be.empty((1025, n)))
+    refused(rt.B200Error, fn, a, "shares memory", cost=a["weights"])
+    refused(rt.B200Error, fn, a, "shares memory", cost=a["logits"][0:1])
+    refused(rt.B200Error, fn, a, "shares memory", cost=a["top_logits"][1:2])
+    buf = be.empty((v + 1, n))
+    refused(rt.B200Error, fn, a, "shifted view", logits=buf[:v], delta=buf[1:])
+    b = dict(logits=a["logits"], actions=row(np.int32), old_logp=row(), advantages=row(), cost=row(), delta=a["delta"],
+             logp=row(), ref_logp=row(), weights=row(), clip=(0.2, 0.3), kl_coef=0.1)
+    fn = be.compound_policy
+    refused(TypeError, fn, b, "int32", actions=row())
+    refused(ValueError, fn, b, "ref_logp", ref_logp=None)
+    refused(ValueError, fn, b, "advantages", advantages=None)
+    refused(ValueError, fn, b, "old_logp has shape", old_logp=be.empty((1, n + 1)))
+    refused(rt.B200Error, fn, b, "clip", clip=-0.1)
+    refused(rt.B200Error, fn, b, "clip", clip=(0.1, float("nan")))
+    refused(rt.B200Error, fn, b, "finite", kl_coef=float("inf"))
+    refused(rt.B200Error, fn, b, "share", logp=b["cost"])
+    refused(rt.B200Error, fn, b, "shares memory", logp=b["old_logp"])
+
+
+def test_sharded_tensors_are_refused(be):
+    from neon_b200.sharded import ShardedTensor
+    x = ShardedTensor(be, (8, 12), be.empty((8, 6)), 0)
+    with pytest.raises(NotImplementedError, match="sharded"):
+        be.compound_fprop_ln(x, None, None, None, None, x)
+
+
+def test_entry_points_refuse_null_and_misaligned(be):
+    lib = rt.lib()
+    m = rt.Matrix(1 << 20, 1, 8, rt.F32, 0)
+    odd = rt.Matrix((1 << 20) + 2, 1, 8, rt.F32, 0)
+    far = rt.Matrix(1 << 30, 1, 8, rt.F32, 0)
+    assert lib.b200_ln_fprop(None, m, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 0, None) == -1
+    assert lib.b200_ln_fprop(odd, far, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 0, None) == -1 and "misaligned" in rt.last_error()
+    assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 0, 4, 1e-5, 0, None) == -1
+    assert lib.b200_ln_fprop(m, far, 0, 0, rt.I32, 0, 0, 8, 4, 1e-5, 0, None) == -7
+    assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 8, -1, 1e-5, 0, None) == -1
+    assert lib.b200_lut_bprop(1 << 22, m, far, 8, 8, 4, -1, 1.0, 0.0, 0, 0, 0, None) == -1 and "scratch" in rt.last_error()
+    assert lib.b200_distill(m, None, None, m, 0, 1 << 25, 8, 4, 2, 1.0, 0, None) == -1
+    assert lib.b200_policy(m, None, 0, 0, 0, 0, 0, 1 << 25, 0, 8, 4, 0.2, 0.2, 0.0, 0, None) == -1
+    if rt.device_count() == 0:                       # a good call reports the missing device
+        n = C.c_int32(5)
+        assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 0, n) == -2 and n.value == 0
+
+
+def test_scratch_of_the_table_gradient_is_bounded():
+    for v, f, n in ((10, 8, 1), (50000, 1024, 131072), (262144, 64, 1 << 20), (1000, 16384, 4096), (300000, 4096, 1 << 20)):
+        nbytes = rt.lut_bprop_scratch_bytes(v, f, n)
+        assert 16 * n <= nbytes <= (33 << 20) + 18 * n + 4 * (v + 1) + 16384 + 8 * f
+
+
+@pytest.mark.parametrize("which", ["ln", "distill", "policy"])
+def test_reference_gradients_against_differences(which):
+    rng = np.random.RandomState(0)
+    v, n, step = 9, 3, 1e-6
+    z = rng.standard_normal((v, n)) * 2
+    if which == "ln":
+        gamma, beta, e = rng.uniform(0.5, 1.5, (v, 1)), rng.uniform(-1, 1, (v, 1)), rng.standard_normal((v, n))
+        loss = lambda a: (ref.ln_fprop(a, gamma, beta, 1e-5, np.float32)["y"][0] * e).sum()        # noqa: E731
+        out = ref.ln_fprop(z, gamma, beta, 1e-5, np.float32)
+        delta = ref.ln_bprop(e, z, out["mean"][0], out["rstd"][0], gamma, np.float32, np.float32)["delta"][0]
+    elif which == "distill":
+        ids = np.array([[0, 1, -1], [3, 1, 2], [8, 4, 2]])
+        top, w = rng.standard_normal((3, n)), np.array([[1.0, 0.5, 2.0]])
+        loss = lambda a: ref.distill(a, ids, top, w, 1.7, np.float32)["cost"][0].sum()              # noqa: E731
+        delta = ref.distill(z, ids, top, w, 1.7, np.float32)["delta"][0]
+    else:
+        act, old = np.array([[0, 5, 8]]), np.array([[-2.0, -1.0, -4.0]])
+        new_ref, adv = np.array([[-1.5, -2.5, -3.0]]), np.array([[1.0, -1.0, 0.5]])
+        args = (act, old, new_ref, adv, None, 0.2, 0.28, 0.1, np.float32)
+        loss = lambda a: ref.policy(a, *args)["cost"][0].sum()                                       # noqa: E731
+        delta = ref.policy(z, *args)["delta"][0]
+    for i in range(v):
+        for j in range(n):
+            up, down = z.copy(), z.copy()
+            up[i, j] += step
+            down[i, j] -= step
+            assert abs((loss(up) - loss(down)) / (2 * step) - delta[i, j]) < 1e-7

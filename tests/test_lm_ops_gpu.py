@@ -1,0 +1,565 @@
+"""
+Layer normalisation, the embedding table, and the distillation and policy costs on the GPU
+against their formulas in float64 (tests/lm_reference.py), at the sizes, orders and masks where
+they can go wrong.
+"""
+import numpy as np
+import pytest
+
+from tests import lm_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+bf16 = pytest.importorskip("ml_dtypes").bfloat16
+DTYPES = [np.float32, np.float16, bf16]
+ORDERS = ["rows", "cols", "pitched", "shifted", "strided"]
+MARK = 77.0
+
+
+class Held(object):
+    """A (f, n) matrix on the device in some order of memory, and the elements around it."""
+
+    def __init__(self, be, host, dtype, order):
+        host = np.asarray(host).astype(dtype)
+        f, n = host.shape
+        self.order = order
+        if order == "rows":
+            self.base = be.array(np.ascontiguousarray(host.T), dtype=dtype)
+            self.view = self.base.T
+            self.inside = np.s_[:, :]
+        elif order == "cols":
+            self.base = self.view = be.array(host, dtype=dtype)
+            self.inside = np.s_[:, :]
+        elif order in ("pitched", "shifted"):            # rows of a wider buffer, at an aligned or odd offset
+            first, wide = (16, f + 32 + (-f) % 16) if order == "pitched" else (3, f + 5)
+            buf = np.full((n, wide), MARK, dtype)
+            buf[:, first:first + f] = host.T
+            self.base = be.array(buf, dtype=dtype)
+            self.view = self.base[:, first:first + f].T
+            self.inside = np.s_[:, first:first + f]
+        else:                                            # every second element of both axes
+            buf = np.full((2 * f, 2 * n), MARK, dtype)
+            buf[::2, ::2] = host
+            self.base = be.array(buf, dtype=dtype)
+            self.view = self.base[::2, ::2]
+            self.inside = np.s_[::2, ::2]
+
+    def get(self):
+        """The matrix; the elements around it must be as they were."""
+        buf = self.base.get()
+        if self.order in ("pitched", "shifted", "strided"):
+            out = np.ones(buf.shape, bool)
+            out[self.inside] = False
+            assert (buf[out].astype(np.float32) == MARK).all(), "elements outside the matrix were written"
+        part = buf[self.inside]
+        return part.T if self.order in ("rows", "pitched", "shifted") else part
+
+
+def vector(be, host, dtype=np.float32):
+    return be.array(np.asarray(host), dtype=dtype)
+
+
+def nan_like(shape):
+    return np.full(shape, np.nan)
+
+
+def compare(got, want):
+    for name in want:
+        if name in got:
+            ref.check(name, got[name], want[name])
+
+
+# ---------------------------------------------------------------- layer normalisation
+LN_SIZES = [(1, 1), (1, 5), (7, 3), (64, 33), (129, 17), (256, 40), (1000, 9), (1001, 70), (1024, 32), (2048, 300),
+            (4096, 5), (8200, 3), (16384, 2), (40000, 2)]
+
+
+def ln_inputs(f, n, dtype, pdtype, seed=0):
+    rng = np.random.RandomState(seed + f * 131 + n)
+    x = (rng.standard_normal((f, n)) * rng.uniform(0.5, 2, (1, n)) + rng.uniform(-4, 4, (1, n))).astype(dtype)
+    gamma = rng.uniform(0.5, 1.5, (f, 1)).astype(pdtype)
+    beta = rng.uniform(-1, 1, (f, 1)).astype(pdtype)
+    e = rng.standard_normal((f, n)).astype(dtype)
+    return x, gamma, beta, e
+
+
+def run_ln(be, x, gamma, beta, e, dtype, pdtype, order, eps=1e-5, inplace=False):
+    f, n = x.shape
+    hx = Held(be, x, dtype, order)
+    hy = hx if inplace else Held(be, nan_like((f, n)), dtype, order)
+    mean, rstd = vector(be, nan_like((1, n))), vector(be, nan_like((1, n)))
+    g = None if gamma is None else vector(be, gamma, pdtype)
+    b = None if beta is None else vector(be, beta, pdtype)
+    be.compound_fprop_ln(hx.view, mean, rstd, g, b, hy.view, eps)
+    got = {"y": hy.get(), "mean": mean.get(), "rstd": rstd.get()}
+    hx = Held(be, x, dtype, order)
+    he = Held(be, e, dtype, order)
+    hd = {False: None, True: he, "x": hx}[inplace] or Held(be, nan_like((f, n)), dtype, order)
+    gg, gb = vector(be, nan_like((f, 1)), pdtype), vector(be, nan_like((f, 1)), pdtype)
+    be.compound_bprop_ln(hd.view, gg, gb, he.view, hx.view, mean, rstd, g)
+    got.update(delta=hd.get(), grad_gamma=gg.get(), grad_beta=gb.get())
+    return got
+
+
+def want_ln(x, gamma, beta, e, got, dtype, pdtype, eps=1e-5):
+    want = ref.ln_fprop(x, gamma, beta, eps, dtype)
+    want.update(ref.ln_bprop(e, x, got["mean"], got["rstd"], gamma, dtype, pdtype))
+    return want
+
+
+@pytest.mark.parametrize("f,n", LN_SIZES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: np.dtype(d).name)
+def test_layer_norm_sizes_and_orders(b200, f, n, dtype):
+    for order in ORDERS:
+        pdtype = np.float32 if order != "cols" else dtype
+        x, gamma, beta, e = ln_inputs(f, n, dtype, pdtype)
+        got = run_ln(b200, x, gamma, beta, e, dtype, pdtype, order)
+        compare(got, want_ln(x, gamma, beta, e, got, dtype, pdtype))
+
+
+@pytest.mark.parametrize("order", ["rows", "cols", "shifted"])
+@pytest.mark.parametrize("inplace", [True, "x"])
+@pytest.mark.parametrize("f,n", [(100, 7), (2048, 30), (20000, 3)])
+def test_layer_norm_in_place(b200, f, n, inplace, order):
+    x, gamma, beta, e = ln_inputs(f, n, bf16, np.float32)
+    got = run_ln(b200, x, gamma, beta, e, bf16, np.float32, order, inplace=inplace)
+    compare(got, want_ln(x, gamma, beta, e, got, bf16, np.float32))
+
+
+@pytest.mark.parametrize("order", ["rows", "cols"])
+def test_layer_norm_without_parameters_and_statistics(b200, order):
+    be = b200
+    x, gamma, beta, e = ln_inputs(520, 12, np.float32, np.float32)
+    for g, b in ((None, None), (gamma, None), (None, beta)):
+        got = run_ln(be, x, g, b, e, np.float32, np.float32, order)
+        compare(got, want_ln(x, g, b, e, got, np.float32, np.float32))
+    hx, hy = Held(be, x, np.float32, order), Held(be, nan_like(x.shape), np.float32, order)
+    be.compound_fprop_ln(hx.view, None, None, vector(be, gamma), vector(be, beta), hy.view)
+    ref.check("y", hy.get(), ref.ln_fprop(x, gamma, beta, 1e-5, np.float32)["y"])
+    # the error with respect to x alone
+    mean, rstd = x.mean(0, keepdims=True), 1 / np.sqrt(x.var(0, keepdims=True) + 1e-5)
+    hd = Held(be, nan_like(x.shape), np.float32, order)
+    be.compound_bprop_ln(hd.view, None, None, Held(be, e, np.float32, order).view, hx.view, vector(be, mean),
+                         vector(be, rstd), vector(be, gamma))
+    ref.check("delta", hd.get(), ref.ln_bprop(e, x, mean, rstd, gamma, np.float32, np.float32)["delta"])
+
+
+@pytest.mark.parametrize("order", ["rows", "cols"])
+def test_layer_norm_constant_items_offsets_and_bad_items(b200, order):
+    f, n = 768, 10
+    x, gamma, beta, e = ln_inputs(f, n, np.float32, np.float32)
+    x[:, 0] = 3.0                                   # no variance: eps decides
+    x[:, 1] = 0.0
+    x[:, 2] += 4096.0                               # mean far from zero
+    got = run_ln(b200, x, gamma, beta, e, np.float32, np.float32, order)
+    compare(got, want_ln(x, gamma, beta, e, got, np.float32, np.float32))
+    bad = x.copy()
+    bad[5, 4], bad[6, 7] = np.nan, np.inf           # reach their own items and no other
+    hx, hy = Held(b200, bad, np.float32, order), Held(b200, nan_like(x.shape), np.float32, order)
+    b200.compound_fprop_ln(hx.view, None, None, vector(b200, gamma), vector(b200, beta), hy.view)
+    y, clean = hy.get(), np.delete(np.arange(n), [4, 7])
+    assert np.isnan(y[:, [4, 7]]).all()
+    want = ref.ln_fprop(x, gamma, beta, 1e-5, np.float32)["y"]
+    ref.check("y", y[:, clean], (want[0][:, clean], want[1][:, clean]))
+
+
+def test_layer_norm_no_items(b200):
+    be = b200
+    x = be.empty((16, 0))
+    gg, gb = vector(be, nan_like((16, 1))), vector(be, nan_like((16, 1)))
+    be.compound_fprop_ln(x, None, None, None, None, be.empty((16, 0)))
+    be.compound_bprop_ln(be.empty((16, 0)), gg, gb, be.empty((16, 0)), x, be.empty((1, 0)), be.empty((1, 0)), None)
+    assert (gg.get() == 0).all() and (gb.get() == 0).all()
+
+
+def test_layer_norm_gradient_against_differences(b200):
+    f, n, step = 24, 5, 1e-5
+    rng = np.random.RandomState(3)
+    x, gamma, beta, e = ln_inputs(f, n, np.float32, np.float32)
+    got = run_ln(b200, x, gamma, beta, e, np.float32, np.float32, "rows")
+
+    def loss(x64, g64, b64):
+        return (ref.ln_fprop(x64, g64, b64, 1e-5, np.float32)["y"][0] * e).sum()
+
+    x, gamma, beta = (a.astype(np.float64) for a in (x, gamma, beta))
+    for name, a, args in (("delta", x, 0), ("grad_gamma", gamma, 1), ("grad_beta", beta, 2)):
+        for _ in range(12):
+            at = (rng.randint(a.shape[0]), rng.randint(a.shape[1]))
+            up, down = a.copy(), a.copy()
+            up[at] += step
+            down[at] -= step
+            sets = [[x, gamma, beta], [x, gamma, beta]]
+            sets[0][args], sets[1][args] = up, down
+            slope = (loss(*sets[0]) - loss(*sets[1])) / (2 * step)
+            # central differences: step^2 times the third derivative, and 2^-53 of the loss over the step
+            assert abs(got[name][at] - slope) < 1e-4 * max(1.0, abs(slope)), (name, at)
+
+
+# ---------------------------------------------------------------- embedding table
+def words(rng, v, n):
+    """Word numbers with a few frequent ones."""
+    ids = rng.randint(0, v, n)
+    often = rng.rand(n) < 0.4
+    ids[often] = rng.randint(0, v, 3)[rng.randint(0, 3, often.sum())]
+    return ids.astype(np.int32)
+
+
+LUT_SIZES = [(1, 1, 1), (5, 3, 40), (100, 64, 1), (300, 33, 500), (1000, 128, 4096), (511, 40, 5000), (512, 16, 9000),
+             (50000, 8, 300), (20, 1000, 70), (3, 256, 20000)]
+
+
+@pytest.mark.parametrize("v,f,n", LUT_SIZES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: np.dtype(d).name)
+def test_lookup_sizes_and_orders(b200, v, f, n, dtype):
+    be = b200
+    rng = np.random.RandomState(v + f + n)
+    w = rng.standard_normal((v, f)).astype(dtype)
+    ids = words(rng, v, n)
+    e = rng.standard_normal((f, n)).astype(dtype)
+    old = rng.standard_normal((v, f))
+    for i, order in enumerate(ORDERS):
+        out = Held(be, nan_like((f, n)), dtype, order)
+        # the table: row by row, or the same strides as the result's
+        table = Held(be, w, dtype, "cols" if i % 2 == 0 else "strided")
+        be.compound_fprop_lut(be.array(ids.reshape(1, n), dtype=np.int32), table.view, out.view, scale=1.7)
+        ref.check("out", out.get(), ref.lut_fprop(ids, w, np.float32(1.7), dtype)["out"])
+        wdt = np.float32 if i % 2 == 0 else dtype
+        pad = [None, 0, int(ids[0])][i % 3]
+        alpha, beta = [(1.0, 0.0), (0.5, 1.0), (2.0, -0.25)][(i + v) % 3]
+        dw = Held(be, old if beta else nan_like((v, f)), wdt, "cols" if i % 2 == 0 else "strided")
+        error = Held(be, e, dtype, order)
+        et = be.empty((n, f), dtype=dtype) if i % 2 else None
+        be.compound_bprop_lut(1, be.array(ids.reshape(n, 1), dtype=np.int32), error.view, et, dw.view, pad, alpha, beta)
+        want = ref.lut_bprop(ids, e, old.astype(wdt), pad, alpha, beta, wdt)
+        ref.check("dW", dw.get(), want["dW"])
+
+
+@pytest.mark.parametrize("order", ["rows", "cols"])
+def test_lookup_numbers_outside_the_table(b200, order):
+    be = b200
+    v, f, n = 37, 24, 200
+    rng = np.random.RandomState(0)
+    ids = rng.randint(-3, v + 3, n).astype(np.int32)
+    ids[:3] = [-2 ** 31, 2 ** 31 - 1, v]
+    w, e = rng.standard_normal((v, f)).astype(np.float32), rng.standard_normal((f, n)).astype(np.float32)
+    out = Held(be, nan_like((f, n)), np.float32, order)
+    dev = be.array(ids.reshape(1, n), dtype=np.int32)
+    be.compound_fprop_lut(dev, be.array(w), out.view)
+    ref.check("out", out.get(), ref.lut_fprop(ids, w, 1.0, np.float32)["out"])
+    dw = be.array(nan_like((v, f)))
+    be.compound_bprop_lut(1, dev, Held(be, e, np.float32, order).view, be.empty((n, f)), dw, 5)
+    ref.check("dW", dw.get(), ref.lut_bprop(ids, e, w, 5, 1.0, 0.0, np.float32)["dW"])
+    # nothing but skipped positions, whose error may be anything
+    dev = be.array(np.full((1, n), 5), dtype=np.int32)
+    be.compound_bprop_lut(1, dev, Held(be, nan_like((f, n)), np.float32, order).view, None, dw, 5)
+    assert (dw.get() == 0).all()
+
+
+def test_lookup_no_positions(b200):
+    be = b200
+    ids, dw = be.empty((1, 0), dtype=np.int32), be.array(np.ones((6, 4)))
+    be.compound_fprop_lut(ids, be.array(np.ones((6, 4))), be.empty((4, 0)))
+    be.compound_bprop_lut(1, ids, be.empty((4, 0)), None, dw, beta=0.5)
+    assert (dw.get() == 0.5).all()
+    be.compound_bprop_lut(1, ids, be.empty((4, 0)), None, dw)
+    assert (dw.get() == 0).all()
+
+
+@pytest.mark.parametrize("n", [700, 30000])
+def test_lookup_gradient_has_the_same_bits_in_every_run(b200, n):
+    be = b200
+    rng = np.random.RandomState(1)
+    ids = be.array(words(rng, 600, n).reshape(1, n), dtype=np.int32)
+    e = be.array(rng.standard_normal((n, 96)).astype(np.float32))
+    got = []
+    for _ in range(3):
+        dw = be.empty((600, 96))
+        be.compound_bprop_lut(1, ids, e.T, None, dw)
+        got.append(dw.get())
+    assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+
+
+def test_lookup_gradient_on_neon_s_layer_call(b200):
+    """The statements of neon's lookup layer: take in the forward pass, then the gradient."""
+    be = b200
+    rng = np.random.RandomState(4)
+    w = rng.standard_normal((50, 12)).astype(np.float32)
+    ids = rng.randint(0, 50, 64).astype(np.int32)
+    inputs, table = be.array(ids.reshape(-1, 1), dtype=np.int32), be.array(w)
+    out_t = be.empty((64, 12))
+    out_t[:] = table.take(inputs, axis=0)
+    out = be.empty((12, 64))
+    be.compound_fprop_lut(inputs, table, out)
+    assert np.array_equal(out.get(), out_t.get().T)
+    e = rng.standard_normal((12, 64)).astype(np.float32)
+    dw, error, error_t = be.zeros((50, 12)), be.array(e), be.empty((64, 12))
+    be.compound_bprop_lut(4, inputs, error, error_t, dW=dw, pad_idx=0, alpha=1.0, beta=0)
+    assert np.array_equal(error_t.get(), e.T)
+    ref.check("dW", dw.get(), ref.lut_bprop(ids, e, w, 0, 1.0, 0.0, np.float32)["dW"])
+
+
+# ---------------------------------------------------------------- costs on logits
+COST_SIZES = [(1, 1, 1), (2, 3, 2), (31, 20, 5), (64, 33, 64), (257, 9, 100), (1000, 40, 1), (1024, 64, 7), (5003, 11, 50),
+              (8192, 5, 32), (32000, 3, 128), (70001, 2, 64), (140000, 2, 9)]
+
+
+def distill_inputs(v, n, k, dtype, seed=0):
+    rng = np.random.RandomState(seed + v + 7 * n + k)
+    z = (rng.standard_normal((v, n)) * 3).astype(dtype)
+    ids = np.stack([rng.permutation(v)[np.arange(k) % v] for _ in range(n)], axis=1).astype(np.int32)
+    top = (np.take_along_axis(z.astype(np.float32), ids, 0) + rng.standard_normal((k, n))).astype(dtype)
+    w = rng.uniform(0.5, 2, (1, n)).astype(np.float32)
+    return z, ids, top, w
+
+
+def run_distill(be, z, ids, top, w, temp, dtype, order, grad=True, inplace=False, top_order=None):
+    hz = Held(be, z, dtype, order)
+    hd = hz if inplace else Held(be, nan_like(z.shape), dtype, order) if grad else None
+    n = z.shape[1]
+    cost = vector(be, nan_like((1, n)))
+    held = [Held(be, ids, np.int32, top_order or order), Held(be, top, top.dtype, top_order or order)]
+    be.compound_distill(hz.view, held[0].view, held[1].view, cost, hd.view if hd else None,
+                        None if w is None else vector(be, w), temp)
+    got = {"cost": cost.get()}
+    if hd:
+        got["delta"] = hd.get()
+    return got
+
+
+@pytest.mark.parametrize("v,n,k", COST_SIZES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: np.dtype(d).name)
+def test_distill_sizes_and_orders(b200, v, n, k, dtype):
+    z, ids, top, w = distill_inputs(v, n, k, dtype)
+    for i, order in enumerate(ORDERS):
+        temp = [1.0, 2.5, 0.7][i % 3]
+        got = run_distill(b200, z, ids, top, w if i % 2 else None, temp, dtype, order, grad=i != 4,
+                          top_order=ORDERS[(i * 2) % 5])
+        compare(got, ref.distill(z, ids, top, w if i % 2 else None, temp, dtype))
+
+
+@pytest.mark.parametrize("order", ["rows", "cols", "shifted"])
+@pytest.mark.parametrize("v", [70, 3000, 150000])
+def test_distill_in_place(b200, v, order):
+    z, ids, top, w = distill_inputs(v, 4, 20, bf16)
+    got = run_distill(b200, z, ids, top, w, 2.0, bf16, order, inplace=True)
+    compare(got, ref.distill(z, ids, top, w, 2.0, bf16))
+
+
+@pytest.mark.parametrize("order", ["rows", "cols", "strided"])
+@pytest.mark.parametrize("v", [300, 40000])
+def test_distill_masks(b200, v, order):
+    n, k = 12, 6
+    z, ids, top, w = distill_inputs(v, n, k, np.float32)
+    low = np.finfo(np.float32).min
+    w[0, 0] = 0
+    z[:, 0] = np.nan                                 # a masked item may hold anything
+    w[0, 1] = 0
+    z[3, 1], top[0, 1] = np.inf, np.nan
+    ids[:, 2] = -1                                   # no usable entry
+    top[:, 3] = -np.inf
+    ids[0, 4], ids[1, 4] = v, 2 ** 31 - 1            # some entries outside
+    top[2:, 5] = -np.inf
+    top[1:, 6] = low                                 # masked with the lowest value
+    z[v // 2:, 7] = -np.inf                          # masked words
+    ids[:, 7] = np.arange(k)
+    z[v // 2:, 8] = low
+    ids[:, 8] = np.arange(k)
+    ids[:, 9] = ids[0, 9]                            # one word in every entry
+    ids[3:, 10] = ids[:3, 10]
+    z[:, 11] = z[0, 11]                              # all logits alike
+    for inplace in (False, True):
+        got = run_distill(b200, z, ids, top, w, 1.5, np.float32, order, inplace=inplace)
+        compare(got, ref.distill(z, ids, top, w, 1.5, np.float32))
+    # the teacher's mass on a word the student has ruled out; a bad logit in one item only
+    z, ids, top, w = distill_inputs(v, 4, k, np.float32, seed=5)
+    z[ids[0, 1], 1], z[5, 2] = -np.inf, np.nan
+    got = run_distill(b200, z, ids, top, w, 1.0, np.float32, order)
+    assert got["cost"][0, 1] == np.inf and np.isnan(got["cost"][0, 2]) and np.isnan(got["delta"][:, 2]).all()
+    keep = [0, 3]
+    want = ref.distill(z[:, keep], ids[:, keep], top[:, keep], w[:, keep], 1.0, np.float32)
+    compare({"cost": got["cost"][:, keep], "delta": got["delta"][:, keep]}, want)
+
+
+def test_distill_most_entries(b200):
+    z, ids, top, w = distill_inputs(5000, 3, 1024, np.float32)
+    compare(run_distill(b200, z, ids, top, w, 1.0, np.float32, "rows"), ref.distill(z, ids, top, w, 1.0, np.float32))
+    z, ids, top, w = distill_inputs(40, 3, 1024, np.float32)                 # every word many times
+    compare(run_distill(b200, z, ids, top, w, 1.0, np.float32, "cols"), ref.distill(z, ids, top, w, 1.0, np.float32))
+
+
+def policy_inputs(v, n, dtype, seed=0):
+    rng = np.random.RandomState(seed + v + 3 * n)
+    z = (rng.standard_normal((v, n)) * 3).astype(dtype)
+    act = rng.randint(0, v, (1, n)).astype(np.int32)
+    logp = np.take_along_axis(ref._log_softmax(z.astype(np.float64))[0], act, 0)
+    # ratios on both sides of both borders of the clip, none within 2 % of one
+    ratio = rng.choice([0.5, 0.75, 0.85, 1.0, 1.1, 1.15, 1.35, 2.0], (1, n))
+    old = (logp - np.log(ratio)).astype(np.float32)
+    new_ref = (logp + rng.standard_normal((1, n)) * 0.3).astype(np.float32)
+    adv = rng.standard_normal((1, n)).astype(np.float32)
+    w = rng.uniform(0.5, 2, (1, n)).astype(np.float32)
+    return z, act, old, new_ref, adv, w
+
+
+def run_policy(be, z, act, old, new_ref, adv, w, dtype, order, clip=(0.2, 0.28), kl=0.05, grad=True, inplace=False,
+               logp=True):
+    n = z.shape[1]
+    hz = Held(be, z, dtype, order)
+    hd = hz if inplace else Held(be, nan_like(z.shape), dtype, order) if grad else None
+    cost, lp = vector(be, nan_like((1, n))), vector(be, nan_like((1, n))) if logp else None
+    be.compound_policy(hz.view, be.array(act, dtype=np.int32), vector(be, old), vector(be, adv), cost,
+                       hd.view if hd else None, logp=lp, ref_logp=None if new_ref is None else vector(be, new_ref),
+                       weights=None if w is None else vector(be, w), clip=clip, kl_coef=kl)
+    got = {"cost": cost.get()}
+    if logp:
+        got["logp"] = lp.get()
+    if hd:
+        got["delta"] = hd.get()
+    return got
+
+
+@pytest.mark.parametrize("v,n,k", COST_SIZES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: np.dtype(d).name)
+def test_policy_sizes_and_orders(b200, v, n, k, dtype):
+    z, act, old, new_ref, adv, w = policy_inputs(v, n, dtype)
+    for i, order in enumerate(ORDERS):
+        kl = [0.05, 0.0][i % 2]
+        weights = w if i % 3 else None
+        got = run_policy(b200, z, act, old, new_ref if kl else None, adv, weights, dtype, order, kl=kl, grad=i != 3,
+                         logp=i != 2)
+        compare(got, ref.policy(z, act, old, new_ref, adv, weights, 0.2, 0.28, kl, dtype))
+
+
+@pytest.mark.parametrize("order", ["rows", "cols", "strided"])
+@pytest.mark.parametrize("v", [300, 40000, 150000])
+def test_policy_masks_and_in_place(b200, v, order):
+    n = 10
+    z, act, old, new_ref, adv, w = policy_inputs(v, n, np.float32)
+    w[0, 0] = 0
+    z[7, 0] = np.nan                                 # masked
+    act[0, 0] = 3
+    act[0, 1], act[0, 2], act[0, 3] = -1, v, -2 ** 31
+    z[:, 1] = np.nan
+    adv[0, 4] = 0
+    z[v // 2:, 5] = -np.inf
+    act[0, 5] = 1
+    for inplace in (False, True):
+        got = run_policy(b200, z, act, old, new_ref, adv, w, np.float32, order, inplace=inplace)
+        want = ref.policy(z, act, old, new_ref, adv, w, 0.2, 0.28, 0.05, np.float32)
+        assert np.isnan(got["logp"][0, 0])           # asked for, and the logits hold NaN
+        got["logp"], want["logp"] = got["logp"][:, 1:], tuple(a[:, 1:] for a in want["logp"])
+        compare(got, want)
+    got = run_policy(b200, z, act, old, new_ref, adv, w, np.float32, order, logp=False)
+    compare(got, {k: want[k] for k in ("cost", "delta")})
+
+
+def test_costs_no_items(b200):
+    be = b200
+    empty = be.empty((9, 0))
+    be.compound_distill(empty, be.empty((2, 0), dtype=np.int32), be.empty((2, 0)), be.empty((1, 0)), be.empty((9, 0)))
+    be.compound_policy(empty, be.empty((1, 0), dtype=np.int32), be.empty((1, 0)), be.empty((1, 0)), be.empty((1, 0)))
+
+
+@pytest.mark.parametrize("which", ["distill", "policy"])
+def test_cost_gradient_against_differences(b200, which):
+    v, n, step = 30, 4, 1e-5
+    rng = np.random.RandomState(9)
+    if which == "distill":
+        z, ids, top, w = distill_inputs(v, n, 5, np.float32)
+        got = run_distill(b200, z, ids, top, w, 1.5, np.float32, "rows")
+        loss = lambda z64: ref.distill(z64, ids, top, w, 1.5, np.float32)["cost"][0].sum()          # noqa: E731
+    else:
+        z, act, old, new_ref, adv, w = policy_inputs(v, n, np.float32)
+        got = run_policy(b200, z, act, old, new_ref, adv, w, np.float32, "rows")
+        loss = lambda z64: ref.policy(z64, act, old, new_ref, adv, w, 0.2, 0.28, 0.05, np.float32)["cost"][0].sum()   # noqa: E731
+    z = z.astype(np.float64)
+    for _ in range(30):
+        at = (rng.randint(v), rng.randint(n))
+        up, down = z.copy(), z.copy()
+        up[at] += step
+        down[at] -= step
+        slope = (loss(up) - loss(down)) / (2 * step)
+        assert abs(got["delta"][at] - slope) < 1e-4 * max(1.0, abs(slope)), at
+
+
+# ---------------------------------------------------------------- together
+class TinyModel(object):
+    """table -> layer norm -> output matrix -> distillation or policy cost, and the way back."""
+
+    def __init__(self, be, order, v=64, f=32, n=24, seed=0):
+        rng = np.random.RandomState(seed)
+        self.be, self.v, self.f, self.n, self.order = be, v, f, n, order
+        self.host = {"W": rng.standard_normal((v, f)), "gamma": rng.uniform(0.5, 1.5, (f, 1)),
+                     "beta": rng.uniform(-0.5, 0.5, (f, 1)), "out": rng.standard_normal((v, f)) * 0.3}
+        self.host = {k: a.astype(np.float32) for k, a in self.host.items()}
+        self.ids = rng.randint(0, v, (1, n)).astype(np.int32)
+        self.top_ids = np.stack([rng.permutation(v)[:4] for _ in range(n)], axis=1).astype(np.int32)
+        self.top = rng.standard_normal((4, n)).astype(np.float32)
+        self.w = (rng.rand(1, n) < 0.8).astype(np.float32) / n
+        self.p = {k: be.array(a) for k, a in self.host.items()}
+        self.d = {k: be.array(nan_like(a.shape)) for k, a in self.host.items()}
+        mat = lambda r: be.empty((n, r)).T if order == "rows" else be.empty((r, n))             # noqa: E731
+        self.h, self.y, self.z = mat(f), mat(f), mat(v)
+        self.dy, self.dh, self.error_t = mat(f), mat(f), be.empty((n, f))
+        self.mean, self.rstd, self.cost = be.empty((1, n)), be.empty((1, n)), be.empty((1, n))
+        self.dev = [be.array(self.ids, dtype=np.int32), be.array(self.top_ids, dtype=np.int32), be.array(self.top),
+                    be.array(self.w)]
+
+    def step(self):
+        be, p, d = self.be, self.p, self.d
+        ids, top_ids, top, w = self.dev
+        be.compound_fprop_lut(ids, p["W"], self.h, scale=self.f ** 0.5)
+        be.compound_fprop_ln(self.h, self.mean, self.rstd, p["gamma"], p["beta"], self.y)
+        be.compound_dot(p["out"], self.y, self.z)
+        be.compound_distill(self.z, top_ids, top, self.cost, self.z, weights=w, temperature=2.0)
+        be.compound_dot(self.z, self.y.T, d["out"])
+        be.compound_dot(p["out"].T, self.z, self.dy)
+        be.compound_bprop_ln(self.dh, d["gamma"], d["beta"], self.dy, self.h, self.mean, self.rstd, p["gamma"])
+        be.compound_bprop_lut(1, ids, self.dh, self.error_t, d["W"], alpha=self.f ** 0.5)
+
+    def loss(self, host):
+        h = host["W"][self.ids[0]].T * self.f ** 0.5
+        y = ref.ln_fprop(h, host["gamma"], host["beta"], 1e-5, np.float32)["y"][0]
+        return ref.distill(host["out"] @ y, self.top_ids, self.top, self.w, 2.0, np.float32)["cost"][0].sum()
+
+
+@pytest.mark.parametrize("order", ["rows", "cols"])
+def test_operators_together_against_differences(b200, order):
+    model = TinyModel(b200, order)
+    model.step()
+    host = {k: a.astype(np.float64) for k, a in model.host.items()}
+    assert abs(model.cost.get().sum() - model.loss(host)) < 1e-5
+    rng, step = np.random.RandomState(1), 1e-5
+    for name in ("W", "gamma", "beta", "out"):
+        got = model.d[name].get()
+        for _ in range(8):
+            at = (int(model.ids[0, rng.randint(model.n)]) if name == "W" else rng.randint(got.shape[0]), rng.randint(got.shape[1]))
+            slopes = []
+            for sign in (1, -1):
+                moved = {k: a.copy() for k, a in host.items()}
+                moved[name][at] += sign * step
+                slopes.append(model.loss(moved))
+            slope = (slopes[0] - slopes[1]) / (2 * step)
+            assert abs(got[at] - slope) < 1e-5 + 1e-4 * abs(slope), (name, at)
+
+
+def test_operators_recorded_and_replayed(b200):
+    """Two recorded steps that share the backend's scratch, replayed between eager statements."""
+    be = b200
+    models = [TinyModel(be, "rows", seed=1), TinyModel(be, "cols", v=700, f=40, n=300, seed=2)]
+    graphs, want = [], []
+    for m in models:
+        m.step()
+        want.append({k: t.get() for k, t in m.d.items()})
+        graphs.append(be.capture(m.step))
+    for m in models:
+        for t in m.d.values():
+            t[:] = float("nan")
+    total = be.empty((1, 1))
+    for _ in range(2):
+        for i in (1, 0):
+            graphs[i].replay()
+            total[:] = be.sum(models[i].cost)
+    for m, w in zip(models, want):
+        for k in w:
+            assert np.array_equal(m.d[k].get(), w[k]), k
