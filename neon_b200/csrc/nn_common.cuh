@@ -140,4 +140,38 @@ DEV float block_max(float v, float* s) {
     return warp_max(lane < warps ? s[lane] : -INFINITY);
 }
 
+// The same with one barrier: `s` holds 64 floats, `turn` alternates from call to call, so that a
+// buffer is written again only after every thread has passed the barrier of the call in between.
+DEV float block_sum_turn(float v, float* s, int& turn) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
+    v = warp_sum(v);
+    if (lane == 0) s[turn * 32 + warp] = v;
+    __syncthreads();
+    v = warp_sum(lane < warps ? s[turn * 32 + lane] : 0.f);
+    turn ^= 1;
+    return v;
+}
+DEV float2 block_sum2_turn(float a, float b, float2* s, int& turn) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if (lane == 0) s[turn * 32 + warp] = make_float2(a, b);
+    __syncthreads();
+    const float2 t = lane < warps ? s[turn * 32 + lane] : make_float2(0.f, 0.f);
+    turn ^= 1;
+    return make_float2(warp_sum(t.x), warp_sum(t.y));
+}
+
+// Blocks of a kernel that can be resident at once, over all SMs.
+template <typename K> inline int resident_blocks(K kernel, int threads, int smem) {
+    static thread_local int sms = 0;
+    if (!sms) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
+    }
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
+    return n * sms;
+}
+
 }  // namespace nn
