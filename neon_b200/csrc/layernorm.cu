@@ -105,289 +105,346 @@ __global__ void __launch_bounds__(256) ln_grads_any(const __grid_constant__ LnGr
 
 // ---- features of an item next to each other (their stride is 1)
 //
-// An item lives in registers: every thread holds NV vectors of V elements of it, so x is read
-// once for the mean, the centred variance and the result.  Blocks are persistent: gamma and beta
-// (and, backwards, the sums for their gradients) stay in registers from item to item, and the
-// next item is loaded while this one is worked on.  WARP: a warp per item instead of a block, for
-// items that fit into the registers of one.
-template <int DT, int V, int NV> struct Slice {
-    static constexpr int W = (dt_size<DT>::value * V + 3) / 4;
-    u32 w[NV][W];
-    DEV void load(u64 base, i64 at, int me, int T, int F) {
+// A group of T threads (one warp, or a whole block) works on one item, of which every thread holds
+// NV 16-byte vectors; blocks are persistent, so gamma and beta, and backwards the sums for their
+// gradients, stay in the registers of the thread that owns the feature.  Items come through a ring
+// of RING items in shared memory, filled by asynchronous copies: a thread reads only what it
+// copied itself, so the ring needs no barrier, and RING - 1 items are under way whatever the
+// registers hold.  x (and the error) are read once.
+//
+// An item's vectors start at the 16-byte boundary at or before it, `mis` elements early; elements
+// outside the item are masked and the vectors at its ends stored element by element, so odd widths
+// and pitches run at nearly the speed of even ones.  A group's items are a multiple of 8 apart
+// then (MIS), so `mis`, and with it the features a thread owns, are the same for all of them.
+// Clears the elements of a vector that lie outside [0, F); its first is element f.
+template <int DT, int V> DEV void mask(u32* w, int f, int F) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int f = (j * T + me) * V;
-            if (f < F) ld_w<DT, V, false>(base, at + f, w[j]);
-        }
+    for (int i = 0; i < V; ++i) {
+        if ((unsigned)(f + i) < (unsigned)F) continue;
+        if (dt_size<DT>::value == 4) w[i] = 0;
+        else w[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u;
     }
-    DEV void get(int j, float* v) const { cvt_in<DT, V>(w[j], v); }
-};
-
-template <int V, int NV> DEV void load_params(u64 base, int dt, float fill, int me, int T, int F, float (&v)[NV][V]) {
+}
+// Stores a vector at element f of an item, leaving out what lies outside [0, F).
+template <int DT, int V, bool MIS> DEV void put(u64 base, i64 item, int f, int F, const u32* w) {
+    if (!MIS || (f >= 0 && f + V <= F)) { st_raw<16>(reinterpret_cast<char*>(base) + (item + f) * dt_size<DT>::value, w); return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if ((unsigned)(f + i) >= (unsigned)F) continue;
+        if constexpr (dt_size<DT>::value == 4) reinterpret_cast<u32*>(base)[item + f + i] = w[i];
+        else reinterpret_cast<u16*>(base)[item + f + i] = (u16)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]);
+    }
+}
+// The parameters of a thread's features.
+template <int V, int NV> DEV void load_params(u64 base, int dt, float fill, int me, int T, int mis, int F, f32x2 (&v)[NV][V / 2]) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int f = (j * T + me) * V + i;
-            v[j][i] = base && f < F ? ld_any(base, f, dt) : fill;
+        for (int k = 0; k < V / 2; ++k) {
+            const int f = (j * T + me) * V - mis + 2 * k;
+            v[j][k] = pair(base && (unsigned)f < (unsigned)F ? ld_any(base, f, dt) : fill,
+                           base && (unsigned)(f + 1) < (unsigned)F ? ld_any(base, f + 1, dt) : fill);
         }
 }
 
-template <bool WARP> DEV float item_sum(float v, float* s, int& turn) {
-    if constexpr (WARP) return warp_sum(v);
-    else return block_sum_turn(v, s, turn);
-}
-template <bool WARP> DEV float2 item_sum2(float a, float b, float2* s, int& turn) {
-    if constexpr (WARP) return make_float2(warp_sum(a), warp_sum(b));
-    else return block_sum2_turn(a, b, s, turn);
-}
-
-template <int DT, int V, int NV, bool WARP, int MAXT>
-__global__ void __launch_bounds__(MAXT) ln_fprop_rows(const __grid_constant__ LnP p) {
+// The variance is a second walk over the item's registers, so there are two barriers per item;
+// slices are wide (32 elements of 16 bits) because few warps per group wait less at them: at
+// 4096 x 32768 bf16, 128 threads with 4 vectors each take 96 us, 256 with 2 take 112.
+template <int DT, int NV, int RING, bool MIS, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) ln_fprop_rows(const __grid_constant__ LnP p, int T) {
+    constexpr int V = 16 / dt_size<DT>::value, W = 4;
+    extern __shared__ __align__(16) u32 ring[];        // [RING][NV][blockDim.x][W]
     __shared__ float s[64];
-    const int T = WARP ? 32 : blockDim.x, me = WARP ? threadIdx.x & 31 : threadIdx.x, F = (int)p.F;
-    const i64 step = WARP ? (i64)gridDim.x * 8 : gridDim.x;
-    i64 n = WARP ? (i64)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
-    if (n >= p.N) return;                              // whole warps, or whole blocks
-    const float inv = 1.f / (float)F;
-    int turn = 0;
-    Slice<DT, V, NV> cur, next;
-    cur.load(p.x, n * p.x1, me, T, F);
-    float gamma[NV][V], beta[NV][V];
-    load_params<V, NV>(p.gamma, p.pdt, 1.f, me, T, F, gamma);
-    load_params<V, NV>(p.beta, p.pdt, 0.f, me, T, F, beta);
-    for (; n < p.N; n += step) {
-        if (n + step < p.N) next.load(p.x, (n + step) * p.x1, me, T, F);
-        float x[NV][V], a = 0.f;
+    const int F = (int)p.F, group = threadIdx.x / T, me = threadIdx.x % T, groups = blockDim.x / T;
+    const i64 step = (i64)gridDim.x * groups, first = (i64)blockIdx.x * groups + group;
+    int mis = 0;
+    if constexpr (MIS) mis = (int)((p.x / dt_size<DT>::value + (u64)(first * p.x1)) % V);
+    const u32 mine = (u32)__cvta_generic_to_shared(ring) + threadIdx.x * 16, slot = blockDim.x * 16;
+    auto fetch = [&](i64 item, int stage) {
+        if (item < p.N) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            cur.get(j, x[j]);
-            if ((j * T + me) * V < F) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) a += x[j][i];
+            for (int j = 0; j < NV; ++j) {
+                const int f = (j * T + me) * V - mis;
+                if (f < F) copy16(mine + (stage * NV + j) * slot, p.x + (u64)((item * p.x1 + f) * dt_size<DT>::value));
             }
         }
-        const float mean = item_sum<WARP>(a, s, turn) * inv;
-        a = 0.f;
+        copy_commit();
+    };
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if ((j * T + me) * V < F) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) { x[j][i] -= mean; a = fmaf(x[j][i], x[j][i], a); }
-            }
-        const float rstd = 1.f / sqrtf(item_sum<WARP>(a, s, turn) * inv + p.eps);
+    for (int k = 0; k < RING - 1; ++k) fetch(first + k * step, k);
+    f32x2 gamma[NV][V / 2], beta[NV][V / 2];
+    load_params<V, NV>(p.gamma, p.pdt, 1.f, me, T, mis, F, gamma);
+    load_params<V, NV>(p.beta, p.pdt, 0.f, me, T, mis, F, beta);
+    const float inv = 1.f / (float)F;
+    int turn = 0, stage = 0;
+    for (i64 n = first; n < p.N; n += step) {
+        fetch(n + (RING - 1) * step, stage == 0 ? RING - 1 : stage - 1);
+        copy_wait<RING - 1>();
+        u32 w[NV][W];
+        f32x2 sum = 0;                                 // two sums of zero
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int f = (j * T + me) * V;
+            const int f = (j * T + me) * V - mis;
+            if (f >= F) continue;
+            ld_raw<16, false>(reinterpret_cast<const char*>(ring + ((stage * NV + j) * blockDim.x + threadIdx.x) * W), w[j]);
+            if constexpr (MIS) if (f < 0 || f + V > F) mask<DT, V>(w[j], f, F);
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) sum = add2(sum, get2<DT>(w[j], k));
+        }
+        const float mean = group_sum(both(sum), s, turn, T, 1) * inv;
+        sum = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int f = (j * T + me) * V - mis;
             if (f >= F) continue;
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[j][i] = fmaf(x[j][i] * rstd, gamma[j][i], beta[j][i]);
-            st_f<DT, V>(p.out, n * p.o1 + f, x[j]);
+            for (int k = 0; k < V / 2; ++k) {
+                f32x2 d = less2<DT>(w[j], k, mean);
+                if constexpr (MIS) {                   // elements before the item or behind it
+                    float lo, hi;
+                    split(d, lo, hi);
+                    if ((unsigned)(f + 2 * k) >= (unsigned)F) lo = 0.f;
+                    if ((unsigned)(f + 2 * k + 1) >= (unsigned)F) hi = 0.f;
+                    d = pair(lo, hi);
+                }
+                sum = fma2(d, d, sum);
+            }
+        }
+        const float rstd = 1.f / sqrtf(group_sum(both(sum), s, turn, T, 1) * inv + p.eps);
+        const f32x2 scale = pair(rstd, rstd);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int f = (j * T + me) * V - mis;
+            if (f >= F) continue;
+            u32 y[W];
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) set2<DT>(y, k, fma2(mul2(less2<DT>(w[j], k, mean), scale), gamma[j][k], beta[j][k]));
+            put<DT, V, MIS>(p.out, n * p.o1, f, F, y);
         }
         if (me == 0) {
             if (p.mean) reinterpret_cast<float*>(p.mean)[n] = mean;
             if (p.rstd) reinterpret_cast<float*>(p.rstd)[n] = rstd;
         }
-        cur = next;
+        stage = stage == RING - 1 ? 0 : stage + 1;
     }
 }
 
-// part[block][0][F]: the block's share of grad_gamma, part[block][1][F]: of grad_beta
-template <int DT, int V, int NV, bool WARP, int MAXT>
-__global__ void __launch_bounds__(MAXT) ln_bprop_rows(const __grid_constant__ LnP p, float* part) {
+// One barrier per item, for both sums at once.
+// part[block][0][F]: the block's share of grad_gamma, part[block][1][F]: of grad_beta.
+template <int DT, int NV, int RING, bool MIS, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) ln_bprop_rows(const __grid_constant__ LnP p, float* part, int T) {
+    constexpr int V = 16 / dt_size<DT>::value, W = 4;
+    extern __shared__ __align__(16) u32 ring[];        // [RING][2][NV][blockDim.x][W]
     __shared__ float2 s[64];
-    const int T = WARP ? 32 : blockDim.x, me = WARP ? threadIdx.x & 31 : threadIdx.x, F = (int)p.F;
-    const i64 step = WARP ? (i64)gridDim.x * 8 : gridDim.x;
-    i64 n = WARP ? (i64)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
-    const float inv = 1.f / (float)F;
-    int turn = 0;
-    Slice<DT, V, NV> x, e, nx, ne;
-    float mean = 0.f, rstd = 0.f;
-    if (n < p.N) {
-        x.load(p.x, n * p.x1, me, T, F);
-        e.load(p.e, n * p.e1, me, T, F);
-        mean = reinterpret_cast<const float*>(p.mean)[n];
-        rstd = reinterpret_cast<const float*>(p.rstd)[n];
-    }
-    float gamma[NV][V], gg[NV][V], gb[NV][V];
-    load_params<V, NV>(p.gamma, p.pdt, 1.f, me, T, F, gamma);
+    const int F = (int)p.F, group = threadIdx.x / T, me = threadIdx.x % T, groups = blockDim.x / T;
+    const i64 step = (i64)gridDim.x * groups, first = (i64)blockIdx.x * groups + group;
+    int mis = 0;
+    if constexpr (MIS) mis = (int)((p.x / dt_size<DT>::value + (u64)(first * p.x1)) % V);
+    const u32 mine = (u32)__cvta_generic_to_shared(ring) + threadIdx.x * 16, slot = blockDim.x * 16;
+    auto fetch = [&](i64 item, int stage) {
+        if (item < p.N) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int f = (j * T + me) * V - mis;
+                if (f >= F) continue;
+                copy16(mine + ((stage * 2 + 0) * NV + j) * slot, p.x + (u64)((item * p.x1 + f) * dt_size<DT>::value));
+                copy16(mine + ((stage * 2 + 1) * NV + j) * slot, p.e + (u64)((item * p.e1 + f) * dt_size<DT>::value));
+            }
+        }
+        copy_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < RING - 1; ++k) fetch(first + k * step, k);
+    f32x2 gamma[NV][V / 2], gg[NV][V / 2], gb[NV][V / 2];
+    load_params<V, NV>(p.gamma, p.pdt, 1.f, me, T, mis, F, gamma);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) gg[j][i] = gb[j][i] = 0.f;
-    for (; n < p.N; n += step) {
-        float nmean = 0.f, nrstd = 0.f;
-        if (n + step < p.N) {
-            nx.load(p.x, (n + step) * p.x1, me, T, F);
-            ne.load(p.e, (n + step) * p.e1, me, T, F);
-            nmean = reinterpret_cast<const float*>(p.mean)[n + step];
-            nrstd = reinterpret_cast<const float*>(p.rstd)[n + step];
-        }
-        float a = 0.f, b = 0.f;
+        for (int k = 0; k < V / 2; ++k) gg[j][k] = gb[j][k] = 0;
+    const float inv = 1.f / (float)F;
+    int turn = 0, stage = 0;
+    const float *means = reinterpret_cast<const float*>(p.mean), *rstds = reinterpret_cast<const float*>(p.rstd);
+    float mean = first < p.N ? means[first] : 0.f, rstd = first < p.N ? rstds[first] : 0.f;
+    for (i64 n = first; n < p.N; n += step) {
+        float mean_next = 0.f, rstd_next = 0.f;
+        if (n + step < p.N) { mean_next = means[n + step]; rstd_next = rstds[n + step]; }
+        fetch(n + (RING - 1) * step, stage == 0 ? RING - 1 : stage - 1);
+        copy_wait<RING - 1>();
+        f32x2 h[NV][V / 2], g[NV][V / 2], a2 = 0, b2 = 0;
+        const f32x2 scale = pair(rstd, rstd);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            if ((j * T + me) * V >= F) continue;
-            float h[V], g[V];
-            x.get(j, h);
-            e.get(j, g);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                h[i] = (h[i] - mean) * rstd;
-                gg[j][i] = fmaf(g[i], h[i], gg[j][i]);
-                gb[j][i] += g[i];
-                g[i] *= gamma[j][i];
-                a += g[i];
-                b = fmaf(g[i], h[i], b);
-            }
-        }
-        const float2 ab = item_sum2<WARP>(a, b, s, turn);
-        a = ab.x * inv;
-        b = ab.y * inv;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int f = (j * T + me) * V;
+            const int f = (j * T + me) * V - mis;
             if (f >= F) continue;
-            float h[V], g[V];
-            x.get(j, h);
-            e.get(j, g);
+            const u32* at = ring + (((stage * 2) * NV + j) * blockDim.x + threadIdx.x) * W;
+            u32 x[W], e[W];
+            ld_raw<16, false>(reinterpret_cast<const char*>(at), x);
+            ld_raw<16, false>(reinterpret_cast<const char*>(at + NV * blockDim.x * W), e);
+            if constexpr (MIS) if (f < 0 || f + V > F) { mask<DT, V>(x, f, F); mask<DT, V>(e, f, F); }   // an error of 0 adds nothing
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                h[i] = (h[i] - mean) * rstd;
-                g[i] = rstd * (g[i] * gamma[j][i] - a - h[i] * b);
+            for (int k = 0; k < V / 2; ++k) {
+                h[j][k] = mul2(less2<DT>(x, k, mean), scale);
+                g[j][k] = get2<DT>(e, k);
+                gg[j][k] = fma2(g[j][k], h[j][k], gg[j][k]);
+                gb[j][k] = add2(g[j][k], gb[j][k]);
+                g[j][k] = mul2(g[j][k], gamma[j][k]);
+                a2 = add2(a2, g[j][k]);
+                b2 = fma2(g[j][k], h[j][k], b2);
             }
-            st_f<DT, V>(p.out, n * p.o1 + f, g);
         }
-        x = nx; e = ne; mean = nmean; rstd = nrstd;
+        const float2 ab = group_sum2(both(a2), both(b2), s, turn, T, 1);
+        const f32x2 a = pair(-ab.x * inv, -ab.x * inv), b = pair(-ab.y * inv, -ab.y * inv);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int f = (j * T + me) * V - mis;
+            if (f >= F) continue;
+            u32 d[W];
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) set2<DT>(d, k, mul2(scale, fma2(h[j][k], b, add2(g[j][k], a))));
+            put<DT, V, MIS>(p.out, n * p.o1, f, F, d);
+        }
+        stage = stage == RING - 1 ? 0 : stage + 1;
+        mean = mean_next;
+        rstd = rstd_next;
     }
     if (!part) return;
-    if constexpr (WARP) {
-        // the warps of a block one after the other, in shared memory
-        extern __shared__ float acc[];                 // [2][F]
-        for (int w = 0; w < 8; ++w) {
-            if ((threadIdx.x >> 5) == w) {
-#pragma unroll
-                for (int j = 0; j < NV; ++j)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const int f = (j * T + me) * V + i;
-                        if (f >= F) continue;
-                        acc[f] = (w ? acc[f] : 0.f) + gg[j][i];
-                        acc[F + f] = (w ? acc[F + f] : 0.f) + gb[j][i];
-                    }
-            }
+    if (T == 32) {
+        // the warps of a block one after the other, where the ring was: all copies have been read
+        float* acc = reinterpret_cast<float*>(ring);   // [2][F], F <= 32 NV V
+        for (int g = 0; g < groups; ++g) {
             __syncthreads();
+            if (group != g) continue;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int k = 0; k < V / 2; ++k) {
+                    float v[4];
+                    split(gg[j][k], v[0], v[1]);
+                    split(gb[j][k], v[2], v[3]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int f = (j * T + me) * V - mis + 2 * k + i;
+                        if ((unsigned)f >= (unsigned)F) continue;
+                        acc[f] = (g ? acc[f] : 0.f) + v[i];
+                        acc[F + f] = (g ? acc[F + f] : 0.f) + v[2 + i];
+                    }
+                }
         }
-        for (int f = threadIdx.x; f < 2 * F; f += 256) part[(i64)blockIdx.x * 2 * F + f] = acc[f];
-    } else {
-        float* to = part + (i64)blockIdx.x * 2 * F;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int f = (j * T + me) * V + i;
-                if (f < F) { to[f] = gg[j][i]; to[F + f] = gb[j][i]; }
-            }
+        __syncthreads();
+        for (int f = threadIdx.x; f < 2 * F; f += blockDim.x) part[(i64)blockIdx.x * 2 * F + f] = acc[f];
+        return;
     }
+    float* to = part + (i64)blockIdx.x * 2 * F;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < V / 2; ++k) {
+            const int f = (j * T + me) * V - mis + 2 * k;
+            float lo, hi;
+            split(gg[j][k], lo, hi);
+            if ((unsigned)f < (unsigned)F) to[f] = lo;
+            if ((unsigned)(f + 1) < (unsigned)F) to[f + 1] = hi;
+            split(gb[j][k], lo, hi);
+            if ((unsigned)f < (unsigned)F) to[F + f] = lo;
+            if ((unsigned)(f + 1) < (unsigned)F) to[F + f + 1] = hi;
+        }
 }
 
-// The sum of the blocks' shares, in the order of the blocks within each of 32 rows of threads.
-__global__ void __launch_bounds__(1024) ln_sum_parts(const float* part, int blocks, i64 F, u64 ggamma, u64 gbeta, int pdt) {
-    __shared__ float s[32][33];
-    const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
-    const i64 c = (i64)blockIdx.x * 32 + lane;          // column of [grad_gamma | grad_beta]
+// The sum of the blocks' shares: 8 columns of [grad_gamma | grad_beta] per block (one sector of
+// every share), 128 rows of threads, each over its shares in their order.
+__global__ void __launch_bounds__(1024) ln_sum_parts(const float* part, int parts, i64 F, u64 ggamma, u64 gbeta, int pdt) {
+    __shared__ float s[32][8];
+    const i64 c = (i64)blockIdx.x * 8 + (threadIdx.x & 7);
     float a = 0.f;
-    if (c < 2 * F)
-        for (int b = row; b < blocks; b += 32) a += part[(i64)b * 2 * F + c];
-    s[row][lane] = a;
+    if (c < 2 * F) {
+#pragma unroll 4
+        for (int b = threadIdx.x >> 3; b < parts; b += 128) a += part[(i64)b * 2 * F + c];
+    }
+    a += __shfl_xor_sync(0xffffffffu, a, 8);
+    a += __shfl_xor_sync(0xffffffffu, a, 16);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane < 8) s[warp][lane] = a;
     __syncthreads();
-    a = warp_sum(s[lane][row]);
-    const i64 out = (i64)blockIdx.x * 32 + row;
+    if (warp >= 8) return;
+    a = warp_sum(s[lane][warp]);
+    const i64 out = (i64)blockIdx.x * 8 + warp;
     if (lane == 0 && out < 2 * F) {
         const u64 to = out < F ? ggamma : gbeta;
         if (to) st_any(to, out < F ? out : out - F, pdt, a);
     }
 }
 
-// Which of the register kernels an item of F features takes: T threads with NV vectors of V
-// elements each; a warp where `most` elements per lane hold an item.
-struct Rows { int V, NV, T; bool warp; };
 enum { kMaxRow = 16384 };
 
-inline bool rows_plan(i64 F, int V, int most, Rows& r) {
+// Whether the register kernels take the call: features next to each other, and at any item the
+// same distance to a 16-byte boundary in every matrix.  `mis`: that distance is not always 0, or
+// items end inside a vector.
+bool rows_fit(const b200_matrix* const* m, int count, i64 F, bool& mis) {
+    const i64 V = 16 / esize(m[0]->dtype);
+    mis = F % V != 0;
     if (F > kMaxRow) return false;
-    const int nvec = (int)((F + V - 1) / V);
-    r.V = V;
-    for (int nv = 1; nv * V <= most; nv *= 2)
-        if (nvec <= 32 * nv) { r.NV = nv; r.T = 32; r.warp = true; return true; }
-    r.warp = false;
-    for (r.NV = 1; r.NV * V <= 16; r.NV *= 2) {
-        r.T = ((nvec + r.NV - 1) / r.NV + 31) / 32 * 32;
-        if (r.T <= 512 || (r.NV * V == 16 && r.T <= 1024)) return true;
+    for (int i = 0; i < count; ++i) {
+        if (m[i]->s0 != 1 && F != 1) return false;
+        const i64 at = (i64)(m[i]->ptr / (uint64_t)esize(m[i]->dtype)) % V, pitch = ((m[i]->s1 % V) + V) % V;
+        if (at != (i64)(m[0]->ptr / (uint64_t)esize(m[0]->dtype)) % V || pitch != ((m[0]->s1 % V) + V) % V) return false;
+        mis = mis || at != 0 || pitch != 0;
     }
-    return false;
-}
-
-template <int DT, int V, int NV> cudaError_t launch_fprop(const LnP& p, const Rows& r, cudaStream_t s) {
-    const i64 want = r.warp ? (p.N + 7) / 8 : p.N;
-    auto go = [&](auto k, int threads) {
-        const i64 most = resident_blocks(k, threads, 0);
-        k<<<(unsigned)(want < most ? want : most), threads, 0, s>>>(p);
-        return cudaGetLastError();
-    };
-    if (r.warp) return go(ln_fprop_rows<DT, V, NV, true, 256>, 256);
-    if (r.T <= 512) return go(ln_fprop_rows<DT, V, NV, false, 512>, r.T);
-    if constexpr (V * NV == 16) return go(ln_fprop_rows<DT, V, NV, false, 1024>, r.T);
-    return cudaErrorInvalidValue;
-}
-template <int DT, int V> cudaError_t launch_fprop_v(const LnP& p, const Rows& r, cudaStream_t s) {
-    if (r.NV == 1) return launch_fprop<DT, V, 1>(p, r, s);
-    if (r.NV == 2) return launch_fprop<DT, V, 2>(p, r, s);
-    if constexpr (V <= 4) { if (r.NV == 4) return launch_fprop<DT, V, 4>(p, r, s); }
-    if constexpr (V == 1) {
-        if (r.NV == 8) return launch_fprop<DT, V, 8>(p, r, s);
-        if (r.NV == 16) return launch_fprop<DT, V, 16>(p, r, s);
-    }
-    return cudaErrorInvalidValue;
+    return !mis || F <= kMaxRow - V;
 }
 
 // Most blocks whose shares of the parameters' gradients fit into 32 MB.
 inline i64 most_parts(i64 F) {
-    const i64 fit = (32ll << 20) / (8 * F);
-    return fit < 1 ? 1 : fit > 2048 ? 2048 : fit;
+    const i64 fit = (32ll << 20) / (8 * F) / 8 * 8;
+    return fit > 2048 ? 2048 : fit;
 }
 
-template <int DT, int V, int NV> cudaError_t launch_bprop(const LnP& p, const Rows& r, float* part, int& blocks, cudaStream_t s) {
-    const i64 want = r.warp ? (p.N + 7) / 8 : p.N;
-    const int smem = r.warp ? (int)(8 * p.F) : 0;
-    auto go = [&](auto k, int threads) {
-        i64 most = resident_blocks(k, threads, smem);
-        if (part && most > most_parts(p.F)) most = most_parts(p.F);
-        blocks = (int)(want < most ? want : most);
-        k<<<blocks, threads, smem, s>>>(p, part);
-        return cudaGetLastError();
-    };
-    if (r.warp) return go(ln_bprop_rows<DT, V, NV, true, 256>, 256);
-    if (r.T <= 512) return go(ln_bprop_rows<DT, V, NV, false, 512>, r.T);
-    if constexpr (V * NV == 16) return go(ln_bprop_rows<DT, V, NV, false, 1024>, r.T);
-    return cudaErrorInvalidValue;
-}
-template <int DT, int V> cudaError_t launch_bprop_v(const LnP& p, const Rows& r, float* part, int& blocks, cudaStream_t s) {
-    if (r.NV == 1) return launch_bprop<DT, V, 1>(p, r, part, blocks, s);
-    if (r.NV == 2) return launch_bprop<DT, V, 2>(p, r, part, blocks, s);
-    if constexpr (V <= 4) { if (r.NV == 4) return launch_bprop<DT, V, 4>(p, r, part, blocks, s); }
-    if constexpr (V == 1) {
-        if (r.NV == 8) return launch_bprop<DT, V, 8>(p, r, part, blocks, s);
-        if (r.NV == 16) return launch_bprop<DT, V, 16>(p, r, part, blocks, s);
+// One kernel of either direction: T threads per item; a block is one group, or 8 warps that are
+// groups of their own (4 where there are few items).  `parts`: the blocks, whose shares lie in `part`.
+template <int DT, int NV, int RING, bool MIS, int MAXT, int MINB, bool BACK>
+cudaError_t launch_rows(const LnP& p, int T, float* part, int* parts, cudaStream_t s) {
+    const int groups = T > 32 ? 1 : p.N < 148 * 8 ? 4 : 8, smem = RING * (BACK ? 2 : 1) * NV * T * groups * 16;
+    i64 most;
+    if constexpr (BACK) most = resident_blocks(ln_bprop_rows<DT, NV, RING, MIS, MAXT, MINB>, T * groups, smem);
+    else most = resident_blocks(ln_fprop_rows<DT, NV, RING, MIS, MAXT, MINB>, T * groups, smem);
+    if (!most) return cudaErrorInvalidConfiguration;
+    i64 grid = (p.N + groups - 1) / groups;
+    if (grid > most) grid = most;
+    if (part && grid > most_parts(p.F)) grid = most_parts(p.F);
+    if (MIS) grid = grid < 8 ? 8 : grid / 8 * 8;
+    if constexpr (BACK) {
+        *parts = (int)grid;
+        ln_bprop_rows<DT, NV, RING, MIS, MAXT, MINB><<<(unsigned)grid, T * groups, smem, s>>>(p, part, T);
+    } else {
+        ln_fprop_rows<DT, NV, RING, MIS, MAXT, MINB><<<(unsigned)grid, T * groups, smem, s>>>(p, T);
     }
-    return cudaErrorInvalidValue;
+    return cudaGetLastError();
 }
-
-// Whether every item of the matrices starts on a 16-byte boundary and is a whole number of
-// vectors of V elements long.
-inline bool vectors(const b200_matrix& m, i64 F, int V) {
-    return m.ptr % 16 == 0 && m.s1 % V == 0 && F % V == 0;
+template <int DT, bool MIS, bool BACK> cudaError_t launch_width(const LnP& p, float* part, int* parts, cudaStream_t s) {
+    constexpr int V = 16 / dt_size<DT>::value;
+    const i64 nvec = (p.F + (MIS ? V - 1 : 0) + V - 1) / V;
+    auto width = [&](int nv) { return (int)((nvec + nv - 1) / nv + 31) / 32 * 32; };
+    if constexpr (!BACK) {
+        const bool many = p.N * nvec >= 148 * 4096;     // more than one item for every group there is room for
+        if (width(1) <= 32 || (!many && width(1) <= 128)) return launch_rows<DT, 1, 3, MIS, 512, 1, BACK>(p, width(1), part, parts, s);
+        if (!many && width(2) <= 512) return launch_rows<DT, 2, 3, MIS, 512, 1, BACK>(p, width(2), part, parts, s);
+        if (width(4) <= 256) return launch_rows<DT, 4, 3, MIS, 256, 2, BACK>(p, width(4), part, parts, s);
+        if constexpr (V == 8) return launch_rows<DT, 4, 2, MIS, 512, 1, BACK>(p, width(4), part, parts, s);
+        else return launch_rows<DT, 4, 2, MIS, 1024, 1, BACK>(p, width(4), part, parts, s);
+    } else {
+        // the sums take 4 registers per pair of elements: at most 16 elements per thread
+        if (width(1) <= 64) return launch_rows<DT, 1, 3, MIS, 512, 1, BACK>(p, width(1), part, parts, s);
+        if (width(2) <= 512) return launch_rows<DT, 2, 3, MIS, 512, 1, BACK>(p, width(2), part, parts, s);
+        if constexpr (V == 4) if (width(4) <= 512) return launch_rows<DT, 4, 3, MIS, 512, 1, BACK>(p, width(4), part, parts, s);
+        return launch_rows<DT, 16 / V, 1, MIS, 1024, 1, BACK>(p, width(16 / V), part, parts, s);
+    }
 }
-inline bool is_rows(const b200_matrix& m, i64 F) { return m.s0 == 1 || F == 1; }
+template <bool BACK> cudaError_t launch_type(const LnP& p, bool mis, float* part, int* parts, cudaStream_t s) {
+    switch (p.dt) {
+    case B200_F32: return mis ? launch_width<F32, true, BACK>(p, part, parts, s) : launch_width<F32, false, BACK>(p, part, parts, s);
+    case B200_F16: return mis ? launch_width<F16, true, BACK>(p, part, parts, s) : launch_width<F16, false, BACK>(p, part, parts, s);
+    default: return mis ? launch_width<BF16, true, BACK>(p, part, parts, s) : launch_width<BF16, false, BACK>(p, part, parts, s);
+    }
+}
 
 unsigned blocks_for(i64 n) { return (unsigned)(n < 65536 ? n : 65536); }
 
@@ -437,17 +494,10 @@ extern "C" b200_status b200_ln_fprop(const b200_matrix* x, const b200_matrix* y,
     p.x0 = x->s0; p.x1 = x->s1; p.e0 = p.e1 = 0; p.o0 = y->s0; p.o1 = y->s1;
     p.dt = x->dtype; p.pdt = param_dtype; p.F = features; p.N = items; p.eps = eps;
     cudaError_t e = cudaSuccess;
-    Rows r;
-    const int V = 16 / (int)esize(x->dtype);
-    const bool rows = is_rows(*x, features) && is_rows(*y, features);
-    if (rows && vectors(*x, features, V) && vectors(*y, features, V) && rows_plan(features, V, 16, r)) {
-        if (x->dtype == B200_F32) e = launch_fprop_v<F32, 4>(p, r, s);
-        else if (x->dtype == B200_F16) e = launch_fprop_v<F16, 8>(p, r, s);
-        else e = launch_fprop_v<BF16, 8>(p, r, s);
-    } else if (rows && rows_plan(features, 1, 16, r)) {
-        if (x->dtype == B200_F32) e = launch_fprop_v<F32, 1>(p, r, s);
-        else if (x->dtype == B200_F16) e = launch_fprop_v<F16, 1>(p, r, s);
-        else e = launch_fprop_v<BF16, 1>(p, r, s);
+    const b200_matrix* all[2] = {x, y};
+    bool mis;
+    if (rows_fit(all, 2, features, mis)) {
+        e = launch_type<false>(p, mis, nullptr, nullptr, s);
     } else {
         ln_fprop_any<<<blocks_for(items), 256, 0, s>>>(p);
         e = cudaGetLastError();
@@ -458,8 +508,8 @@ extern "C" b200_status b200_ln_fprop(const b200_matrix* x, const b200_matrix* y,
 
 extern "C" uint64_t b200_ln_bprop_scratch_bytes(int64_t features, int64_t items) {
     if (features < 1 || items < 1 || features > kMaxRow) return 0;
-    const i64 parts = most_parts(features);
-    return (uint64_t)((items < parts ? items : parts) * 8 * features);
+    const i64 parts = most_parts(features), want = items < 32 ? 32 : (items + 7) / 8 * 8;
+    return (uint64_t)((want < parts ? want : parts) * 8 * features);
 }
 
 extern "C" b200_status b200_ln_bprop(const b200_matrix* delta, const b200_matrix* error, const b200_matrix* x,
@@ -508,25 +558,14 @@ extern "C" b200_status b200_ln_bprop(const b200_matrix* delta, const b200_matrix
     p.x0 = x->s0; p.x1 = x->s1; p.e0 = error->s0; p.e1 = error->s1; p.o0 = delta->s0; p.o1 = delta->s1;
     p.dt = x->dtype; p.pdt = param_dtype; p.F = features; p.N = items; p.eps = 0.f;
     int count = 1;
-    Rows r;
-    const int V = 16 / (int)esize(x->dtype);
-    const bool rows = is_rows(*x, features) && is_rows(*error, features) && is_rows(*delta, features);
-    const bool wide = rows && vectors(*x, features, V) && vectors(*error, features, V) && vectors(*delta, features, V)
-                      && rows_plan(features, V, 8, r);
-    if (wide || (rows && rows_plan(features, 1, 8, r))) {
+    const b200_matrix* all[3] = {x, error, delta};
+    bool mis;
+    if (rows_fit(all, 3, features, mis)) {
         float* part = grad_gamma || grad_beta ? reinterpret_cast<float*>(scratch) : nullptr;
-        int blocks = 0;
-        if (wide) {
-            if (x->dtype == B200_F32) err = launch_bprop_v<F32, 4>(p, r, part, blocks, s);
-            else if (x->dtype == B200_F16) err = launch_bprop_v<F16, 8>(p, r, part, blocks, s);
-            else err = launch_bprop_v<BF16, 8>(p, r, part, blocks, s);
-        } else {
-            if (x->dtype == B200_F32) err = launch_bprop_v<F32, 1>(p, r, part, blocks, s);
-            else if (x->dtype == B200_F16) err = launch_bprop_v<F16, 1>(p, r, part, blocks, s);
-            else err = launch_bprop_v<BF16, 1>(p, r, part, blocks, s);
-        }
+        int parts = 0;
+        err = launch_type<true>(p, mis, part, &parts, s);
         if (part && err == cudaSuccess) {
-            ln_sum_parts<<<(unsigned)((2 * features + 31) / 32), 1024, 0, s>>>(part, blocks, features, grad_gamma, grad_beta, param_dtype);
+            ln_sum_parts<<<(unsigned)((2 * features + 7) / 8), 1024, 0, s>>>(part, parts, features, grad_gamma, grad_beta, param_dtype);
             err = cudaGetLastError();
             ++count;
         }

@@ -111,6 +111,34 @@ template <int DT, int V> DEV void st_f(u64 base, i64 off, const float* v) {
     st_raw<B>(reinterpret_cast<char*>(base) + off * dt_size<DT>::value, w);
 }
 
+// Two fp32 values in a register pair, for the instructions that work on both at once (sm_100).
+typedef u64 f32x2;
+DEV f32x2 pair(float lo, float hi) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+DEV void split(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+DEV float both(f32x2 v) { float lo, hi; split(v, lo, hi); return lo + hi; }
+DEV f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+DEV f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+DEV f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
+// Pairs of a loaded 16-byte vector: elements 2 k and 2 k + 1, and the same less c.  A 16-bit
+// element is subtracted without being converted first.
+template <int DT> DEV f32x2 get2(const u32* w, int k) {
+    if constexpr (DT == F32) return pair(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+    else if constexpr (DT == BF16) return pair(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+    else { float lo, hi; h2f2(w[k], lo, hi); return pair(lo, hi); }
+}
+template <int DT> DEV f32x2 less2(const u32* w, int k, float c) {
+    if constexpr (DT == F32) return add2(get2<DT>(w, k), pair(-c, -c));
+    else return pair(mx_half<DT, 0, true>(w[k], c), mx_half<DT, 1, true>(w[k], c));
+}
+// the pair rounded to the stored type, into its place of a vector
+template <int DT> DEV void set2(u32* w, int k, f32x2 v) {
+    float lo, hi;
+    split(v, lo, hi);
+    if constexpr (DT == F32) { w[2 * k] = __float_as_uint(lo); w[2 * k + 1] = __float_as_uint(hi); }
+    else w[k] = DT == F16 ? f2h2_rn(lo, hi) : f2bf2_rn(lo, hi);
+}
+
 DEV float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -140,38 +168,74 @@ DEV float block_max(float v, float* s) {
     return warp_max(lane < warps ? s[lane] : -INFINITY);
 }
 
-// The same with one barrier: `s` holds 64 floats, `turn` alternates from call to call, so that a
-// buffer is written again only after every thread has passed the barrier of the call in between.
-DEV float block_sum_turn(float v, float* s, int& turn) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
+// Sums over a group of T threads (whole warps) of a block: a warp needs no barrier, a wider group
+// uses the named barrier `id` and its own 32 slots of `s` twice over: `turn` alternates from call
+// to call, so a buffer is written again only after the whole group has passed the barrier of the
+// call in between.  The same order in every run; every thread of the group gets the result.
+DEV void group_barrier(int id, int T) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(T) : "memory"); }
+
+DEV float group_sum(float v, float* s, int& turn, int T, int id) {
     v = warp_sum(v);
-    if (lane == 0) s[turn * 32 + warp] = v;
-    __syncthreads();
-    v = warp_sum(lane < warps ? s[turn * 32 + lane] : 0.f);
+    if (T == 32) return v;
+    const int warps = T >> 5, warp = (threadIdx.x % T) >> 5, lane = threadIdx.x & 31;
+    float* buf = s + turn * 32;
+    if (lane == 0) buf[warp] = v;
+    group_barrier(id, T);
+    v = lane < warps ? buf[lane] : 0.f;
     turn ^= 1;
-    return v;
+    return warp_sum(v);
 }
-DEV float2 block_sum2_turn(float a, float b, float2* s, int& turn) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
-    a = warp_sum(a);
-    b = warp_sum(b);
-    if (lane == 0) s[turn * 32 + warp] = make_float2(a, b);
-    __syncthreads();
-    const float2 t = lane < warps ? s[turn * 32 + lane] : make_float2(0.f, 0.f);
+// Two sums at once: after the first exchange the lower half of a warp carries a, the upper half b.
+DEV float2 warp_sum2(float a, float b) {
+    const int lane = threadIdx.x & 31;
+    const bool up = lane & 16;
+    const float other = __shfl_xor_sync(0xffffffffu, up ? a : b, 16);
+    float v = (up ? b : a) + other;
+#pragma unroll
+    for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const float w = __shfl_xor_sync(0xffffffffu, v, 16);
+    return up ? make_float2(w, v) : make_float2(v, w);
+}
+DEV float2 group_sum2(float a, float b, float2* s, int& turn, int T, int id) {
+    float2 v = warp_sum2(a, b);
+    if (T == 32) return v;
+    const int warps = T >> 5, warp = (threadIdx.x % T) >> 5, lane = threadIdx.x & 31;
+    float2* buf = s + turn * 32;
+    if (lane == 0) buf[warp] = v;
+    group_barrier(id, T);
+    v = lane < warps ? buf[lane] : make_float2(0.f, 0.f);
     turn ^= 1;
-    return make_float2(warp_sum(t.x), warp_sum(t.y));
+    return warp_sum2(v.x, v.y);
 }
 
-// Blocks of a kernel that can be resident at once, over all SMs.
-template <typename K> inline int resident_blocks(K kernel, int threads, int smem) {
+// 16 bytes from global to shared memory behind the thread's back; the thread that issued a copy
+// reads it after waiting until at most `LEFT` younger groups of its copies are under way.
+DEV void copy16(u32 to, u64 from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(from) : "memory"); }
+DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> DEV void copy_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(LEFT) : "memory"); }
+
+// Blocks of a kernel that can be resident at once, over all SMs (0: the launch is not possible).
+// Asking the runtime takes longer than a launch, so answers are kept per kernel and block shape.
+inline int resident_blocks(const void* kernel, int threads, int smem) {
+    struct Known { const void* kernel; int threads, smem, blocks; };
+    static thread_local Known known[256] = {};
     static thread_local int sms = 0;
-    if (!sms) {
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
+    Known& k = known[((uintptr_t)kernel / 16 + (unsigned)threads * 7u + (unsigned)smem / 16u) % 256];
+    if (k.kernel == kernel && k.threads == threads && k.smem == smem) return k.blocks;
+    int dev = 0, n = 0;
+    if (!sms && (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)) return 0;
+    if (smem > 32 * 1024) {                            // all that a block may have, so that no later call lowers it
+        cudaFuncAttributes a;
+        if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess) return 0;
+        const int most = 227 * 1024 - (int)a.sharedSizeBytes;
+        if (smem > most || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return 0;
     }
-    int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
-    return n * sms;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) return 0;
+    k.kernel = kernel; k.threads = threads; k.smem = smem; k.blocks = n * sms;
+    return k.blocks;
+}
+template <typename K> inline int resident_blocks(K* kernel, int threads, int smem) {
+    return resident_blocks(reinterpret_cast<const void*>(kernel), threads, smem);
 }
 
 }  // namespace nn
