@@ -125,15 +125,9 @@ template <int DT, int V> DEV void mask(u32* w, int f, int F) {
         else w[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u;
     }
 }
-// Stores a vector at element f of an item, leaving out what lies outside [0, F).
 template <int DT, int V, bool MIS> DEV void put(u64 base, i64 item, int f, int F, const u32* w) {
-    if (!MIS || (f >= 0 && f + V <= F)) { st_raw<16>(reinterpret_cast<char*>(base) + (item + f) * dt_size<DT>::value, w); return; }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        if ((unsigned)(f + i) >= (unsigned)F) continue;
-        if constexpr (dt_size<DT>::value == 4) reinterpret_cast<u32*>(base)[item + f + i] = w[i];
-        else reinterpret_cast<u16*>(base)[item + f + i] = (u16)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]);
-    }
+    if constexpr (MIS) put_part<DT, V>(base, item, f, F, w);
+    else st_raw<16>(reinterpret_cast<char*>(base) + (item + f) * dt_size<DT>::value, w);
 }
 // The parameters of a thread's features.
 template <int V, int NV> DEV void load_params(u64 base, int dt, float fill, int me, int T, int mis, int F, f32x2 (&v)[NV][V / 2]) {
@@ -395,7 +389,7 @@ bool rows_fit(const b200_matrix* const* m, int count, i64 F, bool& mis) {
 // Most blocks whose shares of the parameters' gradients fit into 32 MB.
 inline i64 most_parts(i64 F) {
     const i64 fit = (32ll << 20) / (8 * F) / 8 * 8;
-    return fit > 2048 ? 2048 : fit;
+    return fit > 2048 ? 2048 : fit < 8 ? 8 : fit;
 }
 
 // One kernel of either direction: T threads per item; a block is one group, or 8 warps that are
@@ -446,11 +440,196 @@ template <bool BACK> cudaError_t launch_type(const LnP& p, bool mis, float* part
     }
 }
 
+// ---- items next to each other (their stride is 1; neon's own order)
+//
+// A block takes a stripe of neighbouring items, `lanes` threads with V items each side by side and
+// its other threads down the features, so every access is a run of 32 to 128 bytes of a feature's
+// row.  The stripe is walked through three times forward (sum, centred squares, result) and twice
+// backwards; only the first walk reads HBM: the stripes under way, at most 128 bytes times F per
+// block, stay in L2 or L1.
+template <int V> DEV void stripe_sum(float (&v)[V], float* s, int lanes) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, tx = threadIdx.x & (lanes - 1);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        for (int o = 16; o >= lanes; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    __syncthreads();
+    if (lane < lanes) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[(warp * lanes + tx) * V + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float a = 0.f;
+        for (int w = 0; w < warps; ++w) a += s[(w * lanes + tx) * V + i];
+        v[i] = a;
+    }
+}
+
+template <int DT, int V>
+__global__ void __launch_bounds__(512) ln_fprop_cols(const __grid_constant__ LnP p, int lanes) {
+    __shared__ float s[16 * 32 * (V > 1 ? 2 : 1)];     // [warps][lanes][V]: 8 lanes of vectors, or 32 of single items
+    const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = blockDim.x / lanes, F = (int)p.F;
+    const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
+    const bool in = n < p.N;
+    const float inv = 1.f / (float)F;
+    float mean[V], rstd[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) mean[i] = rstd[i] = 0.f;
+    if (in) {
+#pragma unroll 4
+        for (int f = ty; f < F; f += rows) {
+            float x[V];
+            ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
+#pragma unroll
+            for (int i = 0; i < V; ++i) mean[i] += x[i];
+        }
+    }
+    stripe_sum<V>(mean, s, lanes);
+#pragma unroll
+    for (int i = 0; i < V; ++i) mean[i] *= inv;
+    if (in) {
+#pragma unroll 4
+        for (int f = ty; f < F; f += rows) {
+            float x[V];
+            ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
+#pragma unroll
+            for (int i = 0; i < V; ++i) { x[i] -= mean[i]; rstd[i] = fmaf(x[i], x[i], rstd[i]); }
+        }
+    }
+    stripe_sum<V>(rstd, s, lanes);
+#pragma unroll
+    for (int i = 0; i < V; ++i) rstd[i] = 1.f / sqrtf(rstd[i] * inv + p.eps);
+    if (!in) return;
+    if (ty == 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (p.mean) reinterpret_cast<float*>(p.mean)[n + i] = mean[i];
+            if (p.rstd) reinterpret_cast<float*>(p.rstd)[n + i] = rstd[i];
+        }
+    }
+#pragma unroll 4
+    for (int f = ty; f < F; f += rows) {
+        const float g = p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f, b = p.beta ? ld_any(p.beta, f, p.pdt) : 0.f;
+        float x[V];
+        ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = fmaf((x[i] - mean[i]) * rstd[i], g, b);
+        st_f<DT, V>(p.out, f * p.o0 + n, x);
+    }
+}
+
+// part[block][0][F]: the block's share of grad_gamma, part[block][1][F]: of grad_beta; a block
+// works through stripes gridDim.x apart and adds to its own shares.
+template <int DT, int V>
+__global__ void __launch_bounds__(512) ln_bprop_cols(const __grid_constant__ LnP p, float* part, int lanes, i64 stripes) {
+    __shared__ float s[16 * 32 * (V > 1 ? 2 : 1)];
+    const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = blockDim.x / lanes, F = (int)p.F;
+    const float inv = 1.f / (float)F;
+    float* mine = part + (i64)blockIdx.x * 2 * F;
+    for (i64 stripe = blockIdx.x; stripe < stripes; stripe += gridDim.x) {
+        const i64 n = (stripe * lanes + tx) * V;
+        const bool in = n < p.N;
+        float mean[V], rstd[V], a[V], b[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            mean[i] = in ? reinterpret_cast<const float*>(p.mean)[n + i] : 0.f;
+            rstd[i] = in ? reinterpret_cast<const float*>(p.rstd)[n + i] : 0.f;
+            a[i] = b[i] = 0.f;
+        }
+        for (int f0 = 0; f0 < F; f0 += rows) {         // all threads: the lanes of a feature add up below
+            const int f = f0 + ty;
+            float gg = 0.f, gb = 0.f;
+            if (in && f < F) {
+                const float gamma = p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f;
+                float x[V], e[V];
+                ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
+                ld_f<DT, V, false>(p.e, f * p.e0 + n, e);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    x[i] = (x[i] - mean[i]) * rstd[i];
+                    gg = fmaf(e[i], x[i], gg);
+                    gb += e[i];
+                    e[i] *= gamma;
+                    a[i] += e[i];
+                    b[i] = fmaf(e[i], x[i], b[i]);
+                }
+            }
+            if (part) {
+                for (int o = lanes >> 1; o; o >>= 1) {
+                    gg += __shfl_xor_sync(0xffffffffu, gg, o);
+                    gb += __shfl_xor_sync(0xffffffffu, gb, o);
+                }
+                if (tx == 0 && f < F) {
+                    const bool more = stripe != blockIdx.x;
+                    mine[f] = (more ? mine[f] : 0.f) + gg;
+                    mine[F + f] = (more ? mine[F + f] : 0.f) + gb;
+                }
+            }
+        }
+        stripe_sum<V>(a, s, lanes);
+        stripe_sum<V>(b, s, lanes);
+        if (!in) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) { a[i] *= inv; b[i] *= inv; }
+#pragma unroll 2
+        for (int f = ty; f < F; f += rows) {
+            const float gamma = p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f;
+            float x[V], e[V];
+            ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
+            ld_f<DT, V, false>(p.e, f * p.e0 + n, e);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                x[i] = (x[i] - mean[i]) * rstd[i];
+                e[i] = rstd[i] * ((e[i] * gamma - a[i]) - x[i] * b[i]);
+            }
+            st_f<DT, V>(p.out, f * p.o0 + n, e);
+        }
+    }
+}
+
+// Whether the matrices have their items next to each other; `wide`: in whole 16-byte vectors.
+bool cols_fit(const b200_matrix* const* m, int count, i64 N, bool& wide) {
+    const i64 V = 16 / esize(m[0]->dtype);
+    wide = N % V == 0;
+    for (int i = 0; i < count; ++i) {
+        if (m[i]->s1 != 1 && N != 1) return false;
+        wide = wide && m[i]->ptr % 16 == 0 && m[i]->s0 % V == 0;
+    }
+    return true;
+}
+
+// Stripes of 128 bytes, or down to 32 bytes where wider ones would leave SMs without a block.
+template <int DT, int V, bool BACK> cudaError_t launch_cols(const LnP& p, float* part, int* parts, cudaStream_t s) {
+    constexpr int size = dt_size<DT>::value * V;
+    int lanes = 128 / size > 32 ? 32 : 128 / size;
+    while (lanes * size > 32 && lanes > 1 && (p.N + (i64)lanes * V - 1) / ((i64)lanes * V) < 2 * 148) lanes /= 2;
+    const i64 stripes = (p.N + (i64)lanes * V - 1) / ((i64)lanes * V);
+    if constexpr (BACK) {
+        i64 grid = resident_blocks(ln_bprop_cols<DT, V>, 512, 0);
+        if (!grid) return cudaErrorInvalidConfiguration;
+        if (grid > stripes) grid = stripes;
+        if (part && grid > most_parts(p.F)) grid = most_parts(p.F);
+        *parts = (int)grid;
+        ln_bprop_cols<DT, V><<<(unsigned)grid, 512, 0, s>>>(p, part, lanes, stripes);
+    } else {
+        ln_fprop_cols<DT, V><<<(unsigned)stripes, 512, 0, s>>>(p, lanes);
+    }
+    return cudaGetLastError();
+}
+template <bool BACK> cudaError_t launch_cols_type(const LnP& p, bool wide, float* part, int* parts, cudaStream_t s) {
+    switch (p.dt) {
+    case B200_F32: return wide ? launch_cols<F32, 4, BACK>(p, part, parts, s) : launch_cols<F32, 1, BACK>(p, part, parts, s);
+    case B200_F16: return wide ? launch_cols<F16, 8, BACK>(p, part, parts, s) : launch_cols<F16, 1, BACK>(p, part, parts, s);
+    default: return wide ? launch_cols<BF16, 8, BACK>(p, part, parts, s) : launch_cols<BF16, 1, BACK>(p, part, parts, s);
+    }
+}
+
 unsigned blocks_for(i64 n) { return (unsigned)(n < 65536 ? n : 65536); }
 
 // Checks that the matrices and vectors of either direction have in common.
 int32_t check_sizes(const char* where, i64 F, i64 N) {
-    if (F < 1 || F > 0x7fffffff) return refuse(where, "between 1 and 2^31 - 1 features");
+    if (F < 1 || F > (1 << 30)) return refuse(where, "between 1 and 2^30 features");
     if (N < 0 || N > 0x7fffffff) return refuse(where, "between 0 and 2^31 - 1 items");
     return B200_OK;
 }
@@ -495,9 +674,11 @@ extern "C" b200_status b200_ln_fprop(const b200_matrix* x, const b200_matrix* y,
     p.dt = x->dtype; p.pdt = param_dtype; p.F = features; p.N = items; p.eps = eps;
     cudaError_t e = cudaSuccess;
     const b200_matrix* all[2] = {x, y};
-    bool mis;
+    bool mis, wide;
     if (rows_fit(all, 2, features, mis)) {
         e = launch_type<false>(p, mis, nullptr, nullptr, s);
+    } else if (cols_fit(all, 2, items, wide)) {
+        e = launch_cols_type<false>(p, wide, nullptr, nullptr, s);
     } else {
         ln_fprop_any<<<blocks_for(items), 256, 0, s>>>(p);
         e = cudaGetLastError();
@@ -507,7 +688,7 @@ extern "C" b200_status b200_ln_fprop(const b200_matrix* x, const b200_matrix* y,
 }
 
 extern "C" uint64_t b200_ln_bprop_scratch_bytes(int64_t features, int64_t items) {
-    if (features < 1 || items < 1 || features > kMaxRow) return 0;
+    if (features < 1 || items < 1) return 0;
     const i64 parts = most_parts(features), want = items < 32 ? 32 : (items + 7) / 8 * 8;
     return (uint64_t)((want < parts ? want : parts) * 8 * features);
 }
@@ -559,11 +740,12 @@ extern "C" b200_status b200_ln_bprop(const b200_matrix* delta, const b200_matrix
     p.dt = x->dtype; p.pdt = param_dtype; p.F = features; p.N = items; p.eps = 0.f;
     int count = 1;
     const b200_matrix* all[3] = {x, error, delta};
-    bool mis;
-    if (rows_fit(all, 3, features, mis)) {
+    bool mis, wide;
+    const bool rows = rows_fit(all, 3, features, mis);
+    if (rows || cols_fit(all, 3, items, wide)) {
         float* part = grad_gamma || grad_beta ? reinterpret_cast<float*>(scratch) : nullptr;
         int parts = 0;
-        err = launch_type<true>(p, mis, part, &parts, s);
+        err = rows ? launch_type<true>(p, mis, part, &parts, s) : launch_cols_type<true>(p, wide, part, &parts, s);
         if (part && err == cudaSuccess) {
             ln_sum_parts<<<(unsigned)((2 * features + 7) / 8), 1024, 0, s>>>(part, parts, features, grad_gamma, grad_beta, param_dtype);
             err = cudaGetLastError();

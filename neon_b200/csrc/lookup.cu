@@ -23,6 +23,8 @@ namespace {
 enum { kDigitBits = 9, kDigits = 1 << kDigitBits, kTile = 4096, kSortThreads = 256, kSortWarps = kSortThreads / 32,
        kPerWarp = kTile / kSortWarps };
 
+unsigned blocks_for(i64 n) { return (unsigned)(n < 65536 ? n : 65536); }
+
 struct LutP {
     u64 ids, w, out;
     i64 w0, w1, o0, o1;
@@ -38,6 +40,109 @@ __global__ void __launch_bounds__(256) lut_fprop_any(const __grid_constant__ Lut
         for (i64 f = threadIdx.x; f < p.F; f += blockDim.x)
             st_any(p.out, f * p.o0 + n * p.o1, p.dt, in ? ld_any(p.w, id * p.w0 + f * p.w1, p.dt) * p.scale : 0.f);
     }
+}
+
+// Features of a result next to each other, and of the table: 16-byte vectors of the result, each from
+// one or two vectors of the table's row (which may lie differently to the boundaries).  T threads
+// per position, four positions at a time, so that four independent gathers are under way per thread.
+template <int DT, bool MIS>
+__global__ void __launch_bounds__(256) lut_fprop_rows(const __grid_constant__ LutP p, int T) {
+    constexpr int V = 16 / dt_size<DT>::value, U = 4;
+    const int F = (int)p.F, me = threadIdx.x % T, per = 256 / T;
+    const i64 n0 = ((i64)blockIdx.x * per + threadIdx.x / T) * U;
+    if (threadIdx.x >= per * T) return;
+    int id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = n0 + u < p.N ? reinterpret_cast<const int*>(p.ids)[n0 + u] : -1;
+    const f32x2 scale = pair(p.scale, p.scale);
+    for (int k = me; k * V < F + (MIS ? V - 1 : 0); k += T) {
+        u32 w[U][4];
+        int f[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            f[u] = k * V;
+            if constexpr (MIS) f[u] -= (int)((p.out / dt_size<DT>::value + (u64)((n0 + u) * p.o1)) % V);
+            w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;
+            if (id[u] < 0 || id[u] >= p.V || f[u] >= F) continue;
+            if constexpr (MIS) get_part<DT, V>(p.w, id[u] * p.w0, f[u], F, w[u]);
+            else ld_w<DT, V, true>(p.w, id[u] * p.w0 + f[u], w[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (n0 + u >= p.N) break;
+            if (id[u] >= 0 && id[u] < p.V) {
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) set2<DT>(w[u], i, mul2(get2<DT>(w[u], i), scale));
+            }
+            if constexpr (MIS) { if (f[u] < F) put_part<DT, V>(p.out, (n0 + u) * p.o1, f[u], F, w[u]); }
+            else st_raw<16>(reinterpret_cast<char*>(p.out) + ((n0 + u) * p.o1 + f[u]) * dt_size<DT>::value, w[u]);
+        }
+    }
+}
+
+// Positions of the result next to each other (neon's order): a tile of 64 positions x 64 features
+// is gathered along the features and written along the positions, turned in shared memory.
+template <int DT>
+__global__ void __launch_bounds__(256) lut_fprop_cols(const __grid_constant__ LutP p, int wide) {
+    constexpr int S = dt_size<DT>::value, V = 16 / S, P = 64 * S / 4 + 1;      // words per feature, one spare
+    __shared__ u32 tile[64 * P];
+    __shared__ int ids[64];
+    const i64 n0 = (i64)blockIdx.x * 64;
+    const int f0 = blockIdx.y * 64, F = (int)p.F, left = F - f0 < 64 ? F - f0 : 64;
+    if (threadIdx.x < 64) {
+        const int id = n0 + threadIdx.x < p.N ? reinterpret_cast<const int*>(p.ids)[n0 + threadIdx.x] : -1;
+        ids[threadIdx.x] = id >= 0 && id < p.V ? id : -1;
+    }
+    __syncthreads();
+    auto put = [&](int f, int i, float v) {
+        if constexpr (S == 4) tile[f * P + i] = __float_as_uint(v);
+        else reinterpret_cast<u16*>(tile)[f * (2 * P) + i] = (u16)(DT == F16 ? f2h_rn(v) : f2bf_rn(v));
+    };
+    if (wide) {                                         // whole vectors of the table's rows
+        for (int k = threadIdx.x; k < 64 * (64 / V); k += 256) {
+            const int i = k / (64 / V), f = k % (64 / V) * V;
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = 0.f;
+            if (ids[i] >= 0 && f < left) ld_f<DT, V, true>(p.w, ids[i] * p.w0 + f0 + f, v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) put(f + j, i, v[j] * p.scale);
+        }
+    } else {
+        for (int k = threadIdx.x; k < 64 * 64; k += 256) {
+            const int i = k / 64, f = k % 64;
+            float v[1] = {0.f};
+            if (ids[i] >= 0 && f < left) ld_f<DT, 1, true>(p.w, ids[i] * p.w0 + (f0 + f) * p.w1, v);
+            put(f, i, v[0] * p.scale);
+        }
+    }
+    __syncthreads();
+    const int many = (int)(p.N - n0 < 64 ? p.N - n0 : 64);
+    for (int k = threadIdx.x; k < left * 64; k += 256) {
+        const int f = k / 64, i = k % 64;
+        if (i >= many) continue;
+        const i64 to = (i64)(f0 + f) * p.o0 + n0 + i;
+        if constexpr (S == 4) reinterpret_cast<u32*>(p.out)[to] = tile[f * P + i];
+        else reinterpret_cast<u16*>(p.out)[to] = reinterpret_cast<u16*>(tile)[f * (2 * P) + i];
+    }
+}
+
+template <int DT> cudaError_t launch_fprop(const LutP& p, cudaStream_t s) {
+    constexpr int S = dt_size<DT>::value, V = 16 / S;
+    const bool table = p.w1 == 1 || p.F == 1, aligned = p.w % 16 == 0 && p.w0 % V == 0 && p.F % V == 0;
+    if (table && (p.o0 == 1 || p.F == 1)) {
+        const bool mis = !(aligned && p.out % 16 == 0 && p.o1 % V == 0);
+        const i64 nvec = (p.F + (mis ? V - 1 : 0) + V - 1) / V;
+        const int T = nvec >= 256 ? 256 : nvec <= 32 ? 32 : (int)(nvec + 31) / 32 * 32, per = 256 / T * 4;
+        const unsigned grid = (unsigned)((p.N + per - 1) / per);
+        if (mis) lut_fprop_rows<DT, true><<<grid, 256, 0, s>>>(p, T);
+        else lut_fprop_rows<DT, false><<<grid, 256, 0, s>>>(p, T);
+    } else if (p.o1 == 1 || p.N == 1) {
+        lut_fprop_cols<DT><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)((p.F + 63) / 64)), 256, 0, s>>>(p, table && aligned);
+    } else {
+        lut_fprop_any<<<blocks_for(p.N), 256, 0, s>>>(p);
+    }
+    return cudaGetLastError();
 }
 
 // ------------------------------------------------------------------ sort of (word, position)
@@ -56,6 +161,7 @@ DEV int sort_key(const SortP& p, int i) {
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_count(const __grid_constant__ SortP p) {
+    grid_enter();
     __shared__ int c[kDigits];
     for (int i = threadIdx.x; i < kDigits; i += kSortThreads) c[i] = 0;
     __syncthreads();
@@ -68,6 +174,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count(const __grid_constant
 
 // Exclusive prefix sums of `count` numbers, in place, by one block.
 __global__ void __launch_bounds__(1024) sort_scan(int* a, int count) {
+    grid_enter();
     __shared__ int s[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = (count + 1023) / 1024, lo = min((int)threadIdx.x * per, count), hi = min(lo + per, count);
@@ -98,6 +205,7 @@ __global__ void __launch_bounds__(1024) sort_scan(int* a, int count) {
 // Moves a tile to its places.  A warp takes 512 neighbouring pairs, 32 at a time in their order;
 // lanes with the same digit find each other with match_any, so equal digits keep their order.
 __global__ void __launch_bounds__(kSortThreads) sort_move(const __grid_constant__ SortP p) {
+    grid_enter();
     __shared__ int c[kSortWarps][kDigits];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) (&c[0][0])[i] = 0;
@@ -139,8 +247,37 @@ __global__ void __launch_bounds__(kSortThreads) sort_move(const __grid_constant_
     }
 }
 
+// Few positions: the place of a position is the number of smaller words, and of equal ones before
+// it.  N^2 comparisons in one launch, 32 positions per block, its warps over the other positions:
+// about 3 us at 4096 positions, where the radix sort's launches alone take longer.
+enum { kRankMost = 8192 };
+__global__ void __launch_bounds__(256) sort_rank(const __grid_constant__ SortP p) {
+    grid_enter();
+    __shared__ int part[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+    const int key = i < p.N ? sort_key(p, i) : 0;
+    const int per = ((p.N + 7) / 8 + 31) / 32 * 32, lo = warp * per, hi = min(lo + per, p.N);
+    int before = 0;
+    for (int j0 = lo; j0 < hi; j0 += 32) {
+        const int other = j0 + lane < hi ? sort_key(p, j0 + lane) : 0x7fffffff;
+#pragma unroll 8
+        for (int l = 0; l < 32; ++l) {
+            const int k = __shfl_sync(0xffffffffu, other, l);
+            before += k < key || (k == key && j0 + l < i);
+        }
+    }
+    part[warp][lane] = before;
+    __syncthreads();
+    if (warp || i >= p.N) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) before += part[w][lane];
+    p.key_out[before] = key;
+    p.pos_out[before] = i;
+}
+
 // start[v] = first sorted place whose word is at least v, for v in 0 .. V
 __global__ void __launch_bounds__(256) sort_starts(const int* key, int N, int* start, int V) {
+    grid_enter();
     const int v = blockIdx.x * 256 + threadIdx.x;
     if (v > V) return;
     int lo = 0, hi = N;
@@ -156,62 +293,148 @@ struct SumP {
     const int *key, *pos, *start;
     u64 e, w;
     i64 e0, e1, w0, w1;
-    int edt, wdt, V;
+    int edt, wdt, V, wide;                // wide: dW's rows are whole 16-byte vectors of its own type and of 8 elements
     i64 F, L;                             // L sorted places per chunk
     float* part;                          // [chunk][2][F]: 0 continues an earlier chunk, 1 begins here and goes on
     float alpha, beta;
 };
 
-DEV void put_dw(const SumP& p, int v, i64 f, float sum) {
+template <int V> DEV void put_dw(const SumP& p, i64 v, int f, const float* sum) {
     const i64 at = v * p.w0 + f * p.w1;
-    float r = p.alpha * sum;
-    if (p.beta != 0.f) r += p.beta * ld_any(p.w, at, p.wdt);
-    st_any(p.w, at, p.wdt, r);
+    float r[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = p.alpha * sum[i];
+    if (p.beta != 0.f) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (f + i < p.F) r[i] += p.beta * ld_any(p.w, at + i * p.w1, p.wdt);
+    }
+    if (V > 1 && p.wide) {
+        if (p.wdt == F32) {
+#pragma unroll
+            for (int i = 0; i < V; i += 4) st_f<F32, V < 4 ? V : 4>(p.w, at + i, r + i);
+        } else if (p.wdt == F16) st_f<F16, V>(p.w, at, r);
+        else st_f<BF16, V>(p.w, at, r);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (f + i < p.F) st_any(p.w, at + i * p.w1, p.wdt, r[i]);
 }
 
-__global__ void __launch_bounds__(256) lut_chunks_any(const __grid_constant__ SumP p) {
+// A thread adds up V features of the places of one chunk, in their order; neighbouring threads take
+// neighbouring features.  V > 1: the error's features are next to each other.  `aligned`: its
+// positions start on 16-byte boundaries.
+template <int DT, int V>
+__global__ void __launch_bounds__(256) lut_chunks(const __grid_constant__ SumP p, i64 chunks, int nvec, int aligned) {
+    grid_enter();
+    const i64 id = (i64)blockIdx.x * 256 + threadIdx.x, chunk = id / nvec;
+    if (chunk >= chunks) return;
+    const int f = (int)(id - chunk * nvec) * V, F = (int)p.F;
     const int used = p.start[p.V];
-    const i64 f = (i64)blockIdx.y * 256 + threadIdx.x;
-    const i64 lo = (i64)blockIdx.x * p.L;
-    const i64 hi = lo + p.L < used ? lo + p.L : used;
-    if (lo >= used || f >= p.F) return;
-    float sum = 0.f;
+    const i64 lo = chunk * p.L, hi = lo + p.L < used ? lo + p.L : used;
+    if (lo >= used) return;
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
     int v = p.key[lo];
-    for (i64 i = lo; i < hi; ++i) {
-        sum += ld_any(p.e, f * p.e0 + p.pos[i] * p.e1, p.edt);
-        const int next = i + 1 < hi ? p.key[i + 1] : -1;
-        if (next == v) continue;
-        const bool from_before = p.start[v] < lo, goes_on = p.start[v + 1] > hi;
-        if (from_before || goes_on) p.part[((i64)blockIdx.x * 2 + (from_before ? 0 : 1)) * p.F + f] = sum;
-        else put_dw(p, v, f, sum);
-        sum = 0.f;
-        v = next;
+    bool from_before = lo > 0 && p.key[lo - 1] == v;
+    for (i64 i0 = lo; i0 < hi; i0 += 4) {
+        float e[4][V];
+        int next[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            next[u] = i0 + u + 1 < hi ? p.key[i0 + u + 1] : -1;
+            if (i0 + u >= hi) continue;
+            const i64 at = p.pos[i0 + u] * p.e1;
+            if constexpr (V == 1) ld_f<DT, 1, true>(p.e, at + f * p.e0, e[u]);
+            else if (aligned) ld_f<DT, V, true>(p.e, at + f, e[u]);
+            else {
+                u32 w[4];
+                get_part<DT, V>(p.e, at, f, F, w);
+                cvt_in<DT, V>(w, e[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (i0 + u >= hi) break;
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] += e[u][i];
+            if (next[u] == v) continue;
+            const bool goes_on = next[u] < 0 && hi < used && p.key[hi] == v;
+            if (from_before || goes_on) {
+                float* to = p.part + (chunk * 2 + (from_before ? 0 : 1)) * F + f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) if (f + i < F) to[i] = sum[i];
+            } else {
+                put_dw<V>(p, v, f, sum);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] = 0.f;
+            v = next[u];
+            from_before = false;
+        }
     }
 }
 
-// Words without a position, and words that cross a border between chunks.
-__global__ void __launch_bounds__(256) lut_finish_any(const __grid_constant__ SumP p) {
-    for (i64 v = blockIdx.x; v < p.V; v += gridDim.x) {
-        const int lo = p.start[v], hi = p.start[v + 1];
-        if (lo == hi) {
-            if (p.beta != 1.f)
-                for (i64 f = threadIdx.x; f < p.F; f += 256) {
-                    const i64 at = v * p.w0 + f * p.w1;
-                    st_any(p.w, at, p.wdt, p.beta == 0.f ? 0.f : p.beta * ld_any(p.w, at, p.wdt));
-                }
-            continue;
+// 64 words x 32 V features per block: words without a position are cleared (or scaled), words that
+// cross a border between chunks get their partial sums added, each warp over an eighth of the
+// chunks, the warps in their order.
+template <int V>
+__global__ void __launch_bounds__(256) lut_finish(const __grid_constant__ SumP p) {
+    grid_enter();
+    __shared__ int start[65];
+    __shared__ float s[8][32 * V + 1];
+    const i64 v0 = (i64)blockIdx.x * 64;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, f = (blockIdx.y * 32 + lane) * V, F = (int)p.F;
+    const int words = (int)(p.V - v0 < 64 ? p.V - v0 : 64);
+    if (threadIdx.x <= words) start[threadIdx.x] = p.start[v0 + threadIdx.x];
+    __syncthreads();
+    float zero[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) zero[i] = 0.f;
+    if (p.beta != 1.f)
+        for (int k = warp; k < words; k += 8)
+            if (start[k] == start[k + 1] && f < F) put_dw<V>(p, v0 + k, f, zero);
+    for (int k = 0; k < words; ++k) {
+        const int lo = start[k], hi = start[k + 1];
+        if (lo == hi || lo / p.L == (hi - 1) / p.L) continue;
+        const i64 c0 = lo / p.L, c1 = (hi - 1) / p.L, per = (c1 - c0 + 8) / 8;
+        const i64 from = c0 + warp * per, to = from + per < c1 + 1 ? from + per : c1 + 1;
+        float sum[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] = 0.f;
+        if (f < F) {
+#pragma unroll 4
+            for (i64 c = from; c < to; ++c) {
+                const float* at = p.part + (c * 2 + (c == c0 ? 1 : 0)) * F + f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) if (f + i < F) sum[i] += at[i];
+            }
         }
-        const i64 c0 = lo / p.L, c1 = (hi - 1) / p.L;
-        if (c0 == c1) continue;
-        for (i64 f = threadIdx.x; f < p.F; f += 256) {
-            float sum = p.part[(c0 * 2 + 1) * p.F + f];
-            for (i64 c = c0 + 1; c <= c1; ++c) sum += p.part[c * 2 * p.F + f];
-            put_dw(p, (int)v, f, sum);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[warp][lane * V + i] = sum[i];
+        __syncthreads();
+        if (warp == 0 && f < F) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                sum[i] = 0.f;
+                for (int w = 0; w < 8; ++w) sum[i] += s[w][lane * V + i];
+            }
+            put_dw<V>(p, v0 + k, f, sum);
         }
     }
 }
 
-unsigned blocks_for(i64 n) { return (unsigned)(n < 65536 ? n : 65536); }
+template <int DT, int V> cudaError_t launch_chunks(const SumP& p, i64 chunks, bool aligned, cudaStream_t s) {
+    const i64 nvec = (p.F + V - 1) / V, grid = (chunks * nvec + 255) / 256;
+    return launch_dependent(lut_chunks<DT, V>, dim3((unsigned)grid), 256, 0, s, p, chunks, (int)nvec, (int)aligned);
+}
+template <int DT> cudaError_t launch_sums(const SumP& p, i64 chunks, cudaStream_t s) {
+    constexpr int V = 16 / dt_size<DT>::value;
+    if (!chunks) return cudaSuccess;
+    if (p.e0 != 1 && p.F != 1) return launch_chunks<DT, 1>(p, chunks, false, s);
+    return launch_chunks<DT, V>(p, chunks, p.e % 16 == 0 && p.e1 % V == 0 && p.F % V == 0, s);
+}
 
 // Where the pieces of the gradient's scratch lie.
 struct Plan {
@@ -241,7 +464,7 @@ Plan plan(i64 V, i64 F, i64 N) {
 
 int32_t check_sizes(const char* where, i64 V, i64 F, i64 N) {
     if (V < 1 || V >= 0x7fffffff) return refuse(where, "between 1 and 2^31 - 2 words");
-    if (F < 1 || F > 65535 * 256) return refuse(where, "between 1 and 65535 * 256 features");
+    if (F < 1 || F > 65535 * 32) return refuse(where, "between 1 and 65535 * 32 features");
     if (N < 0 || N > 0x7fffffff - kTile) return refuse(where, "fewer than 2^31 - 4096 positions");
     return B200_OK;
 }
@@ -268,8 +491,11 @@ extern "C" b200_status b200_lut_fprop(uint64_t ids, const b200_matrix* table, co
     p.ids = ids; p.w = table->ptr; p.out = out->ptr;
     p.w0 = table->s0; p.w1 = table->s1; p.o0 = out->s0; p.o1 = out->s1;
     p.dt = table->dtype; p.V = (int)words; p.F = features; p.N = positions; p.scale = scale;
-    lut_fprop_any<<<blocks_for(positions), 256, 0, s>>>(p);
-    return cuda_status(where, cudaGetLastError());
+    cudaError_t e;
+    if (p.dt == B200_F32) e = launch_fprop<F32>(p, s);
+    else if (p.dt == B200_F16) e = launch_fprop<F16>(p, s);
+    else e = launch_fprop<BF16>(p, s);
+    return cuda_status(where, e);
 }
 
 extern "C" uint64_t b200_lut_bprop_scratch_bytes(int64_t words, int64_t features, int64_t positions) {
@@ -303,15 +529,22 @@ extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, co
     t.ids = reinterpret_cast<const int*>(ids); t.hist = ints(q.hist);
     t.N = (int)positions; t.V = (int)words; t.tiles = (int)q.tiles;
     t.pad = pad_idx < 0 || pad_idx >= words ? -1 : (int)pad_idx;
-    for (int k = 0; positions && k < q.passes; ++k) {
-        t.first = k == 0; t.shift = k * kDigitBits;
-        t.key_in = ints(q.key[from]); t.pos_in = ints(q.pos[from]);
-        t.key_out = ints(q.key[1 - from]); t.pos_out = ints(q.pos[1 - from]);
-        sort_count<<<(unsigned)q.tiles, kSortThreads, 0, s>>>(t);
-        sort_scan<<<1, 1024, 0, s>>>(t.hist, (int)(kDigits * q.tiles));
-        sort_move<<<(unsigned)q.tiles, kSortThreads, 0, s>>>(t);
-        from = 1 - from;
-        count += 3;
+    cudaError_t e = cudaSuccess;
+    if (positions && positions <= kRankMost) {
+        t.first = 1; t.shift = 0; t.key_in = t.pos_in = nullptr; t.key_out = ints(q.key[0]); t.pos_out = ints(q.pos[0]);
+        e = launch_dependent(sort_rank, dim3((unsigned)(positions + 31) / 32), 256, 0, s, t);
+        ++count;
+    } else if (positions) {
+        for (int k = 0; k < q.passes && e == cudaSuccess; ++k) {
+            t.first = k == 0; t.shift = k * kDigitBits;
+            t.key_in = ints(q.key[from]); t.pos_in = ints(q.pos[from]);
+            t.key_out = ints(q.key[1 - from]); t.pos_out = ints(q.pos[1 - from]);
+            e = launch_dependent(sort_count, dim3((unsigned)q.tiles), kSortThreads, 0, s, t);
+            if (e == cudaSuccess) e = launch_dependent(sort_scan, dim3(1), 1024, 0, s, t.hist, (int)(kDigits * q.tiles));
+            if (e == cudaSuccess) e = launch_dependent(sort_move, dim3((unsigned)q.tiles), kSortThreads, 0, s, t);
+            from = 1 - from;
+            count += 3;
+        }
     }
     SumP p;
     p.key = ints(q.key[from]); p.pos = ints(q.pos[from]); p.start = ints(q.start);
@@ -319,13 +552,20 @@ extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, co
     p.w = dtable->ptr; p.w0 = dtable->s0; p.w1 = dtable->s1; p.wdt = dtable->dtype;
     p.V = (int)words; p.L = q.L; p.F = features; p.part = reinterpret_cast<float*>(base + q.part);
     p.alpha = alpha; p.beta = beta;
-    sort_starts<<<(unsigned)((words + 256) / 256), 256, 0, s>>>(p.key, (int)positions, ints(q.start), (int)words);
-    ++count;
-    if (positions) {
-        lut_chunks_any<<<dim3((unsigned)q.chunks, (unsigned)((features + 255) / 256)), 256, 0, s>>>(p);
-        ++count;
+    p.wide = features % 8 == 0 && dtable->s1 == 1 && dtable->ptr % 16 == 0 && dtable->s0 % 8 == 0;
+    if (e == cudaSuccess)
+        e = launch_dependent(sort_starts, dim3((unsigned)((words + 256) / 256)), 256, 0, s, p.key, (int)positions, ints(q.start), (int)words);
+    if (e == cudaSuccess) {
+        if (p.edt == B200_F32) e = launch_sums<F32>(p, q.chunks, s);
+        else if (p.edt == B200_F16) e = launch_sums<F16>(p, q.chunks, s);
+        else e = launch_sums<BF16>(p, q.chunks, s);
     }
-    lut_finish_any<<<blocks_for(words), 256, 0, s>>>(p);
-    if (launches) *launches = count + 1;
-    return cuda_status(where, cudaGetLastError());
+    // four features per thread in the last kernel, or one where dW's features are not neighbours
+    const int V = dtable->s1 == 1 ? 4 : 1;
+    const dim3 grid((unsigned)((words + 63) / 64), (unsigned)((features + 32 * V - 1) / (32 * V)));
+    if (e == cudaSuccess)
+        e = V == 4 ? launch_dependent(lut_finish<4>, grid, 256, 0, s, p) : launch_dependent(lut_finish<1>, grid, 256, 0, s, p);
+    if (launches) *launches = count + (positions ? 3 : 2);
+    return cuda_status(where, e);
 }
+

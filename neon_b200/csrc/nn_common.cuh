@@ -139,6 +139,42 @@ template <int DT> DEV void set2(u32* w, int k, f32x2 v) {
     else w[k] = DT == F16 ? f2h2_rn(lo, hi) : f2bf2_rn(lo, hi);
 }
 
+// Stores a 16-byte vector at element f of an item, leaving out what lies outside [0, F).
+template <int DT, int V> DEV void put_part(u64 base, i64 item, int f, int F, const u32* w) {
+    if (f >= 0 && f + V <= F) { st_raw<16>(reinterpret_cast<char*>(base) + (item + f) * dt_size<DT>::value, w); return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if ((unsigned)(f + i) >= (unsigned)F) continue;
+        if constexpr (dt_size<DT>::value == 4) reinterpret_cast<u32*>(base)[item + f + i] = w[i];
+        else reinterpret_cast<u16*>(base)[item + f + i] = (u16)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]);
+    }
+}
+
+// V elements from f on of an item that starts anywhere: one aligned vector, or two and a shift.
+// Only 16-byte vectors that hold an element of [0, F) are read; other elements come out undefined.
+template <int DT, int V> DEV void get_part(u64 base, i64 item, int f, int F, u32* w) {
+    constexpr int S = dt_size<DT>::value;
+    const u64 at = base + (u64)((item + f) * S);
+    const int m = (int)(at & 15u) / S;                  // elements behind a boundary
+    const char* from = reinterpret_cast<const char*>(at - m * S);
+    if (m == 0) { ld_raw<16, false>(from, w); return; }
+    u32 x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (f - m + V > 0) ld_raw<16, false>(from, x);
+    if (f - m + V < F) ld_raw<16, false>(from + 16, x + 4);
+    const int words = m * S / 4;
+    if (words & 2) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) x[i] = x[i + 2];
+    }
+    if (words & 1) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) x[i] = x[i + 1];
+    }
+    const u32 bits = S == 2 && (m & 1) ? 16 : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(x[i], x[i + 1], bits);
+}
+
 DEV float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -213,6 +249,19 @@ DEV float2 group_sum2(float a, float b, float2* s, int& turn, int T, int id) {
 DEV void copy16(u32 to, u64 from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(from) : "memory"); }
 DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> DEV void copy_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(LEFT) : "memory"); }
+
+// Launch that may be placed while the previous kernel of the stream drains: the kernel's first
+// statement is grid_enter().
+template <typename... P, typename... A>
+inline cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid; c.blockDim = dim3(threads); c.dynamicSmemBytes = smem; c.stream = s;
+    cudaLaunchAttribute a;
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &a; c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
 
 // Blocks of a kernel that can be resident at once, over all SMs (0: the launch is not possible).
 // Asking the runtime takes longer than a launch, so answers are kept per kernel and block shape.
