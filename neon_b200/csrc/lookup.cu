@@ -20,7 +20,7 @@ using namespace nn;
 
 namespace {
 
-enum { kDigitBits = 9, kDigits = 1 << kDigitBits, kTile = 4096, kSortThreads = 256, kSortWarps = kSortThreads / 32,
+enum { kDigitBits = 9, kDigits = 1 << kDigitBits, kTile = 1024, kSortThreads = 256, kSortWarps = kSortThreads / 32,
        kPerWarp = kTile / kSortWarps };
 
 unsigned blocks_for(i64 n) { return (unsigned)(n < 65536 ? n : 65536); }
@@ -169,40 +169,31 @@ __global__ void __launch_bounds__(kSortThreads) sort_count(const __grid_constant
     for (int i = base + threadIdx.x; i < base + kTile && i < p.N; i += kSortThreads)
         atomicAdd(&c[(sort_key(p, i) >> p.shift) & (kDigits - 1)], 1);
     __syncthreads();
-    for (int i = threadIdx.x; i < kDigits; i += kSortThreads) p.hist[i * p.tiles + blockIdx.x] = c[i];
+    for (int i = threadIdx.x; i < kDigits; i += kSortThreads) p.hist[(i64)i * p.tiles + blockIdx.x] = c[i];
 }
 
-// Exclusive prefix sums of `count` numbers, in place, by one block.
-__global__ void __launch_bounds__(1024) sort_scan(int* a, int count) {
+// Per digit, a warp turns the tiles' counts into the number of such keys in earlier tiles and
+// leaves their total behind the counts: hist[kDigits * tiles + digit].
+__global__ void __launch_bounds__(256) sort_scan(int* hist, int tiles) {
     grid_enter();
-    __shared__ int s[32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per = (count + 1023) / 1024, lo = min((int)threadIdx.x * per, count), hi = min(lo + per, count);
+    const int lane = threadIdx.x & 31, d = blockIdx.x * 8 + (threadIdx.x >> 5);
+    int* row = hist + (i64)d * tiles;
     int sum = 0;
-    for (int i = lo; i < hi; ++i) sum += a[i];
-    int x = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    if (lane == 31) s[warp] = x;
-    __syncthreads();
-    if (warp == 0) {
-        int y = s[lane];
+    for (int t0 = 0; t0 < tiles; t0 += 32) {
+        const int own = t0 + lane < tiles ? row[t0 + lane] : 0;
+        int x = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, y, o);
-            if (lane >= o) y += t;
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
         }
-        s[lane] = y;
+        if (t0 + lane < tiles) row[t0 + lane] = sum + x - own;
+        sum += __shfl_sync(0xffffffffu, x, 31);
     }
-    __syncthreads();
-    int at = x - sum + (warp ? s[warp - 1] : 0);
-    for (int i = lo; i < hi; ++i) { const int v = a[i]; a[i] = at; at += v; }
+    if (lane == 0) hist[(i64)kDigits * tiles + d] = sum;
 }
 
-// Moves a tile to its places.  A warp takes 512 neighbouring pairs, 32 at a time in their order;
+// Moves a tile to its places.  A warp takes 128 neighbouring pairs, 32 at a time in their order;
 // lanes with the same digit find each other with match_any, so equal digits keep their order.
 __global__ void __launch_bounds__(kSortThreads) sort_move(const __grid_constant__ SortP p) {
     grid_enter();
@@ -230,11 +221,25 @@ __global__ void __launch_bounds__(kSortThreads) sort_move(const __grid_constant_
         rank[r] = before + __popc(peers & ((1u << lane) - 1));
         __syncwarp();
     }
-    __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += kSortThreads) {
-        int at = p.hist[d * p.tiles + blockIdx.x];
+    // keys with smaller digits: two digits per thread
+    __shared__ int warp_sums[kSortWarps];
+    const int* totals = p.hist + (i64)kDigits * p.tiles;
+    const int d0 = 2 * threadIdx.x, t0 = totals[d0], t1 = totals[d0 + 1];
+    int x = t0 + t1;
 #pragma unroll
-        for (int w = 0; w < kSortWarps; ++w) { const int v = c[w][d]; c[w][d] = at; at += v; }
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    int smaller = x - t0 - t1;
+    for (int w = 0; w < warp; ++w) smaller += warp_sums[w];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        int at = smaller + (k ? t0 : 0) + p.hist[(i64)(d0 + k) * p.tiles + blockIdx.x];
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) { const int v = c[w][d0 + k]; c[w][d0 + k] = at; at += v; }
     }
     __syncthreads();
 #pragma unroll
@@ -248,29 +253,37 @@ __global__ void __launch_bounds__(kSortThreads) sort_move(const __grid_constant_
 }
 
 // Few positions: the place of a position is the number of smaller words, and of equal ones before
-// it.  N^2 comparisons in one launch, 32 positions per block, its warps over the other positions:
-// about 3 us at 4096 positions, where the radix sort's launches alone take longer.
+// it.  N^2 comparisons in one launch: 32 positions per block, one per lane, its 16 warps over the
+// other positions.
 enum { kRankMost = 8192 };
-__global__ void __launch_bounds__(256) sort_rank(const __grid_constant__ SortP p) {
+__global__ void __launch_bounds__(512) sort_rank(const __grid_constant__ SortP p) {
     grid_enter();
-    __shared__ int part[8][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
-    const int key = i < p.N ? sort_key(p, i) : 0;
-    const int per = ((p.N + 7) / 8 + 31) / 32 * 32, lo = warp * per, hi = min(lo + per, p.N);
+    __shared__ __align__(16) int keys[kRankMost];
+    __shared__ int part[16][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i0 = blockIdx.x * 32, i = i0 + lane;
+    for (int j = threadIdx.x; j < kRankMost && j < (p.N + 3) / 4 * 4; j += 512) keys[j] = j < p.N ? sort_key(p, j) : 0x7fffffff;
+    __syncthreads();
+    const int key = i < p.N ? keys[i] : 0, quads = (p.N + 3) / 4, per = (quads + 15) / 16;
+    const int lo = min(warp * per, quads), hi = min(lo + per, quads), mid = min(max(i0 / 4, lo), hi), end = min(max((i0 + 32) / 4, lo), hi);
     int before = 0;
-    for (int j0 = lo; j0 < hi; j0 += 32) {
-        const int other = j0 + lane < hi ? sort_key(p, j0 + lane) : 0x7fffffff;
-#pragma unroll 8
-        for (int l = 0; l < 32; ++l) {
-            const int k = __shfl_sync(0xffffffffu, other, l);
-            before += k < key || (k == key && j0 + l < i);
-        }
+    const int4* four = reinterpret_cast<const int4*>(keys);
+#pragma unroll 4
+    for (int q = lo; q < mid; ++q) {                   // positions before all of the block's
+        const int4 k = four[q];
+        before += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
+    }
+    for (int q = mid; q < end; ++q)                    // the block's own
+        for (int e = 0; e < 4; ++e) before += keys[4 * q + e] < key || (keys[4 * q + e] == key && 4 * q + e < i);
+#pragma unroll 4
+    for (int q = end; q < hi; ++q) {
+        const int4 k = four[q];
+        before += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
     }
     part[warp][lane] = before;
     __syncthreads();
     if (warp || i >= p.N) return;
 #pragma unroll
-    for (int w = 1; w < 8; ++w) before += part[w][lane];
+    for (int w = 1; w < 16; ++w) before += part[w][lane];
     p.key_out[before] = key;
     p.pos_out[before] = i;
 }
@@ -320,47 +333,71 @@ template <int V> DEV void put_dw(const SumP& p, i64 v, int f, const float* sum) 
     for (int i = 0; i < V; ++i) if (f + i < p.F) st_any(p.w, at + i * p.w1, p.wdt, r[i]);
 }
 
-// A thread adds up V features of the places of one chunk, in their order; neighbouring threads take
-// neighbouring features.  V > 1: the error's features are next to each other.  `aligned`: its
-// positions start on 16-byte boundaries.
+// The first `sum_blocks` blocks: a thread adds up V features of the places of one chunk, in their
+// order; neighbouring threads take neighbouring features.  Eight places are under way at a time, and
+// the numbers of the next eight are read meanwhile.  V > 1: the error's features are next to each
+// other; `aligned`: its positions start on 16-byte boundaries.
+// The other blocks: a warp looks at 32 words and clears (or scales) those that have no position.
 template <int DT, int V>
-__global__ void __launch_bounds__(256) lut_chunks(const __grid_constant__ SumP p, i64 chunks, int nvec, int aligned) {
+__global__ void __launch_bounds__(256) lut_chunks(const __grid_constant__ SumP p, i64 chunks, int nvec, int aligned, unsigned sum_blocks) {
     grid_enter();
+    const int F = (int)p.F;
+    if (blockIdx.x >= sum_blocks) {
+        const int lane = threadIdx.x & 31;
+        const i64 step = (i64)(gridDim.x - sum_blocks) * 8 * 32;
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        for (i64 v0 = ((i64)(blockIdx.x - sum_blocks) * 8 + (threadIdx.x >> 5)) * 32; v0 < p.V; v0 += step) {
+            unsigned none = __ballot_sync(0xffffffffu, v0 + lane < p.V && p.start[v0 + lane] == p.start[v0 + lane + 1]);
+            while (none) {
+                const i64 v = v0 + __ffs(none) - 1;
+                none &= none - 1;
+                for (int f = lane * 4; f < F; f += 128) put_dw<4>(p, v, f, zero);
+            }
+        }
+        return;
+    }
+    constexpr int U = 8, W = V == 1 ? 1 : 4;
     const i64 id = (i64)blockIdx.x * 256 + threadIdx.x, chunk = id / nvec;
     if (chunk >= chunks) return;
-    const int f = (int)(id - chunk * nvec) * V, F = (int)p.F;
+    const int f = (int)(id - chunk * nvec) * V;
     const int used = p.start[p.V];
-    const i64 lo = chunk * p.L, hi = lo + p.L < used ? lo + p.L : used;
+    const i64 lo = chunk * p.L;
     if (lo >= used) return;
+    const int many = (int)(used - lo < p.L ? used - lo : p.L);
+    const int *keys = p.key + lo, *poss = p.pos + lo;
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f;
-    int v = p.key[lo];
-    bool from_before = lo > 0 && p.key[lo - 1] == v;
-    for (i64 i0 = lo; i0 < hi; i0 += 4) {
-        float e[4][V];
-        int next[4];
+    int key[U], pos[U], v = keys[0];
+    bool from_before = lo > 0 && keys[-1] == v;
+    const bool goes_on = lo + many < used && keys[many] == keys[many - 1];      // the last word of the chunk
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            next[u] = i0 + u + 1 < hi ? p.key[i0 + u + 1] : -1;
-            if (i0 + u >= hi) continue;
-            const i64 at = p.pos[i0 + u] * p.e1;
-            if constexpr (V == 1) ld_f<DT, 1, true>(p.e, at + f * p.e0, e[u]);
-            else if (aligned) ld_f<DT, V, true>(p.e, at + f, e[u]);
-            else {
-                u32 w[4];
-                get_part<DT, V>(p.e, at, f, F, w);
-                cvt_in<DT, V>(w, e[u]);
-            }
+    for (int u = 0; u < U; ++u) if (u < many) { key[u] = keys[u]; pos[u] = poss[u]; }
+    for (int i0 = 0; i0 < many; i0 += U) {
+        u32 w[U][W];
+        int now[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            now[u] = key[u];
+            if (i0 + u >= many) continue;
+            const i64 at = pos[u] * p.e1;
+            if constexpr (V == 1) ld_w<DT, 1, true>(p.e, at + f * p.e0, w[u]);
+            else if (aligned) ld_w<DT, V, true>(p.e, at + f, w[u]);
+            else get_part<DT, V>(p.e, at, f, F, w[u]);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (i0 + u >= hi) break;
+        for (int u = 0; u < U; ++u) if (i0 + U + u < many) { key[u] = keys[i0 + U + u]; pos[u] = poss[i0 + U + u]; }
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum[i] += e[u][i];
-            if (next[u] == v) continue;
-            const bool goes_on = next[u] < 0 && hi < used && p.key[hi] == v;
-            if (from_before || goes_on) {
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u >= many) break;
+            float e[V];
+            cvt_in<DT, V>(w[u], e);
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] += e[i];
+            const bool last = i0 + u + 1 == many;
+            const int next = last ? -1 : u + 1 < U ? now[u + 1 < U ? u + 1 : 0] : key[0];
+            if (next == v) continue;
+            if (from_before || (last && goes_on)) {
                 float* to = p.part + (chunk * 2 + (from_before ? 0 : 1)) * F + f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) if (f + i < F) to[i] = sum[i];
@@ -369,69 +406,92 @@ __global__ void __launch_bounds__(256) lut_chunks(const __grid_constant__ SumP p
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) sum[i] = 0.f;
-            v = next[u];
+            v = next;
             from_before = false;
         }
     }
 }
 
-// 64 words x 32 V features per block: words without a position are cleared (or scaled), words that
-// cross a border between chunks get their partial sums added, each warp over an eighth of the
-// chunks, the warps in their order.
-template <int V>
-__global__ void __launch_bounds__(256) lut_finish(const __grid_constant__ SumP p) {
-    grid_enter();
-    __shared__ int start[65];
-    __shared__ float s[8][32 * V + 1];
-    const i64 v0 = (i64)blockIdx.x * 64;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, f = (blockIdx.y * 32 + lane) * V, F = (int)p.F;
-    const int words = (int)(p.V - v0 < 64 ? p.V - v0 : 64);
-    if (threadIdx.x <= words) start[threadIdx.x] = p.start[v0 + threadIdx.x];
-    __syncthreads();
-    float zero[V];
+// The partial sums of chunks [from, to) of a word that begins in chunk c0, features f ... f + V - 1.
+template <int V> DEV void add_parts(const SumP& p, i64 c0, i64 from, i64 to, int f, int F, float (&sum)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) zero[i] = 0.f;
-    if (p.beta != 1.f)
-        for (int k = warp; k < words; k += 8)
-            if (start[k] == start[k + 1] && f < F) put_dw<V>(p, v0 + k, f, zero);
-    for (int k = 0; k < words; ++k) {
-        const int lo = start[k], hi = start[k + 1];
-        if (lo == hi || lo / p.L == (hi - 1) / p.L) continue;
-        const i64 c0 = lo / p.L, c1 = (hi - 1) / p.L, per = (c1 - c0 + 8) / 8;
-        const i64 from = c0 + warp * per, to = from + per < c1 + 1 ? from + per : c1 + 1;
-        float sum[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] = 0.f;
-        if (f < F) {
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
+    if (f >= F) return;
+    if (V == 4 && F % 4 == 0) {
 #pragma unroll 4
-            for (i64 c = from; c < to; ++c) {
-                const float* at = p.part + (c * 2 + (c == c0 ? 1 : 0)) * F + f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) if (f + i < F) sum[i] += at[i];
-            }
+        for (i64 c = from; c < to; ++c) {
+            const float4 x = *reinterpret_cast<const float4*>(p.part + (c * 2 + (c == c0 ? 1 : 0)) * F + f);
+            sum[0] += x.x; sum[1 % V] += x.y; sum[2 % V] += x.z; sum[3 % V] += x.w;
         }
-        __syncthreads();
+    } else {
+        for (i64 c = from; c < to; ++c) {
+            const float* at = p.part + (c * 2 + (c == c0 ? 1 : 0)) * F + f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[warp][lane * V + i] = sum[i];
-        __syncthreads();
-        if (warp == 0 && f < F) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sum[i] = 0.f;
-                for (int w = 0; w < 8; ++w) sum[i] += s[w][lane * V + i];
-            }
-            put_dw<V>(p, v0 + k, f, sum);
+            for (int i = 0; i < V; ++i) if (f + i < F) sum[i] += at[i];
         }
     }
 }
 
+// Words that cross a border between chunks, at the first border they cross.  A block looks at 16
+// borders, and at 32 V features of the words it finds: a warp each adds up the words of up to 16
+// chunks, then the block as a whole the longer ones, each warp over an eighth of the chunks, the
+// warps in their order.
+template <int V>
+__global__ void __launch_bounds__(256) lut_cross(const __grid_constant__ SumP p, i64 borders) {
+    grid_enter();
+    __shared__ float s[8][32 * V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, f = (blockIdx.y * 32 + lane) * V, F = (int)p.F;
+    const i64 mine = (i64)blockIdx.x * 16 + lane;      // the chunk before the border
+    bool owner = false;
+    int word = 0, hi = 0;
+    if (lane < 16 && mine < borders) {
+        const i64 at = (mine + 1) * p.L;
+        word = p.key[at];
+        if (word < p.V && p.key[at - 1] == word) {
+            hi = p.start[word + 1];
+            owner = p.start[word] >= mine * p.L;
+        }
+    }
+    const bool is_long = owner && (hi - 1) / p.L - mine >= 16;
+    unsigned found = __ballot_sync(0xffffffffu, owner && !is_long), rest = __ballot_sync(0xffffffffu, is_long);
+    float sum[V];
+    for (int k = 0; found; ++k) {                      // the same in every warp
+        const int l = __ffs(found) - 1;
+        found &= found - 1;
+        if ((k & 7) != warp) continue;
+        const int v = __shfl_sync(0xffffffffu, word, l), end = __shfl_sync(0xffffffffu, hi, l);
+        const i64 c0 = (i64)blockIdx.x * 16 + l;
+        add_parts<V>(p, c0, c0, (end - 1) / p.L + 1, f, F, sum);
+        if (f < F) put_dw<V>(p, v, f, sum);
+    }
+    while (rest) {
+        const int l = __ffs(rest) - 1;
+        rest &= rest - 1;
+        const int v = __shfl_sync(0xffffffffu, word, l), end = __shfl_sync(0xffffffffu, hi, l);
+        const i64 c0 = (i64)blockIdx.x * 16 + l, c1 = (end - 1) / p.L, per = (c1 - c0 + 8) / 8;
+        const i64 from = c0 + warp * per, to = from + per < c1 + 1 ? from + per : c1 + 1;
+        add_parts<V>(p, c0, from, to, f, F, sum);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[warp][i * 32 + lane] = sum[i];
+        __syncthreads();
+        if (warp || f >= F) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            for (int w = 1; w < 8; ++w) sum[i] += s[w][i * 32 + lane];
+        put_dw<V>(p, v, f, sum);
+    }
+}
+
 template <int DT, int V> cudaError_t launch_chunks(const SumP& p, i64 chunks, bool aligned, cudaStream_t s) {
-    const i64 nvec = (p.F + V - 1) / V, grid = (chunks * nvec + 255) / 256;
-    return launch_dependent(lut_chunks<DT, V>, dim3((unsigned)grid), 256, 0, s, p, chunks, (int)nvec, (int)aligned);
+    const i64 nvec = (p.F + V - 1) / V, sums = (chunks * nvec + 255) / 256;
+    i64 fill = p.beta == 1.f ? 0 : ((i64)p.V + 255) / 256;
+    if (fill > 148 * 16) fill = 148 * 16;
+    if (!(sums + fill)) return cudaSuccess;
+    return launch_dependent(lut_chunks<DT, V>, dim3((unsigned)(sums + fill)), 256, 0, s, p, chunks, (int)nvec, (int)aligned, (unsigned)sums);
 }
 template <int DT> cudaError_t launch_sums(const SumP& p, i64 chunks, cudaStream_t s) {
     constexpr int V = 16 / dt_size<DT>::value;
-    if (!chunks) return cudaSuccess;
     if (p.e0 != 1 && p.F != 1) return launch_chunks<DT, 1>(p, chunks, false, s);
     return launch_chunks<DT, V>(p, chunks, p.e % 16 == 0 && p.e1 % V == 0 && p.F % V == 0, s);
 }
@@ -447,15 +507,16 @@ Plan plan(i64 V, i64 F, i64 N) {
     q.tiles = (N + kTile - 1) / kTile;
     q.passes = 1;
     while ((V >> (kDigitBits * q.passes)) != 0) ++q.passes;
-    // chunks of 64 places (512 bytes of partials per column against 64 elements read), longer
-    // where the partial sums would outgrow their share of the scratch
-    q.L = 64;
+    // chunks of 8 to 64 places: as long as leaves a thread for 8 features of each chunk on every
+    // one of 148 x 1024 places for threads; longer where the partial sums would outgrow their scratch
+    q.L = 8;
+    while (q.L < 64 && N / (2 * q.L) * ((F + 7) / 8) >= 148 * 1024) q.L *= 2;
     while ((N + q.L - 1) / q.L * 8 * F > kPartBytes && q.L < N) q.L *= 2;
     q.chunks = (N + q.L - 1) / q.L;
     i64 at = 0;
     auto take = [&at](i64 bytes) { const i64 r = at; at += (bytes + 255) & ~255ll; return r; };
     for (int k = 0; k < 2; ++k) { q.key[k] = take(4 * N); q.pos[k] = take(4 * N); }
-    q.hist = take(4 * kDigits * q.tiles);
+    q.hist = take(4 * kDigits * (q.tiles + 1));
     q.start = take(4 * (V + 1));
     q.part = take(8 * F * q.chunks);
     q.bytes = at;
@@ -532,7 +593,7 @@ extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, co
     cudaError_t e = cudaSuccess;
     if (positions && positions <= kRankMost) {
         t.first = 1; t.shift = 0; t.key_in = t.pos_in = nullptr; t.key_out = ints(q.key[0]); t.pos_out = ints(q.pos[0]);
-        e = launch_dependent(sort_rank, dim3((unsigned)(positions + 31) / 32), 256, 0, s, t);
+        e = launch_dependent(sort_rank, dim3((unsigned)(positions + 31) / 32), 512, 0, s, t);
         ++count;
     } else if (positions) {
         for (int k = 0; k < q.passes && e == cudaSuccess; ++k) {
@@ -540,7 +601,7 @@ extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, co
             t.key_in = ints(q.key[from]); t.pos_in = ints(q.pos[from]);
             t.key_out = ints(q.key[1 - from]); t.pos_out = ints(q.pos[1 - from]);
             e = launch_dependent(sort_count, dim3((unsigned)q.tiles), kSortThreads, 0, s, t);
-            if (e == cudaSuccess) e = launch_dependent(sort_scan, dim3(1), 1024, 0, s, t.hist, (int)(kDigits * q.tiles));
+            if (e == cudaSuccess) e = launch_dependent(sort_scan, dim3(kDigits / 8), 256, 0, s, t.hist, (int)q.tiles);
             if (e == cudaSuccess) e = launch_dependent(sort_move, dim3((unsigned)q.tiles), kSortThreads, 0, s, t);
             from = 1 - from;
             count += 3;
@@ -560,12 +621,14 @@ extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, co
         else if (p.edt == B200_F16) e = launch_sums<F16>(p, q.chunks, s);
         else e = launch_sums<BF16>(p, q.chunks, s);
     }
-    // four features per thread in the last kernel, or one where dW's features are not neighbours
-    const int V = dtable->s1 == 1 ? 4 : 1;
-    const dim3 grid((unsigned)((words + 63) / 64), (unsigned)((features + 32 * V - 1) / (32 * V)));
-    if (e == cudaSuccess)
-        e = V == 4 ? launch_dependent(lut_finish<4>, grid, 256, 0, s, p) : launch_dependent(lut_finish<1>, grid, 256, 0, s, p);
-    if (launches) *launches = count + (positions ? 3 : 2);
+    int last = 0;
+    if (e == cudaSuccess && q.chunks > 1) {
+        const int V = features >= 128 ? 4 : 1;         // features per thread
+        const dim3 grid((unsigned)((q.chunks + 14) / 16), (unsigned)((features + 32 * V - 1) / (32 * V)));
+        e = V == 4 ? launch_dependent(lut_cross<4>, grid, 256, 0, s, p, q.chunks - 1) : launch_dependent(lut_cross<1>, grid, 256, 0, s, p, q.chunks - 1);
+        last = 1;
+    }
+    if (launches) *launches = count + 1 + (q.chunks || beta != 1.f ? 1 : 0) + last;
     return cuda_status(where, e);
 }
 
