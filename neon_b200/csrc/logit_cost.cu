@@ -12,10 +12,9 @@
 //     cost  = w (kl (exp(d) - d - 1) - min(r A, clip(r, 1 - lo, 1 + hi) A))
 //     delta_v = s ([v = a] - q_v)    s = w (kl (1 - exp(d)) - r A [r A is the smaller one])
 //
-// Both read every logit for the softmax and then touch K (or one) of them again.  The softmax is
-// kept in base 2: with c = log2(e) / T and M = fl(c max z), s = sum 2^(z c - M) uses the same
-// rounded M as the gradient's 2^(z c - M) / s, so that M's rounding cancels there, and
-// ln sum exp(z / T) = max z / T + ln s - ln 2 (c max z - M) takes it out of the cost.
+// Both read every logit for the softmax and then touch K (or one) of them again.  Exponentials are
+// taken in base 2 of differences to the largest logit m, 2^((z_v - m) c) with c = log2(e) / T, so
+// nothing overflows whatever the logits' offset; s is their sum, q_v = 2^((z_v - m) c) / s.
 //
 // An item of weight 0, an item whose word lies outside the vocabulary and a teacher's list
 // without a usable entry (words outside, or logits of -inf) give cost 0 and delta 0, whatever
@@ -48,92 +47,87 @@ struct CostP {
     float lo, hi, kl;
 };
 
-// What an item's gradient needs besides the logits: delta_v = scale 2^(z_v c - M) for the words
-// without an entry of their own.
-struct Item { float M, scale; bool dead; };
+// What an item's gradient needs besides the logits: delta_v = scale 2^((z_v - m) c) for the words
+// without an entry of their own; 0 for all if dead.
+struct Item { float m, scale; int dead; };
 
-// Shared memory of one item: the word numbers, probabilities and finished gradients of its entries.
-struct Entries { int* id; float* p; float* g; float* red; };
+// One item's entries: word, log-probability at the teacher's (-inf: no entry), student's logit.
+struct Entries { int* id; float* lp; float* z; };
 
 DEV float weight_of(const CostP& p, i64 n) { return p.weights ? reinterpret_cast<const float*>(p.weights)[n] : 1.f; }
 
 // Items that need not be looked at: their cost and delta are zero.
-DEV bool skipped(const CostP& p, i64 n, bool policy) {
-    if (weight_of(p, n) == 0.f && !(policy && p.logp)) return true;
-    if (policy) {
+template <bool POLICY> DEV bool skipped(const CostP& p, i64 n) {
+    if (weight_of(p, n) == 0.f && !(POLICY && p.logp)) return true;
+    if (POLICY) {
         const int a = reinterpret_cast<const int*>(p.actions)[n];
         return a < 0 || a >= p.V;
     }
     return false;
 }
-
-// The entries of one item, by all threads of its block, once the logits' maximum and sum are known.
-DEV Item distill_entries(const CostP& p, i64 n, float zmax, float s, const Entries& e) {
-    const int tid = threadIdx.x, nt = blockDim.x;
-    Item it;
-    it.M = zmax * p.c;
-    const float w = weight_of(p, n);
-    const float ln_s = logf(s) - fmaf(zmax, p.c, -it.M) * 0.693147182464599609375f;
-    float m = -INFINITY;
-    for (int k = tid; k < p.K; k += nt) {
-        const int id = *(reinterpret_cast<const int*>(p.ids) + k * p.i0 + n * p.i1);
-        float t = ld_any(p.top, k * p.t0 + n * p.t1, p.tdt);
-        const bool used = id >= 0 && id < p.V && t != -INFINITY;
-        e.id[k] = used ? id : -1;
-        e.p[k] = t;
-        if (used) m = fmaxf(m, t);
-    }
-    // a NaN among the teacher's logits reaches the sum below whatever the maximum says
-    m = block_max(m, e.red);
-    float sum = 0.f;
-    int used = 0;
-    for (int k = tid; k < p.K; k += nt) {
-        if (e.id[k] < 0) { e.p[k] = 0.f; continue; }
-        used = 1;
-        e.p[k] = (e.p[k] - m) * p.inv_temp;
-        sum += expf(e.p[k]);
-    }
-    sum = block_sum(sum, e.red);
-    const bool any = __syncthreads_or(used);
-    it.dead = w == 0.f || !any;
-    it.scale = w * p.temp / s;
-    const float ln_sum = logf(sum);
-    float cost = 0.f;
-    for (int k = tid; k < p.K; k += nt) {
-        float zk = 0.f;
-        if (e.id[k] >= 0) {
-            zk = ld_any(p.z, (i64)e.id[k] * p.z0 + n * p.z1, p.dt);
-            const float lp = e.p[k] - ln_sum, pk = expf(lp);
-            e.p[k] = pk;
-            if (pk != 0.f) cost += pk * (lp - ((zk - zmax) * p.inv_temp - ln_s));
-        }
-        e.g[k] = zk;
-    }
-    cost = block_sum(cost, e.red);
-    if (tid == 0) reinterpret_cast<float*>(p.cost)[n] = it.dead ? 0.f : w * p.temp * p.temp * cost;
-    if (p.d) {
-        // a word listed more than once: all of its entries hold (and later write) the same value
-        __syncthreads();
-        for (int k = tid; k < p.K; k += nt) {
-            const int id = e.id[k];
-            if (id < 0) continue;
-            float mass = 0.f;
-            for (int j = 0; j < p.K; ++j) mass += e.id[j] == id ? e.p[j] : 0.f;
-            e.g[k] = it.scale * exp2f(fmaf(e.g[k], p.c, -it.M)) - w * p.temp * mass;
-        }
-        __syncthreads();
-    }
-    return it;
+template <bool POLICY> DEV void put_skipped(const CostP& p, i64 n) {
+    reinterpret_cast<float*>(p.cost)[n] = 0.f;
+    if (POLICY && p.logp) reinterpret_cast<float*>(p.logp)[n] = 0.f;
 }
 
-DEV Item policy_entry(const CostP& p, i64 n, float zmax, float s, const Entries& e) {
+// The maximum of a running softmax as the exponentials use it: items (or parts of one) that hold
+// nothing but -inf so far take differences to 0, which leaves their exponentials at 0 and a NaN a NaN.
+DEV float usable(float m) { return m == -INFINITY ? 0.f : m; }
+DEV float exp_of(float z, float m, float c) { return ex2_approx((z - m) * c); }
+// Teacher's entries of one item, by one warp: words, log-probabilities, and the student's logits
+// there.  Nothing here needs the student's softmax.
+DEV void read_entries(const CostP& p, i64 n, const Entries& e) {
+    const int lane = threadIdx.x & 31;
+    float top = -INFINITY;
+    for (int k = lane; k < p.K; k += 32) {
+        const int id = *(reinterpret_cast<const int*>(p.ids) + k * p.i0 + n * p.i1);
+        const float t = ld_any(p.top, k * p.t0 + n * p.t1, p.tdt);
+        const bool used = id >= 0 && id < p.V && t != -INFINITY;
+        e.id[k] = used ? id : -1;
+        e.lp[k] = t;
+        e.z[k] = used ? ld_any(p.z, (i64)id * p.z0 + n * p.z1, p.dt) : 0.f;
+        if (used) top = fmaxf(top, t);
+    }
+    top = usable(warp_max(top));                       // (a NaN reaches the sum whatever the maximum says)
+    float sum = 0.f;
+    for (int k = lane; k < p.K; k += 32)
+        if (e.id[k] >= 0) sum += expf((e.lp[k] - top) * p.inv_temp);
+    const float ln_sum = logf(warp_sum(sum));
+    for (int k = lane; k < p.K; k += 32) e.lp[k] = e.id[k] >= 0 ? (e.lp[k] - top) * p.inv_temp - ln_sum : -INFINITY;
+}
+
+// The item's cost, by one warp (all lanes), from its entries and its logits' maximum and sum.
+DEV Item distill_item(const CostP& p, i64 n, float m, float s, const Entries& e) {
+    const float w = weight_of(p, n), ln_s = logf(s);
+    float cost = 0.f;
+    int any = 0;
+    for (int k = threadIdx.x & 31; k < p.K; k += 32) {
+        if (e.id[k] < 0) continue;
+        any = 1;
+        const float lp = e.lp[k], pk = expf(lp);
+        if (pk != 0.f) cost += pk * (lp - ((e.z[k] - m) * p.inv_temp - ln_s));
+    }
+    cost = warp_sum(cost);
+    any = __any_sync(0xffffffffu, any);
     Item it;
-    it.M = zmax * p.c;
-    const float w = weight_of(p, n);
-    const int a = reinterpret_cast<const int*>(p.actions)[n];
-    const float za = ld_any(p.z, (i64)a * p.z0 + n * p.z1, p.dt);
-    const float ln_s = logf(s) - fmaf(zmax, p.c, -it.M) * 0.693147182464599609375f;
-    const float l = (za - zmax) - ln_s;
+    it.m = usable(m);
+    it.dead = w == 0.f || !any;
+    it.scale = w * p.temp / s;
+    if ((threadIdx.x & 31) == 0) reinterpret_cast<float*>(p.cost)[n] = it.dead ? 0.f : w * p.temp * p.temp * cost;
+    return it;
+}
+// The gradient at an entry's word: a word listed more than once collects all its entries, so each
+// of them holds the same value.
+DEV float entry_delta(const CostP& p, const Item& it, float w, const Entries& e, int k) {
+    const int id = e.id[k];
+    float mass = 0.f;
+    for (int j = 0; j < p.K; ++j) if (e.id[j] == id) mass += expf(e.lp[j]);
+    return it.scale * exp_of(e.z[k], it.m, p.c) - w * p.temp * mass;
+}
+
+// Policy: cost and log-probability of one item; `at_word`: the gradient at the word chosen.
+DEV Item policy_item(const CostP& p, i64 n, float m, float s, float za, bool put, float& at_word) {
+    const float w = weight_of(p, n), l = (za - m) - logf(s);
     const float adv = reinterpret_cast<const float*>(p.adv)[n];
     const float r = expf(l - reinterpret_cast<const float*>(p.old)[n]);
     const float free = r * adv, held = fminf(fmaxf(r, 1.f - p.lo), 1.f + p.hi) * adv;
@@ -145,59 +139,201 @@ DEV Item policy_entry(const CostP& p, i64 n, float zmax, float s, const Entries&
         slope -= p.kl * m1;
     }
     slope *= w;
+    Item it;
+    it.m = usable(m);
     it.dead = w == 0.f;
     it.scale = -slope / s;
-    if (threadIdx.x == 0) {
+    at_word = fmaf(it.scale, exp_of(za, it.m, p.c), slope);
+    if (put) {
         reinterpret_cast<float*>(p.cost)[n] = it.dead ? 0.f : w * cost;
         if (p.logp) reinterpret_cast<float*>(p.logp)[n] = l;
-        e.id[0] = a;
-        e.g[0] = fmaf(it.scale, exp2f(fmaf(za, p.c, -it.M)), slope);
     }
-    __syncthreads();
     return it;
 }
 
-// ---- any strides: a block per item, one logit per thread and step
-template <bool POLICY>
-__global__ void __launch_bounds__(256) cost_any(const __grid_constant__ CostP p) {
-    __shared__ float red[32];
-    __shared__ int ids[POLICY ? 1 : kMaxTop];
-    __shared__ float probs[POLICY ? 1 : kMaxTop], grads[POLICY ? 1 : kMaxTop];
-    const Entries e = {ids, probs, grads, red};
-    const int entries = POLICY ? 1 : p.K;
-    for (i64 n = blockIdx.x; n < p.N; n += gridDim.x) {
-        __syncthreads();                               // the entries of the previous item are written
-        Item it;
-        it.dead = skipped(p, n, POLICY);
-        if (it.dead) {
-            if (threadIdx.x == 0) {
-                reinterpret_cast<float*>(p.cost)[n] = 0.f;
-                if (POLICY && p.logp) reinterpret_cast<float*>(p.logp)[n] = 0.f;
+// ---- any strides, and words next to each other (their stride is 1)
+//
+// A block per item, items from a persistent grid.  The first walk over the logits keeps a running
+// maximum and sum per thread (rescaled when a group of vectors holds a larger logit, which is rare
+// after the first), the second writes the gradient.  The second read comes from L2: the rows under
+// way, at most 512 KB times the blocks that fit on the GPU, stay there, so HBM sees one read and
+// one write.  Meanwhile one warp reads the teacher's entries.  DT >= 0: 16-byte vectors, the first of which starts at
+// the boundary at or before the row; DT < 0: one logit at a time with any strides.
+template <int DT> struct Words {                       // loads and stores of one vector of a row
+    static constexpr int V = 16 / dt_size<DT>::value;
+    u32 w[4];
+    DEV void load(const CostP& p, i64 row, int f) {
+        ld_w<DT, V, false>(p.z, row + f, w);
+        if (f < 0 || f + V > p.V) {                    // -inf where there is no word
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if ((unsigned)(f + i) < (unsigned)p.V) continue;
+                if constexpr (DT == F32) w[i] = 0xff800000u;
+                else {
+                    const u32 low = DT == F16 ? 0xfc00u : 0xff80u;
+                    w[i >> 1] = i & 1 ? (w[i >> 1] & 0xffffu) | low << 16 : (w[i >> 1] & 0xffff0000u) | low;
+                }
             }
-        } else {
-            float m = -INFINITY;
-            for (int v = threadIdx.x; v < p.V; v += blockDim.x) m = fmaxf(m, ld_any(p.z, v * p.z0 + n * p.z1, p.dt));
-            m = block_max(m, red);
-            const float M = m * p.c;
-            float s = 0.f;
-            for (int v = threadIdx.x; v < p.V; v += blockDim.x) s += exp2f(fmaf(ld_any(p.z, v * p.z0 + n * p.z1, p.dt), p.c, -M));
-            s = block_sum(s, red);
-            it = POLICY ? policy_entry(p, n, m, s, e) : distill_entries(p, n, m, s, e);
         }
-        if (!p.d) continue;
-        for (int v = threadIdx.x; v < p.V; v += blockDim.x) {
-            const float z = ld_any(p.z, v * p.z0 + n * p.z1, p.dt);
-            st_any(p.d, v * p.d0 + n * p.d1, p.dt, it.dead ? 0.f : it.scale * exp2f(fmaf(z, p.c, -it.M)));
-        }
-        if (it.dead) continue;
-        __syncthreads();
-        for (int k = threadIdx.x; k < entries; k += blockDim.x)
-            if (e.id[k] >= 0)
-                st_any(p.d, (i64)e.id[k] * p.d0 + n * p.d1, p.dt, e.g[k]);
+    }
+};
+// the largest of four vectors' elements (NaN is passed over)
+DEV u32 max_pair(u32 a, u32 b, int dt) {
+    u32 r;
+    if (dt == F16) asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <int DT, int U> DEV float top_of(const Words<DT> (&x)[U]) {
+    if constexpr (DT == F32) {
+        float m = __uint_as_float(x[0].w[0]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = fmaxf(m, __uint_as_float(x[u].w[i]));
+        return m;
+    } else {
+        u32 m = x[0].w[0];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = max_pair(m, x[u].w[i], DT);
+        float lo, hi;
+        split(get2<DT>(&m, 0), lo, hi);
+        return fmaxf(lo, hi);
     }
 }
 
-unsigned blocks_for(i64 n) { return (unsigned)(n < 65536 ? n : 65536); }
+template <bool POLICY, int DT>
+__global__ void __launch_bounds__(512) cost_rows(const __grid_constant__ CostP p) {
+    constexpr bool VEC = DT >= 0;
+    constexpr int D = VEC ? DT : 0, V = VEC ? 16 / dt_size<D>::value : 1, U = 4;
+    // [2][3][K], and below [2][32]: an item's are read and written while others use the last one's;
+    // the barrier of the item in between keeps two uses of one half apart
+    extern __shared__ float entries[];
+    __shared__ float2 red[64];
+    const int tid = threadIdx.x, T = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = T >> 5;
+    int turn = 0;
+    for (i64 n = blockIdx.x; n < p.N; n += gridDim.x) {
+        const bool skip = skipped<POLICY>(p, n);
+        Item it;
+        float za = 0.f, at_word = 0.f;
+        const i64 row = n * p.z1, drow = n * p.d1;
+        int mis = 0, nvec = p.V;
+        if constexpr (VEC) {
+            mis = (int)((p.z / dt_size<D>::value + (u64)row) % V);
+            nvec = (p.V + mis + V - 1) / V;
+        }
+        Entries e;
+        e.id = reinterpret_cast<int*>(entries) + turn * 3 * p.K;
+        e.lp = entries + (turn * 3 + 1) * p.K;
+        e.z = entries + (turn * 3 + 2) * p.K;
+        if (skip) {
+            it.dead = 1;
+            if (tid == 0) put_skipped<POLICY>(p, n);
+        } else {
+            if (POLICY) za = ld_any(p.z, reinterpret_cast<const int*>(p.actions)[n] * p.z0 + row, p.dt);
+            else if (warp == 0) read_entries(p, n, e);
+            float m = -INFINITY, s = 0.f;
+            if constexpr (VEC) {
+                f32x2 sum = 0;
+                const f32x2 c2 = pair(p.c, p.c);
+                for (int k0 = tid; k0 < nvec; k0 += T * U) {
+                    Words<D> x[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        if (k0 + u * T < nvec) x[u].load(p, row, (k0 + u * T) * V - mis);
+                        else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[u].w[i] = D == F32 ? 0xff800000u : D == F16 ? 0xfc00fc00u : 0xff80ff80u;
+                        }
+                    }
+                    const float top = top_of<D, U>(x);
+                    if (top > m) {
+                        const float f = exp_of(m, top, p.c);
+                        sum = mul2(sum, pair(f, f));
+                        m = top;
+                    }
+                    const float t = usable(m);
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int i = 0; i < V / 2; ++i) {
+                            float lo, hi;
+                            split(mul2(less2<D>(x[u].w, i, t), c2), lo, hi);
+                            sum = add2(sum, pair(ex2_approx(lo), ex2_approx(hi)));
+                        }
+                }
+                s = both(sum);
+            } else {
+                for (int v = tid; v < p.V; v += T) {
+                    const float z = ld_any(p.z, v * p.z0 + row, p.dt);
+                    if (z > m) { s *= exp_of(m, z, p.c); m = z; }
+                    s += exp_of(z, usable(m), p.c);
+                }
+            }
+            // one maximum and sum for the block
+            const float top = warp_max(m);
+            s = warp_sum(s * exp_of(m, usable(top), p.c));
+            if (lane == 0) red[turn * 32 + warp] = make_float2(top, s);
+            __syncthreads();
+            const float2 part = lane < warps ? red[turn * 32 + lane] : make_float2(-INFINITY, 0.f);
+            m = warp_max(part.x);
+            s = warp_sum(part.y * exp_of(part.x, usable(m), p.c));
+            turn ^= 1;
+            if (POLICY) it = policy_item(p, n, m, s, za, tid == 0, at_word);
+            else {
+                if (warp == 0) it = distill_item(p, n, m, s, e);
+                if (p.d) {
+                    // what all need for the gradient, without waiting for the cost
+                    const float w = weight_of(p, n);
+                    int any = 0;
+                    for (int k = lane; k < p.K; k += 32) any |= e.id[k] >= 0;
+                    it.m = usable(m);
+                    it.dead = w == 0.f || !__any_sync(0xffffffffu, any);
+                    it.scale = w * p.temp / s;
+                }
+            }
+        }
+        if (!p.d) continue;
+        if constexpr (VEC) {
+            const f32x2 c2 = pair(p.c, p.c), scale = pair(it.scale, it.scale);
+            for (int k0 = tid; k0 < nvec; k0 += T * U) {
+                Words<D> x[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (k0 + u * T >= nvec || it.dead) x[u].w[0] = x[u].w[1] = x[u].w[2] = x[u].w[3] = 0;
+                    else ld_w<D, V, false>(p.z, row + (k0 + u * T) * V - mis, x[u].w);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (k0 + u * T >= nvec) break;
+                    if (!it.dead) {
+#pragma unroll
+                        for (int i = 0; i < V / 2; ++i) {
+                            float lo, hi;
+                            split(mul2(less2<D>(x[u].w, i, it.m), c2), lo, hi);
+                            set2<D>(x[u].w, i, mul2(scale, pair(ex2_approx(lo), ex2_approx(hi))));
+                        }
+                    }
+                    put_part<D, V>(p.d, drow, (k0 + u * T) * V - mis, p.V, x[u].w);
+                }
+            }
+        } else {
+            for (int v = tid; v < p.V; v += T)
+                st_any(p.d, v * p.d0 + drow, p.dt, it.dead ? 0.f : it.scale * exp_of(ld_any(p.z, v * p.z0 + row, p.dt), it.m, p.c));
+        }
+        __syncthreads();                               // the entries' words have been written with the others
+        if (it.dead) continue;
+        if (POLICY) {
+            if (tid == 0) st_any(p.d, reinterpret_cast<const int*>(p.actions)[n] * p.d0 + drow, p.dt, at_word);
+        } else {
+            const float w = weight_of(p, n);
+            for (int k = tid; k < p.K; k += T)
+                if (e.id[k] >= 0) st_any(p.d, e.id[k] * p.d0 + drow, p.dt, entry_delta(p, it, w, e, k));
+        }
+    }
+}
 
 b200_matrix vec(uint64_t ptr, int dt) { b200_matrix m; m.ptr = ptr; m.s0 = 1; m.s1 = 1; m.dtype = dt; m.reserved = 0; return m; }
 
@@ -232,14 +368,33 @@ int32_t check(const char* where, const b200_matrix* z, const b200_matrix* d, i64
     return B200_OK;
 }
 
+template <bool POLICY, int DT> cudaError_t launch_rows(const CostP& p, cudaStream_t s) {
+    constexpr int V = DT >= 0 ? 16 / dt_size<DT >= 0 ? DT : 0>::value : 1;
+    // as many threads as have two vectors each, up to 512
+    const i64 pairs = ((i64)p.V + 2 * V - 1) / (2 * V);
+    const int T = pairs >= 512 ? 512 : (int)(pairs + 31) / 32 * 32, smem = POLICY ? 0 : 6 * p.K * 4;
+    const i64 most = resident_blocks(cost_rows<POLICY, DT>, T, smem);
+    if (!most) return cudaErrorInvalidConfiguration;
+    cost_rows<POLICY, DT><<<(unsigned)(p.N < most ? p.N : most), T, smem, s>>>(p);
+    return cudaGetLastError();
+}
+
 template <bool POLICY>
 int32_t run(const char* where, CostP& p, uint64_t stream, int32_t* launches) {
     DeviceScope scope;
     if (scope.error() != cudaSuccess) return cuda_status(where, scope.error());
     cudaStream_t s = static_cast<cudaStream_t>(b200_detail_stream(stream));
-    cost_any<POLICY><<<blocks_for(p.N), 256, 0, s>>>(p);
+    // vectors: words next to each other, and logits and delta alike to the 16-byte boundaries
+    const int V = 16 / (int)esize(p.dt);
+    const bool rows = (p.z0 == 1 || p.V == 1) &&
+        (!p.d || ((p.d0 == 1 || p.V == 1) && (p.z - p.d) % 16 == 0 && (p.z1 - p.d1) % V == 0));
+    cudaError_t e;
+    if (!rows) e = launch_rows<POLICY, -1>(p, s);
+    else if (p.dt == B200_F32) e = launch_rows<POLICY, F32>(p, s);
+    else if (p.dt == B200_F16) e = launch_rows<POLICY, F16>(p, s);
+    else e = launch_rows<POLICY, BF16>(p, s);
     if (launches) *launches = 1;
-    return cuda_status(where, cudaGetLastError());
+    return cuda_status(where, e);
 }
 
 void set_logits(CostP& p, const b200_matrix* z, const b200_matrix* d, i64 V, i64 N, uint64_t weights, uint64_t cost) {
