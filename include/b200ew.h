@@ -273,9 +273,11 @@ b200_status b200_lut_bprop(uint64_t ids, const b200_matrix *error, const b200_ma
  * lies outside the vocabulary or whose logit is -inf are left out; an item of weight 0 or without
  * an entry has cost 0 and delta 0. */
 #define B200_DISTILL_MAX_TOP 1024
+uint64_t    b200_cost_scratch_bytes(int64_t words, int64_t items, int64_t top);   /* of either cost; policy: top 1 */
 b200_status b200_distill(const b200_matrix *logits, const b200_matrix *delta, const b200_matrix *top_ids,
                          const b200_matrix *top_logits, uint64_t weights, uint64_t cost, int64_t words,
-                         int64_t items, int64_t top, float temperature, uint64_t stream, int32_t *launches);
+                         int64_t items, int64_t top, float temperature, uint64_t scratch,
+                         uint64_t scratch_bytes, uint64_t stream, int32_t *launches);
 
 /* clipped policy cost: with l the log-probability of the item's word actions[n] (int32; written to
  * logp when that is given), r = exp(l - old_logp) and d = ref_logp - l, cost[n] = weights[n] *
@@ -285,7 +287,7 @@ b200_status b200_distill(const b200_matrix *logits, const b200_matrix *delta, co
 b200_status b200_policy(const b200_matrix *logits, const b200_matrix *delta, uint64_t actions, uint64_t old_logp,
                         uint64_t ref_logp, uint64_t advantages, uint64_t weights, uint64_t cost, uint64_t logp,
                         int64_t words, int64_t items, float clip_low, float clip_high, float kl_coef,
-                        uint64_t stream, int32_t *launches);
+                        uint64_t scratch, uint64_t scratch_bytes, uint64_t stream, int32_t *launches);
 
 /* ---- the same reduction for callers that cannot allocate device memory
  * No counterpart in the reference.  Meant for hosts where cudaMalloc is off

@@ -75,10 +75,11 @@ template <bool POLICY> DEV void put_skipped(const CostP& p, i64 n) {
 DEV float usable(float m) { return m == -INFINITY ? 0.f : m; }
 DEV float exp_of(float z, float m, float c) { return ex2_approx((z - m) * c); }
 // Teacher's entries of one item, by one warp: words, log-probabilities, and the student's logits
-// there.  Nothing here needs the student's softmax.
-DEV void read_entries(const CostP& p, i64 n, const Entries& e) {
+// there.  Nothing here needs the student's softmax.  Returns whether there is a usable one.
+DEV bool read_entries(const CostP& p, i64 n, const Entries& e) {
     const int lane = threadIdx.x & 31;
     float top = -INFINITY;
+    int any = 0;
     for (int k = lane; k < p.K; k += 32) {
         const int id = *(reinterpret_cast<const int*>(p.ids) + k * p.i0 + n * p.i1);
         const float t = ld_any(p.top, k * p.t0 + n * p.t1, p.tdt);
@@ -86,42 +87,50 @@ DEV void read_entries(const CostP& p, i64 n, const Entries& e) {
         e.id[k] = used ? id : -1;
         e.lp[k] = t;
         e.z[k] = used ? ld_any(p.z, (i64)id * p.z0 + n * p.z1, p.dt) : 0.f;
-        if (used) top = fmaxf(top, t);
+        if (used) { top = fmaxf(top, t); any = 1; }
     }
+    if (lane < 3 && p.K + lane < (p.K + 3) / 4 * 4) e.id[p.K + lane] = -1;
     top = usable(warp_max(top));                       // (a NaN reaches the sum whatever the maximum says)
     float sum = 0.f;
     for (int k = lane; k < p.K; k += 32)
         if (e.id[k] >= 0) sum += expf((e.lp[k] - top) * p.inv_temp);
     const float ln_sum = logf(warp_sum(sum));
     for (int k = lane; k < p.K; k += 32) e.lp[k] = e.id[k] >= 0 ? (e.lp[k] - top) * p.inv_temp - ln_sum : -INFINITY;
+    return __any_sync(0xffffffffu, any);
 }
 
-// The item's cost, by one warp (all lanes), from its entries and its logits' maximum and sum.
-DEV Item distill_item(const CostP& p, i64 n, float m, float s, const Entries& e) {
-    const float w = weight_of(p, n), ln_s = logf(s);
+// The item's cost, by one warp, from its entries and its logits' maximum and sum.
+DEV void distill_cost(const CostP& p, i64 n, float m, float s, bool dead, const Entries& e) {
+    const float ln_s = logf(s);
     float cost = 0.f;
-    int any = 0;
     for (int k = threadIdx.x & 31; k < p.K; k += 32) {
         if (e.id[k] < 0) continue;
-        any = 1;
         const float lp = e.lp[k], pk = expf(lp);
         if (pk != 0.f) cost += pk * (lp - ((e.z[k] - m) * p.inv_temp - ln_s));
     }
     cost = warp_sum(cost);
-    any = __any_sync(0xffffffffu, any);
-    Item it;
-    it.m = usable(m);
-    it.dead = w == 0.f || !any;
-    it.scale = w * p.temp / s;
-    if ((threadIdx.x & 31) == 0) reinterpret_cast<float*>(p.cost)[n] = it.dead ? 0.f : w * p.temp * p.temp * cost;
-    return it;
+    if ((threadIdx.x & 31) == 0) reinterpret_cast<float*>(p.cost)[n] = dead ? 0.f : weight_of(p, n) * p.temp * p.temp * cost;
+}
+DEV Item distill_item(const CostP& p, i64 n, float m, float s, bool any) {
+    const float w = weight_of(p, n);
+    return Item{usable(m), w * p.temp / s, w == 0.f || !any};
 }
 // The gradient at an entry's word: a word listed more than once collects all its entries, so each
-// of them holds the same value.
+// of them holds the same value.  e.id is 16-byte aligned and padded with -1 to a multiple of 4.
 DEV float entry_delta(const CostP& p, const Item& it, float w, const Entries& e, int k) {
     const int id = e.id[k];
-    float mass = 0.f;
-    for (int j = 0; j < p.K; ++j) if (e.id[j] == id) mass += expf(e.lp[j]);
+    float mass = expf(e.lp[k]);
+    int same = 0;
+    const int4* four = reinterpret_cast<const int4*>(e.id);
+#pragma unroll 4
+    for (int j = 0; j < (p.K + 3) / 4; ++j) {
+        const int4 x = four[j];
+        same += (x.x == id) + (x.y == id) + (x.z == id) + (x.w == id);
+    }
+    if (same > 1) {
+        mass = 0.f;
+        for (int j = 0; j < p.K; ++j) if (e.id[j] == id) mass += expf(e.lp[j]);
+    }
     return it.scale * exp_of(e.z[k], it.m, p.c) - w * p.temp * mass;
 }
 
@@ -139,10 +148,7 @@ DEV Item policy_item(const CostP& p, i64 n, float m, float s, float za, bool put
         slope -= p.kl * m1;
     }
     slope *= w;
-    Item it;
-    it.m = usable(m);
-    it.dead = w == 0.f;
-    it.scale = -slope / s;
+    const Item it = {usable(m), -slope / s, w == 0.f};
     at_word = fmaf(it.scale, exp_of(za, it.m, p.c), slope);
     if (put) {
         reinterpret_cast<float*>(p.cost)[n] = it.dead ? 0.f : w * cost;
@@ -151,188 +157,444 @@ DEV Item policy_item(const CostP& p, i64 n, float m, float s, float za, bool put
     return it;
 }
 
-// ---- any strides, and words next to each other (their stride is 1)
-//
-// A block per item, items from a persistent grid.  The first walk over the logits keeps a running
-// maximum and sum per thread (rescaled when a group of vectors holds a larger logit, which is rare
-// after the first), the second writes the gradient.  The second read comes from L2: the rows under
-// way, at most 512 KB times the blocks that fit on the GPU, stay there, so HBM sees one read and
-// one write.  Meanwhile one warp reads the teacher's entries.  DT >= 0: 16-byte vectors, the first of which starts at
-// the boundary at or before the row; DT < 0: one logit at a time with any strides.
-template <int DT> struct Words {                       // loads and stores of one vector of a row
-    static constexpr int V = 16 / dt_size<DT>::value;
-    u32 w[4];
-    DEV void load(const CostP& p, i64 row, int f) {
-        ld_w<DT, V, false>(p.z, row + f, w);
-        if (f < 0 || f + V > p.V) {                    // -inf where there is no word
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if ((unsigned)(f + i) < (unsigned)p.V) continue;
-                if constexpr (DT == F32) w[i] = 0xff800000u;
-                else {
-                    const u32 low = DT == F16 ? 0xfc00u : 0xff80u;
-                    w[i >> 1] = i & 1 ? (w[i >> 1] & 0xffffu) | low << 16 : (w[i >> 1] & 0xffff0000u) | low;
-                }
+// ---- any strides: a block per item, one logit per thread and step
+template <bool POLICY>
+__global__ void __launch_bounds__(256) cost_any(const __grid_constant__ CostP p) {
+    extern __shared__ __align__(16) float entries[];   // [3][K4]
+    __shared__ float red[32];
+    __shared__ int found;
+    const int tid = threadIdx.x;
+    const int K4 = (p.K + 3) / 4 * 4;
+    const Entries e = {reinterpret_cast<int*>(entries), entries + K4, entries + 2 * K4};
+    for (i64 n = blockIdx.x; n < p.N; n += gridDim.x) {
+        __syncthreads();                               // the last item's entries are written
+        const i64 row = n * p.z1, drow = n * p.d1;
+        Item it = {0.f, 0.f, 1};
+        float at_word = 0.f;
+        if (skipped<POLICY>(p, n)) {
+            if (tid == 0) put_skipped<POLICY>(p, n);
+        } else {
+            if (!POLICY && tid < 32) {
+                const bool any = read_entries(p, n, e);
+                if (tid == 0) found = any;
+            }
+            float m = -INFINITY, s = 0.f;
+            for (int v = tid; v < p.V; v += 256) m = fmaxf(m, ld_any(p.z, v * p.z0 + row, p.dt));
+            m = block_max(m, red);
+            for (int v = tid; v < p.V; v += 256) s += exp_of(ld_any(p.z, v * p.z0 + row, p.dt), usable(m), p.c);
+            s = block_sum(s, red);
+            if (POLICY) {
+                const float za = ld_any(p.z, reinterpret_cast<const int*>(p.actions)[n] * p.z0 + row, p.dt);
+                it = policy_item(p, n, m, s, za, tid == 0, at_word);
+                __syncthreads();                       // all have read the word's logit, which delta may overwrite
+            } else {
+                it = distill_item(p, n, m, s, found);
+                if (tid < 32) distill_cost(p, n, m, s, it.dead, e);
             }
         }
+        if (!p.d) continue;
+        for (int v = tid; v < p.V; v += 256)
+            st_any(p.d, v * p.d0 + drow, p.dt, it.dead ? 0.f : it.scale * exp_of(ld_any(p.z, v * p.z0 + row, p.dt), it.m, p.c));
+        if (it.dead) continue;
+        __syncthreads();                               // the entries' words have been written with the others
+        if (POLICY) {
+            if (tid == 0) st_any(p.d, reinterpret_cast<const int*>(p.actions)[n] * p.d0 + drow, p.dt, at_word);
+        } else {
+            for (int k = tid; k < p.K; k += 256)
+                if (e.id[k] >= 0) st_any(p.d, e.id[k] * p.d0 + drow, p.dt, entry_delta(p, it, weight_of(p, n), e, k));
+        }
     }
-};
-// the largest of four vectors' elements (NaN is passed over)
-DEV u32 max_pair(u32 a, u32 b, int dt) {
+}
+
+// ---- words next to each other (their stride is 1)
+//
+// A block per row, rows from a persistent grid.  The first walk over a row keeps a running maximum
+// and sum per thread, rescaled when four vectors hold a larger logit, which is rare after the first;
+// the second writes the gradient, and reads the row from L2.  The 16-byte vectors start at the
+// boundary at or before the row, `mis` words early; the first and the last, which may hold words of
+// other rows, belong to one thread each.  Blocks are small, so that several rows per SM are at
+// different points of their way: loads, exponentials and barriers of one run under the stores of
+// another.
+DEV u32 max_pair(u32 a, u32 b, int dt) {              // NaN is passed over
     u32 r;
     if (dt == F16) asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     else asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-template <int DT, int U> DEV float top_of(const Words<DT> (&x)[U]) {
+template <int DT, int U> DEV float top_of(const u32 (&w)[U][4]) {
     if constexpr (DT == F32) {
-        float m = __uint_as_float(x[0].w[0]);
+        float m = __uint_as_float(w[0][0]);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m = fmaxf(m, __uint_as_float(x[u].w[i]));
+            for (int i = 0; i < 4; ++i) m = fmaxf(m, __uint_as_float(w[u][i]));
         return m;
     } else {
-        u32 m = x[0].w[0];
+        u32 m = w[0][0];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m = max_pair(m, x[u].w[i], DT);
+            for (int i = 0; i < 4; ++i) m = max_pair(m, w[u][i], DT);
         float lo, hi;
         split(get2<DT>(&m, 0), lo, hi);
         return fmaxf(lo, hi);
     }
 }
+// A thread's share of a running softmax: maximum, and pairs of sums.
+struct Running { float m; f32x2 a, b; };
+template <int DT, int U> DEV void take(Running& r, const u32 (&w)[U][4], float c) {
+    const float top = top_of<DT, U>(w);
+    if (top > r.m) {
+        const float f = exp_of(r.m, top, c);
+        r.a = mul2(r.a, pair(f, f));
+        r.b = mul2(r.b, pair(f, f));
+        r.m = top;
+    }
+    const float t = usable(r.m);
+    const f32x2 less = pair(-t, -t), c2 = pair(c, c);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int l = 0; l < 8 / dt_size<DT>::value; ++l) {
+            float lo, hi;
+            split(mul2(add2(get2<DT>(w[u], l), less), c2), lo, hi);
+            f32x2& to = l & 1 ? r.b : r.a;
+            to = add2(to, pair(ex2_approx(lo), ex2_approx(hi)));
+        }
+}
+// The gradient of a vector of logits, in place.
+template <int DT> DEV void give(u32* w, const Item& it, float c) {
+    const f32x2 less = pair(-it.m, -it.m), c2 = pair(c, c), scale = pair(it.scale, it.scale);
+#pragma unroll
+    for (int l = 0; l < 8 / dt_size<DT>::value; ++l) {
+        float lo, hi;
+        split(mul2(add2(get2<DT>(w, l), less), c2), lo, hi);
+        set2<DT>(w, l, mul2(scale, pair(ex2_approx(lo), ex2_approx(hi))));
+    }
+}
+// A vector at the end of a row, with -inf where there is no word.
+template <int DT> DEV void load_end(u32 (&w)[1][4], const char* at, int f, int words) {
+    constexpr int V = 16 / dt_size<DT>::value;
+    constexpr u32 LOW = DT == F32 ? 0xff800000u : DT == F16 ? 0xfc00fc00u : 0xff80ff80u;
+    ld_raw<16, false>(at, w[0]);
+#pragma unroll
+    for (int l = 0; l < V; ++l) {
+        if ((unsigned)(f + l) < (unsigned)words) continue;
+        if constexpr (DT == F32) w[0][l] = LOW;
+        else w[0][l >> 1] = l & 1 ? (w[0][l >> 1] & 0xffffu) | (LOW & 0xffff0000u) : (w[0][l >> 1] & 0xffff0000u) | (LOW & 0xffffu);
+    }
+}
 
-template <bool POLICY, int DT>
-__global__ void __launch_bounds__(512) cost_rows(const __grid_constant__ CostP p) {
-    constexpr bool VEC = DT >= 0;
-    constexpr int D = VEC ? DT : 0, V = VEC ? 16 / dt_size<D>::value : 1, U = 4;
-    // [2][3][K], and below [2][32]: an item's are read and written while others use the last one's;
-    // the barrier of the item in between keeps two uses of one half apart
-    extern __shared__ float entries[];
-    __shared__ float2 red[64];
+template <bool POLICY, int DT, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ CostP p) {
+    constexpr int SZ = dt_size<DT>::value, V = 16 / SZ, U = 4;
+    // [2][3][K4] and below [2]: these alternate from item to item; the barriers of the item in between
+    // keep two uses of one half apart
+    extern __shared__ __align__(16) float entries[];
+    __shared__ float2 red[2][32];
+    __shared__ int found[2];
     const int tid = threadIdx.x, T = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = T >> 5;
+    const int jump = T * 16;                           // bytes from one of a thread's vectors to the next
+    const int K4 = (p.K + 3) / 4 * 4;
     int turn = 0;
     for (i64 n = blockIdx.x; n < p.N; n += gridDim.x) {
         const bool skip = skipped<POLICY>(p, n);
-        Item it;
-        float za = 0.f, at_word = 0.f;
-        const i64 row = n * p.z1, drow = n * p.d1;
-        int mis = 0, nvec = p.V;
-        if constexpr (VEC) {
-            mis = (int)((p.z / dt_size<D>::value + (u64)row) % V);
-            nvec = (p.V + mis + V - 1) / V;
-        }
+        Item it = {0.f, 0.f, 1};
+        const int mis = (int)(p.z / SZ + (u64)(n * p.z1)) & (V - 1);
+        const int nvec = (p.V + mis + V - 1) / V, inner = nvec - 2;         // all but the first and the last
+        const int count = inner > tid ? (inner - 1 - tid) / T + 1 : 0;
+        const i64 drow = n * p.d1;
+        const char* row = reinterpret_cast<const char*>(p.z) + (n * p.z1 - mis) * SZ;
+        const char* mine = row + (i64)(1 + tid) * 16;
+        // the ends belong to the first and the last thread
+        const bool end = tid == 0 || (tid == T - 1 && nvec > 1);
+        const int k_end = tid == 0 ? 0 : nvec - 1;
+        float at_word = 0.f;
         Entries e;
-        e.id = reinterpret_cast<int*>(entries) + turn * 3 * p.K;
-        e.lp = entries + (turn * 3 + 1) * p.K;
-        e.z = entries + (turn * 3 + 2) * p.K;
+        e.id = reinterpret_cast<int*>(entries) + turn * 3 * K4;
+        e.lp = entries + (turn * 3 + 1) * K4;
+        e.z = entries + (turn * 3 + 2) * K4;
         if (skip) {
-            it.dead = 1;
             if (tid == 0) put_skipped<POLICY>(p, n);
         } else {
-            if (POLICY) za = ld_any(p.z, reinterpret_cast<const int*>(p.actions)[n] * p.z0 + row, p.dt);
-            else if (warp == 0) read_entries(p, n, e);
-            float m = -INFINITY, s = 0.f;
-            if constexpr (VEC) {
-                f32x2 sum = 0;
-                const f32x2 c2 = pair(p.c, p.c);
-                for (int k0 = tid; k0 < nvec; k0 += T * U) {
-                    Words<D> x[U];
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        if (k0 + u * T < nvec) x[u].load(p, row, (k0 + u * T) * V - mis);
-                        else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) x[u].w[i] = D == F32 ? 0xff800000u : D == F16 ? 0xfc00fc00u : 0xff80ff80u;
-                        }
-                    }
-                    const float top = top_of<D, U>(x);
-                    if (top > m) {
-                        const float f = exp_of(m, top, p.c);
-                        sum = mul2(sum, pair(f, f));
-                        m = top;
-                    }
-                    const float t = usable(m);
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int i = 0; i < V / 2; ++i) {
-                            float lo, hi;
-                            split(mul2(less2<D>(x[u].w, i, t), c2), lo, hi);
-                            sum = add2(sum, pair(ex2_approx(lo), ex2_approx(hi)));
-                        }
-                }
-                s = both(sum);
-            } else {
-                for (int v = tid; v < p.V; v += T) {
-                    const float z = ld_any(p.z, v * p.z0 + row, p.dt);
-                    if (z > m) { s *= exp_of(m, z, p.c); m = z; }
-                    s += exp_of(z, usable(m), p.c);
-                }
+            float za = 0.f;
+            if (POLICY) za = ld_any(p.z, reinterpret_cast<const int*>(p.actions)[n] + n * p.z1, DT);
+            else if (warp == 0) {
+                const bool any = read_entries(p, n, e);
+                if (lane == 0) found[turn] = any;
             }
-            // one maximum and sum for the block
-            const float top = warp_max(m);
-            s = warp_sum(s * exp_of(m, usable(top), p.c));
-            if (lane == 0) red[turn * 32 + warp] = make_float2(top, s);
+            Running r = {-INFINITY, 0, 0};
+            const char* at = mine;
+            int i = 0;
+            for (; i + U <= count; i += U, at += U * jump) {
+                u32 w[U][4];
+#pragma unroll
+                for (int u = 0; u < U; ++u) ld_raw<16, false>(at + u * jump, w[u]);
+                take<DT, U>(r, w, p.c);
+            }
+            for (; i < count; ++i, at += jump) {
+                u32 w[1][4];
+                ld_raw<16, false>(at, w[0]);
+                take<DT, 1>(r, w, p.c);
+            }
+            if (end) {
+                u32 w[1][4];
+                load_end<DT>(w, row + (i64)k_end * 16, k_end * V - mis, p.V);
+                take<DT, 1>(r, w, p.c);
+            }
+            // one maximum and sum for the row
+            float m = warp_max(r.m), s = warp_sum(both(add2(r.a, r.b)) * exp_of(r.m, usable(m), p.c));
+            if (lane == 0) red[turn][warp] = make_float2(m, s);
             __syncthreads();
-            const float2 part = lane < warps ? red[turn * 32 + lane] : make_float2(-INFINITY, 0.f);
+            const float2 part = lane < warps ? red[turn][lane] : make_float2(-INFINITY, 0.f);
             m = warp_max(part.x);
             s = warp_sum(part.y * exp_of(part.x, usable(m), p.c));
-            turn ^= 1;
             if (POLICY) it = policy_item(p, n, m, s, za, tid == 0, at_word);
             else {
-                if (warp == 0) it = distill_item(p, n, m, s, e);
-                if (p.d) {
-                    // what all need for the gradient, without waiting for the cost
-                    const float w = weight_of(p, n);
-                    int any = 0;
-                    for (int k = lane; k < p.K; k += 32) any |= e.id[k] >= 0;
-                    it.m = usable(m);
-                    it.dead = w == 0.f || !__any_sync(0xffffffffu, any);
-                    it.scale = w * p.temp / s;
-                }
+                it = distill_item(p, n, m, s, found[turn]);
+                if (warp == 0) distill_cost(p, n, m, s, it.dead, e);
             }
         }
-        if (!p.d) continue;
-        if constexpr (VEC) {
-            const f32x2 c2 = pair(p.c, p.c), scale = pair(it.scale, it.scale);
-            for (int k0 = tid; k0 < nvec; k0 += T * U) {
-                Words<D> x[U];
+        if (p.d) {
+            char* to = reinterpret_cast<char*>(p.d) + (drow - mis) * SZ + (i64)(1 + tid) * 16;
+            const char* at = mine;
+            if (it.dead) {
+                const u32 none[4] = {0, 0, 0, 0};
+                for (int i = 0; i < count; ++i, to += jump) st_raw<16>(to, none);
+                if (end) put_part<DT, V>(p.d, drow, k_end * V - mis, p.V, none);
+                if (!skip) __syncthreads();            // all have read the word's logit, which delta may overwrite
+            } else {
+                int i = 0;
+                for (; i + U <= count; i += U, at += U * jump, to += U * jump) {
+                    u32 w[U][4];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (k0 + u * T >= nvec || it.dead) x[u].w[0] = x[u].w[1] = x[u].w[2] = x[u].w[3] = 0;
-                    else ld_w<D, V, false>(p.z, row + (k0 + u * T) * V - mis, x[u].w);
-                }
+                    for (int u = 0; u < U; ++u) ld_raw<16, false>(at + u * jump, w[u]);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (k0 + u * T >= nvec) break;
-                    if (!it.dead) {
-#pragma unroll
-                        for (int i = 0; i < V / 2; ++i) {
-                            float lo, hi;
-                            split(mul2(less2<D>(x[u].w, i, it.m), c2), lo, hi);
-                            set2<D>(x[u].w, i, mul2(scale, pair(ex2_approx(lo), ex2_approx(hi))));
-                        }
+                    for (int u = 0; u < U; ++u) {
+                        give<DT>(w[u], it, p.c);
+                        st_raw<16>(to + u * jump, w[u]);
                     }
-                    put_part<D, V>(p.d, drow, (k0 + u * T) * V - mis, p.V, x[u].w);
+                }
+                for (; i < count; ++i, at += jump, to += jump) {
+                    u32 w[4];
+                    ld_raw<16, false>(at, w);
+                    give<DT>(w, it, p.c);
+                    st_raw<16>(to, w);
+                }
+                if (end) {
+                    u32 w[4];
+                    ld_raw<16, false>(row + (i64)k_end * 16, w);
+                    give<DT>(w, it, p.c);
+                    put_part<DT, V>(p.d, drow, k_end * V - mis, p.V, w);
+                }
+                __syncthreads();                       // the entries' words have been written with the others
+                if (POLICY) {
+                    if (tid == 0) st_any(p.d, drow + reinterpret_cast<const int*>(p.actions)[n], DT, at_word);
+                } else {
+                    const float w = weight_of(p, n);
+                    for (int k = tid; k < p.K; k += T)
+                        if (e.id[k] >= 0) st_any(p.d, drow + e.id[k], DT, entry_delta(p, it, w, e, k));
                 }
             }
-        } else {
-            for (int v = tid; v < p.V; v += T)
-                st_any(p.d, v * p.d0 + drow, p.dt, it.dead ? 0.f : it.scale * exp_of(ld_any(p.z, v * p.z0 + row, p.dt), it.m, p.c));
         }
-        __syncthreads();                               // the entries' words have been written with the others
-        if (it.dead) continue;
-        if (POLICY) {
-            if (tid == 0) st_any(p.d, reinterpret_cast<const int*>(p.actions)[n] * p.d0 + drow, p.dt, at_word);
-        } else {
-            const float w = weight_of(p, n);
-            for (int k = tid; k < p.K; k += T)
-                if (e.id[k] >= 0) st_any(p.d, e.id[k] * p.d0 + drow, p.dt, entry_delta(p, it, w, e, k));
+        if (!skip) turn ^= 1;
+    }
+}
+
+// ---- items next to each other (their stride is 1; neon's own order)
+//
+// Four kernels per slice of items: (1) running maxima and sums, a thread V neighbouring items down a
+// share of the vocabulary, the shares joined per block and written per item; (2) a warp per item
+// joins them, and works out the cost and the gradient at the item's entries; (3) the gradient of
+// all words; (4) the entries' over it.  A slice is as many items as have room for their results in
+// the scratch, 45,000 at one entry.  HBM sees two reads and one write: slices small enough to be
+// read from L2 the second time were measured too and lost more to their launches than they saved
+// (50257 x 8192 bf16: 2125 us in slices of 48 MB, 518 us in one).
+struct ColsP {
+    CostP c;                             // of the slice
+    float2* part;                        // [splits][N] maximum and sum
+    float4* item;                        // [N] m, scale, dead
+    float* grad;                         // [K][N] gradient at the entries
+    int splits, rows;                    // words per split
+    int lanes;
+};
+enum { kSplits = 64, kColThreads = 256 };
+
+template <int DT, int V>
+__global__ void __launch_bounds__(kColThreads) cost_cols_stats(const __grid_constant__ ColsP p) {
+    grid_enter();
+    constexpr int U = 4;
+    __shared__ float2 red[kColThreads * V];
+    const int lanes = p.lanes, tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = kColThreads / lanes;
+    const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
+    const bool in = n < p.c.N;
+    const float c = p.c.c;
+    float m[V], s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) { m[i] = -INFINITY; s[i] = 0.f; }
+    const int lo = blockIdx.y * p.rows, hi = min(lo + p.rows, p.c.V);
+    if (in) {
+        for (int v0 = lo + ty; v0 < hi; v0 += rows * U) {
+            float z[U][V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (v0 + u * rows < hi) ld_f<DT, V, false>(p.c.z, (i64)(v0 + u * rows) * p.c.z0 + n, z[u]);
+                else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) z[u][i] = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float top = fmaxf(fmaxf(z[0][i], z[1][i]), fmaxf(z[2][i], z[3][i]));
+                if (top > m[i]) { s[i] *= exp_of(m[i], top, c); m[i] = top; }
+                const float t = usable(m[i]);
+#pragma unroll
+                for (int u = 0; u < U; ++u) s[i] += exp_of(z[u][i], t, c);
+            }
         }
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[(ty * lanes + tx) * V + i] = make_float2(m[i], s[i]);
+    __syncthreads();
+    const int wide = lanes * V;
+    for (int i = threadIdx.x; i < wide; i += kColThreads) {
+        const i64 item = (i64)blockIdx.x * wide + i;
+        if (item >= p.c.N) continue;
+        float top = -INFINITY, sum = 0.f;
+        for (int r = 0; r < rows; ++r) top = fmaxf(top, red[r * wide + i].x);
+        const float t = usable(top);
+        for (int r = 0; r < rows; ++r) sum += red[r * wide + i].y * exp_of(red[r * wide + i].x, t, c);
+        p.part[(i64)blockIdx.y * p.c.N + item] = make_float2(top, sum);
+    }
+}
+
+template <bool POLICY>
+__global__ void __launch_bounds__(32) cost_cols_items(const __grid_constant__ ColsP p) {
+    grid_enter();
+    extern __shared__ __align__(16) float entries[];   // [3][K4]
+    const CostP& c = p.c;
+    const i64 n = blockIdx.x;
+    const int lane = threadIdx.x;
+    Entries e;
+    e.id = reinterpret_cast<int*>(entries);
+    e.lp = entries + (c.K + 3) / 4 * 4;
+    e.z = entries + (c.K + 3) / 4 * 8;
+    Item it;
+    it.dead = 1;
+    it.m = it.scale = 0.f;
+    if (skipped<POLICY>(c, n)) {
+        if (lane == 0) put_skipped<POLICY>(c, n);
+    } else {
+        bool any = false;
+        if (!POLICY) any = read_entries(c, n, e);
+        float m = -INFINITY, s = 0.f;
+        for (int k = lane; k < p.splits; k += 32) m = fmaxf(m, p.part[(i64)k * c.N + n].x);
+        m = warp_max(m);
+        for (int k = lane; k < p.splits; k += 32) {
+            const float2 x = p.part[(i64)k * c.N + n];
+            s += x.y * exp_of(x.x, usable(m), c.c);
+        }
+        s = warp_sum(s);
+        __syncwarp();
+        if (POLICY) {
+            const float za = ld_any(c.z, reinterpret_cast<const int*>(c.actions)[n] * c.z0 + n * c.z1, c.dt);
+            float at_word;
+            it = policy_item(c, n, m, s, za, lane == 0, at_word);
+            if (c.d && lane == 0) p.grad[n] = at_word;
+        } else {
+            it = distill_item(c, n, m, s, any);
+            distill_cost(c, n, m, s, it.dead, e);
+            if (c.d && !it.dead) {
+                const float w = weight_of(c, n);
+                for (int k = lane; k < c.K; k += 32) if (e.id[k] >= 0) p.grad[(i64)k * c.N + n] = entry_delta(c, it, w, e, k);
+            }
+        }
+    }
+    if (c.d && lane == 0) p.item[n] = make_float4(it.m, it.scale, it.dead ? 1.f : 0.f, 0.f);
+}
+
+template <int DT, int V>
+__global__ void __launch_bounds__(kColThreads) cost_cols_delta(const __grid_constant__ ColsP p) {
+    grid_enter();
+    const int lanes = p.lanes, tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = kColThreads / lanes;
+    const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
+    if (n >= p.c.N) return;
+    const float c = p.c.c;
+    float m[V], scale[V];
+    bool dead[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float4 it = p.item[n + i];
+        m[i] = it.x; scale[i] = it.y; dead[i] = it.z != 0.f;
+    }
+    const int lo = blockIdx.y * p.rows, hi = min(lo + p.rows, p.c.V);
+#pragma unroll 4
+    for (int v = lo + ty; v < hi; v += rows) {
+        float z[V];
+        ld_f<DT, V, false>(p.c.z, (i64)v * p.c.z0 + n, z);
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = dead[i] ? 0.f : scale[i] * exp_of(z[i], m[i], c);
+        st_f<DT, V>(p.c.d, (i64)v * p.c.d0 + n, z);
+    }
+}
+
+template <bool POLICY>
+__global__ void __launch_bounds__(256) cost_cols_put(const __grid_constant__ ColsP p) {
+    grid_enter();
+    const CostP& c = p.c;
+    const i64 at = (i64)blockIdx.x * 256 + threadIdx.x;
+    const int k = (int)(at / c.N);
+    const i64 n = at - k * c.N;
+    if (k >= c.K || p.item[n].z != 0.f) return;
+    const int id = POLICY ? reinterpret_cast<const int*>(c.actions)[n] : *(reinterpret_cast<const int*>(c.ids) + k * c.i0 + n * c.i1);
+    if (id < 0 || id >= c.V) return;
+    if (!POLICY && ld_any(c.top, k * c.t0 + n * c.t1, c.tdt) == -INFINITY) return;
+    st_any(c.d, id * c.d0 + n * c.d1, c.dt, p.grad[at]);
+}
+
+// Items per slice whose results fit the scratch, a multiple of 256.
+inline i64 slice_fit(i64 K) { return (24ll << 20) / (8 * kSplits + 16 + 4 * K) / 256 * 256; }
+
+template <bool POLICY, int DT, int V> cudaError_t launch_cols(const CostP& all, char* scratch, int& launches, cudaStream_t s) {
+    constexpr int size = dt_size<DT>::value;
+    i64 slice = slice_fit(all.K);
+    if (slice > (all.N + 255) / 256 * 256) slice = (all.N + 255) / 256 * 256;
+    for (i64 n0 = 0; n0 < all.N; n0 += slice) {
+        ColsP p;
+        p.c = all;
+        CostP& c = p.c;
+        c.N = all.N - n0 < slice ? all.N - n0 : slice;
+        auto move = [n0](u64 ptr, i64 bytes) { return ptr ? ptr + (u64)(n0 * bytes) : 0; };
+        c.z = move(all.z, all.z1 * size); c.d = move(all.d, all.d1 * size);
+        c.weights = move(all.weights, 4); c.cost = move(all.cost, 4); c.actions = move(all.actions, 4); c.old = move(all.old, 4);
+        c.ref = move(all.ref, 4); c.adv = move(all.adv, 4); c.logp = move(all.logp, 4);
+        c.ids = move(all.ids, all.i1 * 4); c.top = move(all.top, all.t1 * esize(all.tdt));
+        // runs of up to 512 bytes of a word's row, down to 32 where there are few items
+        p.lanes = 32;
+        while (p.lanes > 1 && p.lanes * V * size > 32 && (i64)p.lanes * V / 2 >= c.N) p.lanes /= 2;
+        const int wide = p.lanes * V, rows = kColThreads / p.lanes;
+        const i64 across = (c.N + wide - 1) / wide;
+        i64 splits = (148 * 8 + across - 1) / across, most = ((i64)c.V + rows * 4 - 1) / (rows * 4);
+        if (splits > kSplits) splits = kSplits;
+        if (splits > most) splits = most;
+        p.rows = (int)(((i64)c.V + splits - 1) / splits);
+        p.splits = (int)(((i64)c.V + p.rows - 1) / p.rows);
+        p.part = reinterpret_cast<float2*>(scratch);
+        p.item = reinterpret_cast<float4*>(scratch + 8 * kSplits * slice);
+        p.grad = reinterpret_cast<float*>(scratch + (8 * kSplits + 16) * slice);
+        const dim3 grid((unsigned)across, (unsigned)p.splits);
+        cudaError_t e = launch_dependent(cost_cols_stats<DT, V>, grid, kColThreads, 0, s, p);
+        if (e == cudaSuccess) e = launch_dependent(cost_cols_items<POLICY>, dim3((unsigned)c.N), 32, POLICY ? 0 : 12 * ((c.K + 3) / 4 * 4), s, p);
+        launches += 2;
+        if (e == cudaSuccess && c.d) {
+            e = launch_dependent(cost_cols_delta<DT, V>, grid, kColThreads, 0, s, p);
+            if (e == cudaSuccess) e = launch_dependent(cost_cols_put<POLICY>, dim3((unsigned)((c.N * c.K + 255) / 256)), 256, 0, s, p);
+            launches += 2;
+        }
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 b200_matrix vec(uint64_t ptr, int dt) { b200_matrix m; m.ptr = ptr; m.s0 = 1; m.s1 = 1; m.dtype = dt; m.reserved = 0; return m; }
@@ -368,19 +630,34 @@ int32_t check(const char* where, const b200_matrix* z, const b200_matrix* d, i64
     return B200_OK;
 }
 
-template <bool POLICY, int DT> cudaError_t launch_rows(const CostP& p, cudaStream_t s) {
-    constexpr int V = DT >= 0 ? 16 / dt_size<DT >= 0 ? DT : 0>::value : 1;
-    // as many threads as have two vectors each, up to 512
-    const i64 pairs = ((i64)p.V + 2 * V - 1) / (2 * V);
-    const int T = pairs >= 512 ? 512 : (int)(pairs + 31) / 32 * 32, smem = POLICY ? 0 : 6 * p.K * 4;
-    const i64 most = resident_blocks(cost_rows<POLICY, DT>, T, smem);
-    if (!most) return cudaErrorInvalidConfiguration;
-    cost_rows<POLICY, DT><<<(unsigned)(p.N < most ? p.N : most), T, smem, s>>>(p);
+template <bool POLICY> cudaError_t launch_any(const CostP& p, cudaStream_t s) {
+    cost_any<POLICY><<<(unsigned)(p.N < 65536 ? p.N : 65536), 256, POLICY ? 0 : 12 * ((p.K + 3) / 4 * 4), s>>>(p);
     return cudaGetLastError();
 }
 
+template <bool POLICY, int DT> cudaError_t launch_rows(const CostP& p, cudaStream_t s) {
+    const i64 bytes = (i64)p.V * dt_size<DT>::value, nvec = bytes / 16 + 1;
+    const int smem = POLICY ? 0 : 24 * ((p.K + 3) / 4 * 4);
+    auto go = [&](auto kernel, int T) {
+        i64 most = resident_blocks(kernel, T, smem);
+        if (!most) return cudaErrorInvalidConfiguration;
+        kernel<<<(unsigned)(p.N < most ? p.N : most), T, smem, s>>>(p);
+        return cudaGetLastError();
+    };
+    if (bytes > 160000) return go(cost_rows<POLICY, DT, 512, 2>, 512);
+    int T = (int)(nvec / 8 + 31) / 32 * 32;
+    T = T < 32 ? 32 : T > 256 ? 256 : T;
+    return go(cost_rows<POLICY, DT, 256, 4>, T);
+}
+
+template <bool POLICY, int DT> cudaError_t launch_cols_width(const CostP& p, char* scratch, int& launches, cudaStream_t s) {
+    constexpr int V = 16 / dt_size<DT>::value;
+    const bool wide = p.z % 16 == 0 && p.z0 % V == 0 && p.N % V == 0 && (!p.d || (p.d % 16 == 0 && p.d0 % V == 0));
+    return wide ? launch_cols<POLICY, DT, V>(p, scratch, launches, s) : launch_cols<POLICY, DT, 1>(p, scratch, launches, s);
+}
+
 template <bool POLICY>
-int32_t run(const char* where, CostP& p, uint64_t stream, int32_t* launches) {
+int32_t run(const char* where, CostP& p, uint64_t scratch, uint64_t stream, int32_t* launches) {
     DeviceScope scope;
     if (scope.error() != cudaSuccess) return cuda_status(where, scope.error());
     cudaStream_t s = static_cast<cudaStream_t>(b200_detail_stream(stream));
@@ -388,12 +665,23 @@ int32_t run(const char* where, CostP& p, uint64_t stream, int32_t* launches) {
     const int V = 16 / (int)esize(p.dt);
     const bool rows = (p.z0 == 1 || p.V == 1) &&
         (!p.d || ((p.d0 == 1 || p.V == 1) && (p.z - p.d) % 16 == 0 && (p.z1 - p.d1) % V == 0));
+    const bool cols = (p.z1 == 1 || p.N == 1) && (!p.d || p.d1 == 1 || p.N == 1);
     cudaError_t e;
-    if (!rows) e = launch_rows<POLICY, -1>(p, s);
-    else if (p.dt == B200_F32) e = launch_rows<POLICY, F32>(p, s);
-    else if (p.dt == B200_F16) e = launch_rows<POLICY, F16>(p, s);
-    else e = launch_rows<POLICY, BF16>(p, s);
-    if (launches) *launches = 1;
+    int count = 1;
+    char* at = reinterpret_cast<char*>(scratch);
+    if (rows) {
+        if (p.dt == B200_F32) e = launch_rows<POLICY, F32>(p, s);
+        else if (p.dt == B200_F16) e = launch_rows<POLICY, F16>(p, s);
+        else e = launch_rows<POLICY, BF16>(p, s);
+    } else if (cols) {
+        count = 0;
+        if (p.dt == B200_F32) e = launch_cols_width<POLICY, F32>(p, at, count, s);
+        else if (p.dt == B200_F16) e = launch_cols_width<POLICY, F16>(p, at, count, s);
+        else e = launch_cols_width<POLICY, BF16>(p, at, count, s);
+    } else {
+        e = launch_any<POLICY>(p, s);
+    }
+    if (launches) *launches = count;
     return cuda_status(where, e);
 }
 
@@ -406,9 +694,16 @@ void set_logits(CostP& p, const b200_matrix* z, const b200_matrix* d, i64 V, i64
 
 }  // namespace
 
+extern "C" uint64_t b200_cost_scratch_bytes(int64_t words, int64_t items, int64_t top) {
+    if (words < 1 || items < 1 || top < 1 || top > kMaxTop) return 0;
+    const i64 fit = slice_fit(top), slice = items < fit ? (items + 255) / 256 * 256 : fit;
+    return (uint64_t)(slice * (8 * kSplits + 16 + 4 * top));
+}
+
 extern "C" b200_status b200_distill(const b200_matrix* logits, const b200_matrix* delta, const b200_matrix* top_ids,
                                     const b200_matrix* top_logits, uint64_t weights, uint64_t cost, int64_t words,
-                                    int64_t items, int64_t top, float temperature, uint64_t stream, int32_t* launches) {
+                                    int64_t items, int64_t top, float temperature, uint64_t scratch, uint64_t scratch_bytes,
+                                    uint64_t stream, int32_t* launches) {
     const char* where = "b200_distill";
     if (launches) *launches = 0;
     if (!logits || !top_ids || !top_logits) return refuse(where, "null matrix");
@@ -422,6 +717,7 @@ extern "C" b200_status b200_distill(const b200_matrix* logits, const b200_matrix
     if (!is_float(top_logits->dtype)) return refuse(where, "teacher's logits must be f32, f16 or bf16", B200_ERR_UNSUPPORTED);
     if (items == 0) return B200_OK;
     if (!top_ids->ptr || !top_logits->ptr) return refuse(where, "null device pointer");
+    if (!scratch || scratch % 256 || scratch_bytes < b200_cost_scratch_bytes(words, items, top)) return refuse(where, "scratch too small or misaligned");
     for (const b200_matrix* m : {top_ids, top_logits}) {
         if (!aligned(m->ptr, m->dtype)) return refuse(where, "misaligned pointer");
         if ((d->ptr && meet(*d, words, items, *m, top, items)) || meet(out[0], items, 1, *m, top, items))
@@ -433,13 +729,14 @@ extern "C" b200_status b200_distill(const b200_matrix* logits, const b200_matrix
     p.ids = top_ids->ptr; p.i0 = top_ids->s0; p.i1 = top_ids->s1;
     p.top = top_logits->ptr; p.t0 = top_logits->s0; p.t1 = top_logits->s1; p.tdt = top_logits->dtype;
     p.K = (int)top;
-    return run<false>(where, p, stream, launches);
+    return run<false>(where, p, scratch, stream, launches);
 }
 
 extern "C" b200_status b200_policy(const b200_matrix* logits, const b200_matrix* delta, uint64_t actions,
                                    uint64_t old_logp, uint64_t ref_logp, uint64_t advantages, uint64_t weights,
                                    uint64_t cost, uint64_t logp, int64_t words, int64_t items, float clip_low,
-                                   float clip_high, float kl_coef, uint64_t stream, int32_t* launches) {
+                                   float clip_high, float kl_coef, uint64_t scratch, uint64_t scratch_bytes,
+                                   uint64_t stream, int32_t* launches) {
     const char* where = "b200_policy";
     if (launches) *launches = 0;
     if (!logits) return refuse(where, "null matrix");
@@ -452,11 +749,12 @@ extern "C" b200_status b200_policy(const b200_matrix* logits, const b200_matrix*
     if (int32_t st = check(where, logits, d, words, items, in, 5, out, 2)) return st;
     if (items == 0) return B200_OK;
     if (!actions || !old_logp || !advantages) return refuse(where, "null device pointer");
+    if (!scratch || scratch % 256 || scratch_bytes < b200_cost_scratch_bytes(words, items, 1)) return refuse(where, "scratch too small or misaligned");
     if (kl_coef != 0.f && !ref_logp) return refuse(where, "a KL term needs the reference's log-probabilities");
     CostP p;
     set_logits(p, logits, d, words, items, weights, cost);
     p.temp = p.inv_temp = 1.f; p.c = 1.44269502162933349609375f;
     p.K = 1; p.actions = actions; p.old = old_logp; p.ref = kl_coef != 0.f ? ref_logp : 0; p.adv = advantages; p.logp = logp;
     p.lo = clip_low; p.hi = clip_high; p.kl = kl_coef;
-    return run<true>(where, p, stream, launches);
+    return run<true>(where, p, scratch, stream, launches);
 }

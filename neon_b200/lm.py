@@ -282,7 +282,9 @@ class LanguageModelOps(object):
             raise ValueError("cost must be a tensor")
         args = (self._lm_vector(weights, "weights", n, np.float32), self._lm_vector(cost, "cost", n, np.float32, out=True))
         self._lm_check(logits, delta, top_ids, top_logits, weights, cost)
-        self.launches += rt.distill(mz, md, mi, mt, *args, v, n, k, float(temperature), self.stream)
+        nbytes = rt.cost_scratch_bytes(v, n, k)
+        self.launches += rt.distill(mz, md, mi, mt, *args, v, n, k, float(temperature), self._lm_scratch(nbytes), nbytes,
+                                    self.stream)
         return cost
 
     def _lm_delta(self, delta, logits):
@@ -332,5 +334,7 @@ class LanguageModelOps(object):
                 vec(weights, "weights", n, np.float32), vec(cost, "cost", n, np.float32, out=True),
                 vec(logp, "logp", n, np.float32, out=True))
         self._lm_check(logits, delta, actions, old_logp, ref_logp, advantages, weights, cost, logp)
-        self.launches += rt.policy(mz, md, *args, v, n, float(low), float(high), float(kl_coef), self.stream)
+        nbytes = rt.cost_scratch_bytes(v, n, 1)
+        self.launches += rt.policy(mz, md, *args, v, n, float(low), float(high), float(kl_coef),
+                                   self._lm_scratch(nbytes), nbytes, self.stream)
         return cost

@@ -93,10 +93,11 @@ SIGNATURES = {
     "b200_lut_bprop_scratch_bytes": (u64, [C.c_int64, C.c_int64, C.c_int64]),
     "b200_lut_bprop": (i32, [u64, P(Matrix), P(Matrix), C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_float,
                              C.c_float, u64, u64, u64, P(i32)]),
+    "b200_cost_scratch_bytes": (u64, [C.c_int64, C.c_int64, C.c_int64]),
     "b200_distill": (i32, [P(Matrix), P(Matrix), P(Matrix), P(Matrix), u64, u64, C.c_int64, C.c_int64, C.c_int64,
-                           C.c_float, u64, P(i32)]),
+                           C.c_float, u64, u64, u64, P(i32)]),
     "b200_policy": (i32, [P(Matrix), P(Matrix), u64, u64, u64, u64, u64, u64, u64, C.c_int64, C.c_int64, C.c_float,
-                          C.c_float, C.c_float, u64, P(i32)]),
+                          C.c_float, C.c_float, u64, u64, u64, P(i32)]),
     "b200_reduce_full_noalloc_max_count": (u64, []),
     "b200_reduce_full_noalloc": (i32, [u64, i32, u64, i32, i32, u64, u64]),
     "b200_comm_unique_id": (i32, [P(C.c_uint8)]),
@@ -422,18 +423,23 @@ def lut_bprop(ids, error, dtable, words, features, positions, pad_idx, alpha, be
     return n.value
 
 
-def distill(logits, delta, top_ids, top_logits, weights, cost, words, items, top, temperature, stream=0):
+def cost_scratch_bytes(words, items, top):
+    return int(lib().b200_cost_scratch_bytes(words, items, top))
+
+
+def distill(logits, delta, top_ids, top_logits, weights, cost, words, items, top, temperature, scratch, scratch_bytes,
+            stream=0):
     n = i32(0)
     check(lib().b200_distill(logits, delta, top_ids, top_logits, weights, cost, words, items, top, temperature,
-                             stream, n))
+                             scratch, scratch_bytes, stream, n))
     return n.value
 
 
 def policy(logits, delta, actions, old_logp, ref_logp, advantages, weights, cost, logp, words, items, clip_low,
-           clip_high, kl_coef, stream=0):
+           clip_high, kl_coef, scratch, scratch_bytes, stream=0):
     n = i32(0)
     check(lib().b200_policy(logits, delta, actions, old_logp, ref_logp, advantages, weights, cost, logp, words,
-                            items, clip_low, clip_high, kl_coef, stream, n))
+                            items, clip_low, clip_high, kl_coef, scratch, scratch_bytes, stream, n))
     return n.value
 
 

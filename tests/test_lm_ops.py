@@ -13,9 +13,21 @@ from neon_b200.dryrun import DryRunBackend
 from tests import lm_reference as ref
 
 
+class Scratch(object):
+    """In the place of the backend's scratch memory, which a dry run does not have."""
+
+    def __call__(self, nbytes, zero):
+        return 1 << 40
+
+    def reset(self):
+        pass
+
+
 @pytest.fixture(scope="module")
 def be():
-    return DryRunBackend()
+    be = DryRunBackend()
+    be._scratch = Scratch()
+    return be
 
 
 def ln_args(be, f=8, n=6, dtype=np.float32):
@@ -64,14 +76,9 @@ def test_layer_norm_refusals(be):
     refused(TypeError, fn, b, "one type", grad_beta=be.empty((8, 1), np.float16))
     refused(TypeError, fn, b, "one type", gamma=be.empty((8, 1), np.float16))
     refused(NotImplementedError, fn, b, "stochastic", grad_gamma=rounding(be.empty((8, 1))))
-    be._scratch = lambda nbytes, zero: be._fake(nbytes)
-    be._scratch.reset = lambda: None
-    try:
-        refused(rt.B200Error, fn, b, "shares memory", grad_gamma=b["grad_beta"])
-        refused(rt.B200Error, fn, b, "shares memory", grad_gamma=b["x"].reshape(1, 48)[:, :8])
-        refused(rt.B200Error, fn, b, "shifted view", delta_out=buf[:, :6], x=buf[:, 3:9])
-    finally:
-        be._scratch = None
+    refused(rt.B200Error, fn, b, "shares memory", grad_gamma=b["grad_beta"])
+    refused(rt.B200Error, fn, b, "shares memory", grad_gamma=b["x"].reshape(1, 48)[:, :8])
+    refused(rt.B200Error, fn, b, "shifted view", delta_out=buf[:, :6], x=buf[:, 3:9])
 
 
 def test_lookup_refusals(be):
@@ -148,8 +155,8 @@ def test_entry_points_refuse_null_and_misaligned(be):
     assert lib.b200_ln_fprop(m, far, 0, 0, rt.I32, 0, 0, 8, 4, 1e-5, 0, None) == -7
     assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 8, -1, 1e-5, 0, None) == -1
     assert lib.b200_lut_bprop(1 << 22, m, far, 8, 8, 4, -1, 1.0, 0.0, 0, 0, 0, None) == -1 and "scratch" in rt.last_error()
-    assert lib.b200_distill(m, None, None, m, 0, 1 << 25, 8, 4, 2, 1.0, 0, None) == -1
-    assert lib.b200_policy(m, None, 0, 0, 0, 0, 0, 1 << 25, 0, 8, 4, 0.2, 0.2, 0.0, 0, None) == -1
+    assert lib.b200_distill(m, None, None, m, 0, 1 << 25, 8, 4, 2, 1.0, 0, 0, 0, None) == -1
+    assert lib.b200_policy(m, None, 0, 0, 0, 0, 0, 1 << 25, 0, 8, 4, 0.2, 0.2, 0.0, 0, 0, 0, None) == -1
     if rt.device_count() == 0:                       # a good call reports the missing device
         n = C.c_int32(5)
         assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 0, n) == -2 and n.value == 0
