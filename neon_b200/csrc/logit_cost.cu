@@ -65,6 +65,10 @@ template <bool POLICY> DEV bool skipped(const CostP& p, i64 n) {
     }
     return false;
 }
+// The same from values that were read ahead.
+template <bool POLICY> DEV bool skipped(const CostP& p, float w, int a) {
+    return (w == 0.f && !(POLICY && p.logp)) || (POLICY && (a < 0 || a >= p.V));
+}
 template <bool POLICY> DEV void put_skipped(const CostP& p, i64 n) {
     reinterpret_cast<float*>(p.cost)[n] = 0.f;
     if (POLICY && p.logp) reinterpret_cast<float*>(p.logp)[n] = 0.f;
@@ -74,28 +78,44 @@ template <bool POLICY> DEV void put_skipped(const CostP& p, i64 n) {
 // nothing but -inf so far take differences to 0, which leaves their exponentials at 0 and a NaN a NaN.
 DEV float usable(float m) { return m == -INFINITY ? 0.f : m; }
 DEV float exp_of(float z, float m, float c) { return ex2_approx((z - m) * c); }
-// Teacher's entries of one item, by one warp: words, log-probabilities, and the student's logits
-// there.  Nothing here needs the student's softmax.  Returns whether there is a usable one.
-DEV bool read_entries(const CostP& p, i64 n, const Entries& e) {
+// Teacher's entries of one item, by one warp: the words and both logits, then, from the logits in
+// e.lp, the log-probabilities.  Neither needs the student's softmax.
+DEV bool entry_used(const CostP& p, int id, float t) { return id >= 0 && id < p.V && t != -INFINITY; }
+DEV int entry_id(const CostP& p, i64 n, int k) { return *(reinterpret_cast<const int*>(p.ids) + k * p.i0 + n * p.i1); }
+DEV float entry_top(const CostP& p, i64 n, int k) { return ld_any(p.top, k * p.t0 + n * p.t1, p.tdt); }
+DEV void put_entry(const CostP& p, const Entries& e, int k, int id, float t, float z) {
+    const bool used = entry_used(p, id, t);
+    e.id[k] = used ? id : -1;
+    e.lp[k] = used ? t : -INFINITY;
+    e.z[k] = z;
+}
+DEV void pad_entries(const CostP& p, const Entries& e, int lane) {         // to a multiple of four
+    if (p.K + lane < (p.K + 3) / 4 * 4) e.id[p.K + lane] = -1;
+}
+DEV void teacher(const CostP& p, const Entries& e) {
     const int lane = threadIdx.x & 31;
-    float top = -INFINITY;
-    int any = 0;
-    for (int k = lane; k < p.K; k += 32) {
-        const int id = *(reinterpret_cast<const int*>(p.ids) + k * p.i0 + n * p.i1);
-        const float t = ld_any(p.top, k * p.t0 + n * p.t1, p.tdt);
-        const bool used = id >= 0 && id < p.V && t != -INFINITY;
-        e.id[k] = used ? id : -1;
-        e.lp[k] = t;
-        e.z[k] = used ? ld_any(p.z, (i64)id * p.z0 + n * p.z1, p.dt) : 0.f;
-        if (used) { top = fmaxf(top, t); any = 1; }
-    }
-    if (lane < 3 && p.K + lane < (p.K + 3) / 4 * 4) e.id[p.K + lane] = -1;
+    float top = -INFINITY, sum = 0.f;
+    for (int k = lane; k < p.K; k += 32) top = fmaxf(top, e.lp[k]);
     top = usable(warp_max(top));                       // (a NaN reaches the sum whatever the maximum says)
-    float sum = 0.f;
     for (int k = lane; k < p.K; k += 32)
         if (e.id[k] >= 0) sum += expf((e.lp[k] - top) * p.inv_temp);
     const float ln_sum = logf(warp_sum(sum));
-    for (int k = lane; k < p.K; k += 32) e.lp[k] = e.id[k] >= 0 ? (e.lp[k] - top) * p.inv_temp - ln_sum : -INFINITY;
+    for (int k = lane; k < p.K; k += 32)
+        if (e.id[k] >= 0) e.lp[k] = (e.lp[k] - top) * p.inv_temp - ln_sum;
+    __syncwarp();
+}
+DEV bool read_entries(const CostP& p, i64 n, const Entries& e) {
+    const int lane = threadIdx.x & 31;
+    int any = 0;
+    for (int k = lane; k < p.K; k += 32) {
+        const int id = entry_id(p, n, k);
+        const float t = entry_top(p, n, k);
+        const bool used = entry_used(p, id, t);
+        put_entry(p, e, k, id, t, used ? ld_any(p.z, (i64)id * p.z0 + n * p.z1, p.dt) : 0.f);
+        any |= used;
+    }
+    pad_entries(p, e, lane);
+    teacher(p, e);
     return __any_sync(0xffffffffu, any);
 }
 
@@ -135,23 +155,31 @@ DEV float entry_delta(const CostP& p, const Item& it, float w, const Entries& e,
 }
 
 // Policy: cost and log-probability of one item; `at_word`: the gradient at the word chosen.
-DEV Item policy_item(const CostP& p, i64 n, float m, float s, float za, bool put, float& at_word) {
-    const float w = weight_of(p, n), l = (za - m) - logf(s);
-    const float adv = reinterpret_cast<const float*>(p.adv)[n];
-    const float r = expf(l - reinterpret_cast<const float*>(p.old)[n]);
-    const float free = r * adv, held = fminf(fmaxf(r, 1.f - p.lo), 1.f + p.hi) * adv;
+struct Chosen { float w, old, ref, adv, za; };
+DEV Chosen read_chosen(const CostP& p, i64 n, int a, float w) {
+    Chosen c;
+    c.w = w;
+    c.old = reinterpret_cast<const float*>(p.old)[n];
+    c.ref = p.ref ? reinterpret_cast<const float*>(p.ref)[n] : 0.f;
+    c.adv = reinterpret_cast<const float*>(p.adv)[n];
+    c.za = ld_any(p.z, a * p.z0 + n * p.z1, p.dt);
+    return c;
+}
+DEV Item policy_item(const CostP& p, i64 n, float m, float s, const Chosen& c, bool put, float& at_word) {
+    const float l = (c.za - m) - logf(s), r = expf(l - c.old);
+    const float free = r * c.adv, held = fminf(fmaxf(r, 1.f - p.lo), 1.f + p.hi) * c.adv;
     const bool is_free = !(held < free);
     float cost = -(is_free ? free : held), slope = is_free ? -free : 0.f;
     if (p.ref) {
-        const float d = reinterpret_cast<const float*>(p.ref)[n] - l, m1 = expm1f(d);
+        const float d = c.ref - l, m1 = expm1f(d);
         cost += p.kl * (m1 - d);
         slope -= p.kl * m1;
     }
-    slope *= w;
-    const Item it = {usable(m), -slope / s, w == 0.f};
-    at_word = fmaf(it.scale, exp_of(za, it.m, p.c), slope);
+    slope *= c.w;
+    const Item it = {usable(m), -slope / s, c.w == 0.f};
+    at_word = fmaf(it.scale, exp_of(c.za, it.m, p.c), slope);
     if (put) {
-        reinterpret_cast<float*>(p.cost)[n] = it.dead ? 0.f : w * cost;
+        reinterpret_cast<float*>(p.cost)[n] = it.dead ? 0.f : c.w * cost;
         if (p.logp) reinterpret_cast<float*>(p.logp)[n] = l;
     }
     return it;
@@ -184,8 +212,8 @@ __global__ void __launch_bounds__(256) cost_any(const __grid_constant__ CostP p)
             for (int v = tid; v < p.V; v += 256) s += exp_of(ld_any(p.z, v * p.z0 + row, p.dt), usable(m), p.c);
             s = block_sum(s, red);
             if (POLICY) {
-                const float za = ld_any(p.z, reinterpret_cast<const int*>(p.actions)[n] * p.z0 + row, p.dt);
-                it = policy_item(p, n, m, s, za, tid == 0, at_word);
+                const Chosen c = read_chosen(p, n, reinterpret_cast<const int*>(p.actions)[n], weight_of(p, n));
+                it = policy_item(p, n, m, s, c, tid == 0, at_word);
                 __syncthreads();                       // all have read the word's logit, which delta may overwrite
             } else {
                 it = distill_item(p, n, m, s, found);
@@ -210,11 +238,17 @@ __global__ void __launch_bounds__(256) cost_any(const __grid_constant__ CostP p)
 //
 // A block per row, rows from a persistent grid.  The first walk over a row keeps a running maximum
 // and sum per thread, rescaled when four vectors hold a larger logit, which is rare after the first;
-// the second writes the gradient, and reads the row from L2.  The 16-byte vectors start at the
-// boundary at or before the row, `mis` words early; the first and the last, which may hold words of
-// other rows, belong to one thread each.  Blocks are small, so that several rows per SM are at
-// different points of their way: loads, exponentials and barriers of one run under the stores of
-// another.
+// the second writes the gradient, and reads the row from L2.  Both take the row in steps of four
+// 16-byte vectors per thread, which come through a ring of RING steps in shared memory: asynchronous
+// copies run RING - 1 steps ahead, from the first walk into the second and on into the block's next
+// row, so they run through the barriers as well.  A thread reads only what it copied itself.  The
+// vectors start at the 128-byte boundary at or before the row, `mis` words early, so that a warp's
+// accesses are whole lines whatever the row's length; those without a word of the row are left out.
+//
+// What bounds it: the second read.  At 50257 x 2048 bf16 it takes 95 us where one read and one write
+// of HBM need 64; without any arithmetic it still takes 85, without the gradient 46.  Rows kept in
+// shared memory from one walk to the other (in clusters where they are wide) were measured too, and
+// slower (98 and 681 us at 131072 x 4096, against 95 and 440): too few rows are under way then.
 DEV u32 max_pair(u32 a, u32 b, int dt) {              // NaN is passed over
     u32 r;
     if (dt == F16) asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -272,43 +306,101 @@ template <int DT> DEV void give(u32* w, const Item& it, float c) {
         set2<DT>(w, l, mul2(scale, pair(ex2_approx(lo), ex2_approx(hi))));
     }
 }
-// A vector at the end of a row, with -inf where there is no word.
-template <int DT> DEV void load_end(u32 (&w)[1][4], const char* at, int f, int words) {
-    constexpr int V = 16 / dt_size<DT>::value;
+// Puts -inf where a vector at the end of a row, whose first word is f, holds no word.
+template <int DT> DEV void mask_end(u32* w, int f, int words) {
     constexpr u32 LOW = DT == F32 ? 0xff800000u : DT == F16 ? 0xfc00fc00u : 0xff80ff80u;
-    ld_raw<16, false>(at, w[0]);
 #pragma unroll
-    for (int l = 0; l < V; ++l) {
+    for (int l = 0; l < 16 / dt_size<DT>::value; ++l) {
         if ((unsigned)(f + l) < (unsigned)words) continue;
-        if constexpr (DT == F32) w[0][l] = LOW;
-        else w[0][l >> 1] = l & 1 ? (w[0][l >> 1] & 0xffffu) | (LOW & 0xffff0000u) : (w[0][l >> 1] & 0xffff0000u) | (LOW & 0xffffu);
+        if constexpr (DT == F32) w[l] = LOW;
+        else w[l >> 1] = l & 1 ? (w[l >> 1] & 0xffffu) | (LOW & 0xffff0000u) : (w[l >> 1] & 0xffff0000u) | (LOW & 0xffffu);
     }
 }
 
-template <bool POLICY, int DT, int MAXT, int MINB>
+template <bool POLICY, int DT, int RING, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ CostP p) {
-    constexpr int SZ = dt_size<DT>::value, V = 16 / SZ, U = 4;
-    // [2][3][K4] and below [2]: these alternate from item to item; the barriers of the item in between
-    // keep two uses of one half apart
-    extern __shared__ __align__(16) float entries[];
+    constexpr int SZ = dt_size<DT>::value, V = 16 / SZ, LV = SZ == 4 ? 2 : 3, U = 4;
+    // [RING][U][T] vectors, then the entries [2][3][K4].  These, and what is [2] below, alternate from
+    // item to item; the barriers of the item in between keep two uses of one half apart.
+    extern __shared__ __align__(16) u32 mem[];
     __shared__ float2 red[2][32];
-    __shared__ int found[2];
+    __shared__ Item shared_item[2];
+    __shared__ float shared_word[2];
     const int tid = threadIdx.x, T = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = T >> 5;
     const int jump = T * 16;                           // bytes from one of a thread's vectors to the next
-    const int K4 = (p.K + 3) / 4 * 4;
-    int turn = 0;
+    const int K4 = (p.K + 3) / 4 * 4, walks = p.d ? 2 : 1;
+    float* entries = reinterpret_cast<float*>(mem + RING * U * T * 4);
+    char* mine = reinterpret_cast<char*>(mem) + tid * 16;
+    const u32 mine32 = (u32)__cvta_generic_to_shared(mine);
+    auto mis_of = [&](i64 n) { return (int)(p.z / SZ + (u64)(n * p.z1)) & (128 / SZ - 1); };
+    // what is read for an item, is read an item ahead, and compared only when it is needed
+    auto weight_at = [&](i64 n) { return n < p.N ? weight_of(p, n) : 0.f; };
+    auto action_at = [&](i64 n) { return POLICY && n < p.N ? reinterpret_cast<const int*>(p.actions)[n] : 0; };
+
+    // ---- what the copies are at: row, walk, first vector of the step
+    i64 fn = blockIdx.x;
+    int fwalk = 0, fk = 0, ffirst = 0, fnvec = 0, fslot = 0, fa = action_at(fn);
+    float fw = weight_at(fn);
+    u64 frow = 0;
+    auto enter = [&]() {                               // row fn or the first after it that is not skipped
+        for (;;) {
+            const bool skip = skipped<POLICY>(p, fw, fa);
+            fw = weight_at(fn + gridDim.x);
+            fa = action_at(fn + gridDim.x);
+            if (fn >= p.N || !skip) break;
+            fn += gridDim.x;
+        }
+        const int mis = mis_of(fn);
+        ffirst = mis >> LV;
+        fnvec = (p.V + mis + V - 1) >> LV;
+        frow = p.z + (u64)((fn * p.z1 - mis) * SZ) + (u64)tid * 16;
+        fwalk = fk = 0;
+    };
+    enter();
+    auto fetch = [&]() {
+        if (fn < p.N) {
+            const u32 to = mine32 + fslot * U * jump;
+            const u64 from = frow + (u64)fk * 16;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (fk + u * T + tid >= ffirst && fk + u * T + tid < fnvec) copy16(to + u * jump, from + (u32)(u * jump));
+            fk += U * T;
+            if (fk >= fnvec) {
+                fk = 0;
+                if (++fwalk == walks) { fn += gridDim.x; enter(); }
+            }
+        }
+        fslot = fslot == RING - 1 ? 0 : fslot + 1;
+        copy_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < RING - 1; ++k) fetch();
+
+    const bool ahead = !POLICY && p.K <= T;            // a thread per entry, read an item ahead
+    const bool mine_too = ahead && tid < p.K;
+    int next_a = action_at(blockIdx.x), next_id = -1;
+    float next_w = weight_at(blockIdx.x), next_t = 0.f, next_z = 0.f;
+    if (mine_too && blockIdx.x < p.N) {
+        next_id = entry_id(p, blockIdx.x, tid);
+        next_t = entry_top(p, blockIdx.x, tid);
+        if (next_id >= 0 && next_id < p.V) next_z = ld_any(p.z, blockIdx.x * p.z1 + next_id, DT);
+    }
+    int turn = 0, slot = 0;
     for (i64 n = blockIdx.x; n < p.N; n += gridDim.x) {
-        const bool skip = skipped<POLICY>(p, n);
+        const float w_item = next_w;
+        const int a_item = next_a, id_item = next_id;
+        const float t_item = next_t, z_item = next_z;
+        const i64 after = n + gridDim.x;
+        next_w = weight_at(after);
+        next_a = action_at(after);
+        if (mine_too && after < p.N) {
+            next_id = entry_id(p, after, tid);
+            next_t = entry_top(p, after, tid);
+        }
+        const bool skip = skipped<POLICY>(p, w_item, a_item);
         Item it = {0.f, 0.f, 1};
-        const int mis = (int)(p.z / SZ + (u64)(n * p.z1)) & (V - 1);
-        const int nvec = (p.V + mis + V - 1) / V, inner = nvec - 2;         // all but the first and the last
-        const int count = inner > tid ? (inner - 1 - tid) / T + 1 : 0;
+        const int mis = mis_of(n), kfirst = mis >> LV, nvec = (p.V + mis + V - 1) >> LV;
         const i64 drow = n * p.d1;
-        const char* row = reinterpret_cast<const char*>(p.z) + (n * p.z1 - mis) * SZ;
-        const char* mine = row + (i64)(1 + tid) * 16;
-        // the ends belong to the first and the last thread
-        const bool end = tid == 0 || (tid == T - 1 && nvec > 1);
-        const int k_end = tid == 0 ? 0 : nvec - 1;
         float at_word = 0.f;
         Entries e;
         e.id = reinterpret_cast<int*>(entries) + turn * 3 * K4;
@@ -317,84 +409,100 @@ __global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ 
         if (skip) {
             if (tid == 0) put_skipped<POLICY>(p, n);
         } else {
-            float za = 0.f;
-            if (POLICY) za = ld_any(p.z, reinterpret_cast<const int*>(p.actions)[n] + n * p.z1, DT);
-            else if (warp == 0) {
-                const bool any = read_entries(p, n, e);
-                if (lane == 0) found[turn] = any;
+            Chosen chosen;
+            int used = 0;
+            if (POLICY) {
+                if (warp == 0) chosen = read_chosen(p, n, a_item, w_item);
+            }            else if (ahead) {
+                if (tid < p.K) {
+                    put_entry(p, e, tid, id_item, t_item, z_item);
+                    used = entry_used(p, id_item, t_item);
+                }
+                if (warp == 0) pad_entries(p, e, lane);
+            } else if (warp == 0) {
+                used = read_entries(p, n, e);
             }
             Running r = {-INFINITY, 0, 0};
-            const char* at = mine;
-            int i = 0;
-            for (; i + U <= count; i += U, at += U * jump) {
+            for (int k0 = 0; k0 < nvec; k0 += U * T) {
+                fetch();
+                copy_wait<RING - 1>();
+                const char* at = mine + slot * U * jump;
+                slot = slot == RING - 1 ? 0 : slot + 1;
+                const int k = k0 + tid;
                 u32 w[U][4];
 #pragma unroll
                 for (int u = 0; u < U; ++u) ld_raw<16, false>(at + u * jump, w[u]);
+                if (k0 + U * T >= nvec || k <= kfirst) {        // the row's ends, and vectors around it
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int ku = k + u * T;
+                        if (ku <= kfirst || ku >= nvec - 1) mask_end<DT>(w[u], ku * V - mis, p.V);
+                    }
+                }
                 take<DT, U>(r, w, p.c);
-            }
-            for (; i < count; ++i, at += jump) {
-                u32 w[1][4];
-                ld_raw<16, false>(at, w[0]);
-                take<DT, 1>(r, w, p.c);
-            }
-            if (end) {
-                u32 w[1][4];
-                load_end<DT>(w, row + (i64)k_end * 16, k_end * V - mis, p.V);
-                take<DT, 1>(r, w, p.c);
             }
             // one maximum and sum for the row
             float m = warp_max(r.m), s = warp_sum(both(add2(r.a, r.b)) * exp_of(r.m, usable(m), p.c));
             if (lane == 0) red[turn][warp] = make_float2(m, s);
-            __syncthreads();
+            int any = 0;
+            if (POLICY) __syncthreads();
+            else any = __syncthreads_or(used);
             const float2 part = lane < warps ? red[turn][lane] : make_float2(-INFINITY, 0.f);
             m = warp_max(part.x);
             s = warp_sum(part.y * exp_of(part.x, usable(m), p.c));
-            if (POLICY) it = policy_item(p, n, m, s, za, tid == 0, at_word);
-            else {
-                it = distill_item(p, n, m, s, found[turn]);
-                if (warp == 0) distill_cost(p, n, m, s, it.dead, e);
+            if (POLICY) {
+                if (warp == 0) {
+                    it = policy_item(p, n, m, s, chosen, tid == 0, at_word);
+                    if (lane == 0) { shared_item[turn] = it; shared_word[turn] = at_word; }
+                }
+                if (p.d) {
+                    __syncthreads();
+                    it = shared_item[turn];
+                    at_word = shared_word[turn];
+                }
+            } else {
+                it = Item{usable(m), w_item * p.temp / s, w_item == 0.f || !any};
+                if (warp == 0) {
+                    if (ahead) teacher(p, e);
+                    distill_cost(p, n, m, s, it.dead, e);
+                }
             }
         }
+        if (mine_too && after < p.N) next_z = next_id >= 0 && next_id < p.V ? ld_any(p.z, after * p.z1 + next_id, DT) : 0.f;
         if (p.d) {
-            char* to = reinterpret_cast<char*>(p.d) + (drow - mis) * SZ + (i64)(1 + tid) * 16;
-            const char* at = mine;
-            if (it.dead) {
-                const u32 none[4] = {0, 0, 0, 0};
-                for (int i = 0; i < count; ++i, to += jump) st_raw<16>(to, none);
-                if (end) put_part<DT, V>(p.d, drow, k_end * V - mis, p.V, none);
-                if (!skip) __syncthreads();            // all have read the word's logit, which delta may overwrite
-            } else {
-                int i = 0;
-                for (; i + U <= count; i += U, at += U * jump, to += U * jump) {
-                    u32 w[U][4];
+            char* to = reinterpret_cast<char*>(p.d) + (drow - mis) * SZ + tid * 16;
+            for (int k0 = 0; k0 < nvec; k0 += U * T, to += U * jump) {
+                const char* at = mine + slot * U * jump;
+                if (!skip) {
+                    fetch();
+                    copy_wait<RING - 1>();
+                    slot = slot == RING - 1 ? 0 : slot + 1;
+                }
+                const int k = k0 + tid;
+                const bool ends = k0 + U * T >= nvec || k <= kfirst;
+                u32 w[U][4];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) ld_raw<16, false>(at + u * jump, w[u]);
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
+                for (int u = 0; u < U; ++u) {
+                    if (it.dead) w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;
+                    else {
+                        ld_raw<16, false>(at + u * jump, w[u]);
                         give<DT>(w[u], it, p.c);
-                        st_raw<16>(to + u * jump, w[u]);
                     }
                 }
-                for (; i < count; ++i, at += jump, to += jump) {
-                    u32 w[4];
-                    ld_raw<16, false>(at, w);
-                    give<DT>(w, it, p.c);
-                    st_raw<16>(to, w);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int ku = k + u * T;
+                    if (ends && (ku <= kfirst || ku >= nvec - 1)) put_part<DT, V>(p.d, drow, ku * V - mis, p.V, w[u]);
+                    else st_raw<16>(to + u * jump, w[u]);
                 }
-                if (end) {
-                    u32 w[4];
-                    ld_raw<16, false>(row + (i64)k_end * 16, w);
-                    give<DT>(w, it, p.c);
-                    put_part<DT, V>(p.d, drow, k_end * V - mis, p.V, w);
-                }
+            }
+            if (POLICY) {                              // by the thread that wrote the word's vector
+                if (!it.dead && (a_item + mis) / V % T == tid) st_any(p.d, drow + a_item, DT, at_word);
+            } else if (!skip) {
                 __syncthreads();                       // the entries' words have been written with the others
-                if (POLICY) {
-                    if (tid == 0) st_any(p.d, drow + reinterpret_cast<const int*>(p.actions)[n], DT, at_word);
-                } else {
-                    const float w = weight_of(p, n);
+                if (!it.dead)
                     for (int k = tid; k < p.K; k += T)
-                        if (e.id[k] >= 0) st_any(p.d, drow + e.id[k], DT, entry_delta(p, it, w, e, k));
-                }
+                        if (e.id[k] >= 0) st_any(p.d, drow + e.id[k], DT, entry_delta(p, it, w_item, e, k));
             }
         }
         if (!skip) turn ^= 1;
@@ -498,9 +606,9 @@ __global__ void __launch_bounds__(32) cost_cols_items(const __grid_constant__ Co
         s = warp_sum(s);
         __syncwarp();
         if (POLICY) {
-            const float za = ld_any(c.z, reinterpret_cast<const int*>(c.actions)[n] * c.z0 + n * c.z1, c.dt);
+            const Chosen one = read_chosen(c, n, reinterpret_cast<const int*>(c.actions)[n], weight_of(c, n));
             float at_word;
-            it = policy_item(c, n, m, s, za, lane == 0, at_word);
+            it = policy_item(c, n, m, s, one, lane == 0, at_word);
             if (c.d && lane == 0) p.grad[n] = at_word;
         } else {
             it = distill_item(c, n, m, s, any);
@@ -635,19 +743,28 @@ template <bool POLICY> cudaError_t launch_any(const CostP& p, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+// How many threads a row gets, and with them how many rows are under way: small blocks keep more
+// rows of an SM at different points of their way, but a row stays in L2 between its two walks only
+// if the rows under way hold no more than some 60 MB.  Measured, us: 8192 words bf16 x 16384, 128
+// threads 130, 256 151; 50257 bf16 x 2048, 256 threads 95, 512 101; 32768 f32 x 4096 (128 KB), 256
+// threads 217, 512 189; 131072 bf16 x 4096, 512 threads 490, 1024 440.
+template <bool POLICY, int DT, int RING, int MAXT, int MINB> cudaError_t launch_rows_of(const CostP& p, cudaStream_t s) {
+    constexpr int V = 16 / dt_size<DT>::value, U = 4;
+    const bool even = p.z % 128 == 0 && p.z1 % (8 * V) == 0;        // every row starts on a boundary
+    const i64 nvec = ((i64)p.V + (even ? 0 : 8 * V - 1) + V - 1) / V, steps = (nvec + U * MAXT - 1) / (U * MAXT);
+    const int T = (int)((nvec + U * steps - 1) / (U * steps) + 31) / 32 * 32;
+    const int smem = RING * U * T * 16 + (POLICY ? 0 : 24 * ((p.K + 3) / 4 * 4));
+    const i64 most = resident_blocks(cost_rows<POLICY, DT, RING, MAXT, MINB>, T, smem);
+    if (!most) return cudaErrorInvalidConfiguration;
+    cost_rows<POLICY, DT, RING, MAXT, MINB><<<(unsigned)(p.N < most ? p.N : most), T, smem, s>>>(p);
+    return cudaGetLastError();
+}
 template <bool POLICY, int DT> cudaError_t launch_rows(const CostP& p, cudaStream_t s) {
-    const i64 bytes = (i64)p.V * dt_size<DT>::value, nvec = bytes / 16 + 1;
-    const int smem = POLICY ? 0 : 24 * ((p.K + 3) / 4 * 4);
-    auto go = [&](auto kernel, int T) {
-        i64 most = resident_blocks(kernel, T, smem);
-        if (!most) return cudaErrorInvalidConfiguration;
-        kernel<<<(unsigned)(p.N < most ? p.N : most), T, smem, s>>>(p);
-        return cudaGetLastError();
-    };
-    if (bytes > 160000) return go(cost_rows<POLICY, DT, 512, 2>, 512);
-    int T = (int)(nvec / 8 + 31) / 32 * 32;
-    T = T < 32 ? 32 : T > 256 ? 256 : T;
-    return go(cost_rows<POLICY, DT, 256, 4>, T);
+    const i64 bytes = (i64)p.V * dt_size<DT>::value;
+    if (bytes > 160 * 1024) return launch_rows_of<POLICY, DT, 3, 1024, 1>(p, s);
+    if (bytes > 110 * 1024) return launch_rows_of<POLICY, DT, 3, 512, 2>(p, s);
+    if (bytes > 32 * 1024) return launch_rows_of<POLICY, DT, 3, 256, 4>(p, s);
+    return launch_rows_of<POLICY, DT, 3, 128, 8>(p, s);
 }
 
 template <bool POLICY, int DT> cudaError_t launch_cols_width(const CostP& p, char* scratch, int& launches, cudaStream_t s) {
