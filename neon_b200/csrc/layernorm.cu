@@ -445,8 +445,9 @@ template <bool BACK> cudaError_t launch_type(const LnP& p, bool mis, float* part
 // A block takes a stripe of neighbouring items, `lanes` threads with V items each side by side and
 // its other threads down the features, so every access is a run of 32 to 128 bytes of a feature's
 // row.  The stripe is walked through three times forward (sum, centred squares, result) and twice
-// backwards; only the first walk reads HBM: the stripes under way, at most 128 bytes times F per
-// block, stay in L2 or L1.
+// backwards.  HELD: it is copied to shared memory first, every thread's own vectors by itself, so
+// HBM is read once; a stripe that does not fit is read again, from L2 if that holds the stripes
+// under way.
 template <int V> DEV void stripe_sum(float (&v)[V], float* s, int lanes) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, tx = threadIdx.x & (lanes - 1);
 #pragma unroll
@@ -466,8 +467,23 @@ template <int V> DEV void stripe_sum(float (&v)[V], float* s, int lanes) {
     }
 }
 
-template <int DT, int V>
+// A thread's vectors of a stripe, copied to its own places in shared memory (i: which of them).
+template <int DT> DEV void hold(u32 to, u64 base, i64 f0, i64 step, i64 pitch, i64 n, int F) {
+    for (i64 f = f0; f < F; f += step, to += blockDim.x * 16) copy16(to, base + (u64)((f * pitch + n) * dt_size<DT>::value));
+}
+template <int DT, int V, bool HELD> DEV void look(const u32* held, int i, u64 base, i64 at, float* x) {
+    if constexpr (HELD) {
+        u32 w[4];
+        ld_raw<16, false>(reinterpret_cast<const char*>(held + (i * blockDim.x + threadIdx.x) * 4), w);
+        cvt_in<DT, V>(w, x);
+    } else {
+        ld_f<DT, V, false>(base, at, x);
+    }
+}
+
+template <int DT, int V, bool HELD>
 __global__ void __launch_bounds__(512) ln_fprop_cols(const __grid_constant__ LnP p, int lanes) {
+    extern __shared__ __align__(16) u32 held[];
     __shared__ float s[16 * 32 * (V > 1 ? 2 : 1)];     // [warps][lanes][V]: 8 lanes of vectors, or 32 of single items
     const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = blockDim.x / lanes, F = (int)p.F;
     const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
@@ -476,11 +492,16 @@ __global__ void __launch_bounds__(512) ln_fprop_cols(const __grid_constant__ LnP
     float mean[V], rstd[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) mean[i] = rstd[i] = 0.f;
+    if constexpr (HELD) {
+        if (in) hold<DT>((u32)__cvta_generic_to_shared(held) + threadIdx.x * 16, p.x, ty, rows, p.x0, n, F);
+        copy_commit();
+        copy_wait<0>();
+    }
     if (in) {
 #pragma unroll 4
-        for (int f = ty; f < F; f += rows) {
+        for (int f = ty, k = 0; f < F; f += rows, ++k) {
             float x[V];
-            ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
+            look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
 #pragma unroll
             for (int i = 0; i < V; ++i) mean[i] += x[i];
         }
@@ -490,9 +511,9 @@ __global__ void __launch_bounds__(512) ln_fprop_cols(const __grid_constant__ LnP
     for (int i = 0; i < V; ++i) mean[i] *= inv;
     if (in) {
 #pragma unroll 4
-        for (int f = ty; f < F; f += rows) {
+        for (int f = ty, k = 0; f < F; f += rows, ++k) {
             float x[V];
-            ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
+            look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
 #pragma unroll
             for (int i = 0; i < V; ++i) { x[i] -= mean[i]; rstd[i] = fmaf(x[i], x[i], rstd[i]); }
         }
@@ -509,10 +530,10 @@ __global__ void __launch_bounds__(512) ln_fprop_cols(const __grid_constant__ LnP
         }
     }
 #pragma unroll 4
-    for (int f = ty; f < F; f += rows) {
+    for (int f = ty, k = 0; f < F; f += rows, ++k) {
         const float g = p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f, b = p.beta ? ld_any(p.beta, f, p.pdt) : 0.f;
         float x[V];
-        ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
+        look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
 #pragma unroll
         for (int i = 0; i < V; ++i) x[i] = fmaf((x[i] - mean[i]) * rstd[i], g, b);
         st_f<DT, V>(p.out, f * p.o0 + n, x);
@@ -521,15 +542,26 @@ __global__ void __launch_bounds__(512) ln_fprop_cols(const __grid_constant__ LnP
 
 // part[block][0][F]: the block's share of grad_gamma, part[block][1][F]: of grad_beta; a block
 // works through stripes gridDim.x apart and adds to its own shares.
-template <int DT, int V>
+template <int DT, int V, bool HELD>
 __global__ void __launch_bounds__(512) ln_bprop_cols(const __grid_constant__ LnP p, float* part, int lanes, i64 stripes) {
+    extern __shared__ __align__(16) u32 held[];        // x, then the error
     __shared__ float s[16 * 32 * (V > 1 ? 2 : 1)];
     const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = blockDim.x / lanes, F = (int)p.F;
+    const int each = (F + rows - 1) / rows;            // vectors per thread
+    const u32* held_e = held + each * blockDim.x * 4;
     const float inv = 1.f / (float)F;
     float* mine = part + (i64)blockIdx.x * 2 * F;
     for (i64 stripe = blockIdx.x; stripe < stripes; stripe += gridDim.x) {
         const i64 n = (stripe * lanes + tx) * V;
         const bool in = n < p.N;
+        if constexpr (HELD) {
+            if (in) {
+                const u32 to = (u32)__cvta_generic_to_shared(held) + threadIdx.x * 16;
+                hold<DT>(to, p.x, ty, rows, p.x0, n, F);
+                hold<DT>(to + each * blockDim.x * 16, p.e, ty, rows, p.e0, n, F);
+            }
+            copy_commit();
+        }
         float mean[V], rstd[V], a[V], b[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -537,14 +569,16 @@ __global__ void __launch_bounds__(512) ln_bprop_cols(const __grid_constant__ LnP
             rstd[i] = in ? reinterpret_cast<const float*>(p.rstd)[n + i] : 0.f;
             a[i] = b[i] = 0.f;
         }
-        for (int f0 = 0; f0 < F; f0 += rows) {         // all threads: the lanes of a feature add up below
-            const int f = f0 + ty;
+        if constexpr (HELD) copy_wait<0>();
+#pragma unroll 2
+        for (int k = 0; k < each; ++k) {               // all threads: the lanes of a feature add up below
+            const int f = k * rows + ty;
             float gg = 0.f, gb = 0.f;
             if (in && f < F) {
                 const float gamma = p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f;
                 float x[V], e[V];
-                ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
-                ld_f<DT, V, false>(p.e, f * p.e0 + n, e);
+                look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
+                look<DT, V, HELD>(held_e, k, p.e, f * p.e0 + n, e);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     x[i] = (x[i] - mean[i]) * rstd[i];
@@ -573,11 +607,11 @@ __global__ void __launch_bounds__(512) ln_bprop_cols(const __grid_constant__ LnP
 #pragma unroll
         for (int i = 0; i < V; ++i) { a[i] *= inv; b[i] *= inv; }
 #pragma unroll 2
-        for (int f = ty; f < F; f += rows) {
+        for (int f = ty, k = 0; f < F; f += rows, ++k) {
             const float gamma = p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f;
             float x[V], e[V];
-            ld_f<DT, V, false>(p.x, f * p.x0 + n, x);
-            ld_f<DT, V, false>(p.e, f * p.e0 + n, e);
+            look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
+            look<DT, V, HELD>(held_e, k, p.e, f * p.e0 + n, e);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 x[i] = (x[i] - mean[i]) * rstd[i];
@@ -599,23 +633,33 @@ bool cols_fit(const b200_matrix* const* m, int count, i64 N, bool& wide) {
     return true;
 }
 
-// Stripes of 128 bytes, or down to 32 bytes where wider ones would leave SMs without a block.
-template <int DT, int V, bool BACK> cudaError_t launch_cols(const LnP& p, float* part, int* parts, cudaStream_t s) {
-    constexpr int size = dt_size<DT>::value * V;
-    int lanes = 128 / size > 32 ? 32 : 128 / size;
-    while (lanes * size > 32 && lanes > 1 && (p.N + (i64)lanes * V - 1) / ((i64)lanes * V) < 2 * 148) lanes /= 2;
+// Stripes of 128 bytes, or down to 32 bytes where wider ones would leave SMs without a block, or
+// would not fit twice into an SM's shared memory.
+template <int DT, int V, bool BACK, bool HELD> cudaError_t launch_cols_of(const LnP& p, int lanes, int smem, float* part, int* parts, cudaStream_t s) {
     const i64 stripes = (p.N + (i64)lanes * V - 1) / ((i64)lanes * V);
     if constexpr (BACK) {
-        i64 grid = resident_blocks(ln_bprop_cols<DT, V>, 512, 0);
+        i64 grid = resident_blocks(ln_bprop_cols<DT, V, HELD>, 512, smem);
         if (!grid) return cudaErrorInvalidConfiguration;
         if (grid > stripes) grid = stripes;
         if (part && grid > most_parts(p.F)) grid = most_parts(p.F);
         *parts = (int)grid;
-        ln_bprop_cols<DT, V><<<(unsigned)grid, 512, 0, s>>>(p, part, lanes, stripes);
+        ln_bprop_cols<DT, V, HELD><<<(unsigned)grid, 512, smem, s>>>(p, part, lanes, stripes);
     } else {
-        ln_fprop_cols<DT, V><<<(unsigned)stripes, 512, 0, s>>>(p, lanes);
+        if (!resident_blocks(ln_fprop_cols<DT, V, HELD>, 512, smem)) return cudaErrorInvalidConfiguration;
+        ln_fprop_cols<DT, V, HELD><<<(unsigned)stripes, 512, smem, s>>>(p, lanes);
     }
     return cudaGetLastError();
+}
+template <int DT, int V, bool BACK> cudaError_t launch_cols(const LnP& p, float* part, int* parts, cudaStream_t s) {
+    constexpr int size = dt_size<DT>::value * V;
+    int lanes = 128 / size > 32 ? 32 : 128 / size;
+    while (lanes * size > 32 && lanes > 1 && (p.N + (i64)lanes * V - 1) / ((i64)lanes * V) < 2 * 148) lanes /= 2;
+    if constexpr (V > 1) {
+        auto bytes = [&](int l) { return (p.F + 512 / l - 1) / (512 / l) * 512 * 16 * (BACK ? 2 : 1); };
+        while (lanes > 2 && bytes(lanes) > 100 * 1024) lanes /= 2;
+        if (bytes(lanes) <= 216 * 1024) return launch_cols_of<DT, V, BACK, true>(p, lanes, (int)bytes(lanes), part, parts, s);
+    }
+    return launch_cols_of<DT, V, BACK, false>(p, lanes, 0, part, parts, s);
 }
 template <bool BACK> cudaError_t launch_cols_type(const LnP& p, bool wide, float* part, int* parts, cudaStream_t s) {
     switch (p.dt) {

@@ -528,42 +528,78 @@ struct ColsP {
 };
 enum { kSplits = 64, kColThreads = 256 };
 
+// neighbouring items of a word's row as pairs of fp32; a single item is a pair with -inf
+template <int DT, int V> struct Pairs {
+    static constexpr int P = V > 1 ? V / 2 : 1;
+    u32 w[V > 1 ? 4 : 1];
+    DEV void load(u64 base, i64 at) { ld_w<DT, V, false>(base, at, w); }
+    DEV void none() {
+#pragma unroll
+        for (u32& x : w) x = DT == F32 ? 0xff800000u : DT == F16 ? 0xfc00fc00u : 0xff80ff80u;
+    }
+    DEV f32x2 get(int l) const {
+        if constexpr (V > 1) return get2<DT>(w, l);
+        else { float z[1]; cvt_in<DT, 1>(w, z); return pair(z[0], -INFINITY); }
+    }
+};
+
 template <int DT, int V>
 __global__ void __launch_bounds__(kColThreads) cost_cols_stats(const __grid_constant__ ColsP p) {
     grid_enter();
-    constexpr int U = 4;
+    constexpr int U = 4, P = Pairs<DT, V>::P;
     __shared__ float2 red[kColThreads * V];
     const int lanes = p.lanes, tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = kColThreads / lanes;
     const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
     const bool in = n < p.c.N;
     const float c = p.c.c;
-    float m[V], s[V];
+    const f32x2 c2 = pair(c, c);
+    float m[2 * P];
+    f32x2 s[P], less[P];
 #pragma unroll
-    for (int i = 0; i < V; ++i) { m[i] = -INFINITY; s[i] = 0.f; }
+    for (int l = 0; l < P; ++l) { m[2 * l] = m[2 * l + 1] = -INFINITY; s[l] = less[l] = 0; }
     const int lo = blockIdx.y * p.rows, hi = min(lo + p.rows, p.c.V);
     if (in) {
         for (int v0 = lo + ty; v0 < hi; v0 += rows * U) {
-            float z[U][V];
+            Pairs<DT, V> z[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (v0 + u * rows < hi) ld_f<DT, V, false>(p.c.z, (i64)(v0 + u * rows) * p.c.z0 + n, z[u]);
-                else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) z[u][i] = -INFINITY;
-                }
+                if (v0 + u * rows < hi) z[u].load(p.c.z, (i64)(v0 + u * rows) * p.c.z0 + n);
+                else z[u].none();
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float top = fmaxf(fmaxf(z[0][i], z[1][i]), fmaxf(z[2][i], z[3][i]));
-                if (top > m[i]) { s[i] *= exp_of(m[i], top, c); m[i] = top; }
-                const float t = usable(m[i]);
+            for (int l = 0; l < P; ++l) {
+                float a = -INFINITY, b = -INFINITY;    // the largest of the step
 #pragma unroll
-                for (int u = 0; u < U; ++u) s[i] += exp_of(z[u][i], t, c);
+                for (int u = 0; u < U; ++u) {
+                    float x, y;
+                    split(z[u].get(l), x, y);
+                    a = fmaxf(a, x);
+                    b = fmaxf(b, y);
+                }
+                if (a > m[2 * l] || b > m[2 * l + 1]) {
+                    a = fmaxf(a, m[2 * l]);
+                    b = fmaxf(b, m[2 * l + 1]);
+                    s[l] = mul2(s[l], pair(exp_of(m[2 * l], usable(a), c), exp_of(m[2 * l + 1], usable(b), c)));
+                    m[2 * l] = a;
+                    m[2 * l + 1] = b;
+                    less[l] = pair(-usable(a), -usable(b));
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float x, y;
+                    split(mul2(add2(z[u].get(l), less[l]), c2), x, y);
+                    s[l] = add2(s[l], pair(ex2_approx(x), ex2_approx(y)));
+                }
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) red[(ty * lanes + tx) * V + i] = make_float2(m[i], s[i]);
+    for (int l = 0; l < P; ++l) {
+        float x, y;
+        split(s[l], x, y);
+        red[(ty * lanes + tx) * V + 2 * l] = make_float2(m[2 * l], x);
+        if constexpr (V > 1) red[(ty * lanes + tx) * V + 2 * l + 1] = make_float2(m[2 * l + 1], y);
+    }
     __syncthreads();
     const int wide = lanes * V;
     for (int i = threadIdx.x; i < wide; i += kColThreads) {
@@ -625,25 +661,48 @@ __global__ void __launch_bounds__(32) cost_cols_items(const __grid_constant__ Co
 template <int DT, int V>
 __global__ void __launch_bounds__(kColThreads) cost_cols_delta(const __grid_constant__ ColsP p) {
     grid_enter();
+    constexpr int U = 4, P = Pairs<DT, V>::P;
     const int lanes = p.lanes, tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = kColThreads / lanes;
     const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
     if (n >= p.c.N) return;
-    const float c = p.c.c;
-    float m[V], scale[V];
-    bool dead[V];
+    const f32x2 c2 = pair(p.c.c, p.c.c);
+    f32x2 less[P], scale[P];
+    u32 alive[V > 1 ? 4 : 1];                          // bits of the stored elements of items that are not dead
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float4 it = p.item[n + i];
-        m[i] = it.x; scale[i] = it.y; dead[i] = it.z != 0.f;
+    for (u32& x : alive) x = 0;
+#pragma unroll
+    for (int l = 0; l < P; ++l) {
+        const float4 a = p.item[n + 2 * l], b = V > 1 ? p.item[n + 2 * l + 1] : a;
+        less[l] = pair(-a.x, -b.x);
+        scale[l] = pair(a.y, b.y);
+        if (DT == F32 || V == 1) {
+            alive[V > 1 ? 2 * l : 0] = a.z != 0.f ? 0u : ~0u;
+            if (V > 1) alive[(2 * l + 1) % (V > 1 ? 4 : 1)] = b.z != 0.f ? 0u : ~0u;
+        } else {
+            alive[l % (V > 1 ? 4 : 1)] = (a.z != 0.f ? 0u : 0xffffu) | (b.z != 0.f ? 0u : 0xffff0000u);
+        }
     }
     const int lo = blockIdx.y * p.rows, hi = min(lo + p.rows, p.c.V);
-#pragma unroll 4
-    for (int v = lo + ty; v < hi; v += rows) {
-        float z[V];
-        ld_f<DT, V, false>(p.c.z, (i64)v * p.c.z0 + n, z);
+    for (int v0 = lo + ty; v0 < hi; v0 += rows * U) {
+        Pairs<DT, V> z[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = dead[i] ? 0.f : scale[i] * exp_of(z[i], m[i], c);
-        st_f<DT, V>(p.c.d, (i64)v * p.c.d0 + n, z);
+        for (int u = 0; u < U; ++u) if (v0 + u * rows < hi) z[u].load(p.c.z, (i64)(v0 + u * rows) * p.c.z0 + n);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (v0 + u * rows >= hi) break;
+            u32 w[V > 1 ? 4 : 1];
+#pragma unroll
+            for (int l = 0; l < P; ++l) {
+                float x, y;
+                split(mul2(add2(z[u].get(l), less[l]), c2), x, y);
+                const f32x2 g = mul2(scale[l], pair(ex2_approx(x), ex2_approx(y)));
+                if constexpr (V > 1) set2<DT>(w, l, g);
+                else { split(g, x, y); cvt_out<DT, 1, false>(&x, w, SrCtx(), nullptr); }
+            }
+#pragma unroll
+            for (int i = 0; i < (V > 1 ? 4 : 1); ++i) w[i] &= alive[i];
+            st_raw<dt_size<DT>::value * V>(reinterpret_cast<char*>(p.c.d) + ((i64)(v0 + u * rows) * p.c.d0 + n) * dt_size<DT>::value, w);
+        }
     }
 }
 

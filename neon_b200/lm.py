@@ -21,14 +21,13 @@ Arithmetic is fp32; results are rounded to the tensor's type once, to nearest (a
 call can be recorded with ``be.capture``.
 """
 
-import numpy as np
-
 from . import runtime as rt
 from .lowering import dtype_code
 from .tensor import B200Tensor
 
 _NONE = rt.Matrix(0, 0, 0, rt.F32, 0)
 _FLOATS = (rt.F32, rt.F16, rt.BF16)
+_NAMES = {rt.F32: "float32", rt.I32: "int32"}
 
 
 class LanguageModelOps(object):
@@ -36,49 +35,54 @@ class LanguageModelOps(object):
 
     # ------------------------------------------------------------------ arguments
     @staticmethod
-    def _lm_tensor(t, name):
+    def _lm_describe(t, name):
+        """What the C entry points need to know about a tensor, kept with it (none of it changes
+        afterwards): matrix descriptor, type code, size if it is a contiguous vector (else -1),
+        and whether some stride repeats elements."""
         if not isinstance(t, B200Tensor):
             if hasattr(t, "local"):
                 raise NotImplementedError("%s: sharded tensors" % name)
             raise TypeError("%s must be a tensor of the backend, got %s" % (name, type(t).__name__))
         if t.take_array is not None:
             raise NotImplementedError("%s: a tensor indexed with an array" % name)
-        return t
+        code = dtype_code(t.dtype)
+        matrix = rt.Matrix(t.gpudata, t.strides[0], t.strides[1], code, 0) if len(t.shape) == 2 else None
+        long_axes = [s for d, s in zip(t.shape, t.strides) if d > 1]
+        vector = t.size if not long_axes or long_axes == [1] else -1
+        t._lm = (matrix, code, vector, 0 in long_axes)
+        return t._lm
 
     def _lm_matrix(self, t, name, shape=None, out=False, floats=True):
         """Descriptor of a matrix argument, after its checks."""
-        self._lm_tensor(t, name)
-        if len(t.shape) != 2 or (shape is not None and t.shape != shape):
+        known = getattr(t, "_lm", None) or self._lm_describe(t, name)
+        if known[0] is None or (shape is not None and t.shape != shape):
             raise ValueError("%s has shape %s, expected %s" % (name, t.shape, shape or "two dimensions"))
-        code = dtype_code(t.dtype)
-        if floats and code not in _FLOATS:
+        if floats and known[1] not in _FLOATS:
             raise TypeError("%s must be float32, float16 or bfloat16, not %s" % (name, t.dtype))
-        if out:
-            self._lm_output(t, name)
-        return rt.Matrix(t.gpudata, t.strides[0], t.strides[1], code, 0)
+        if out and (t.rounding or known[3]):
+            self._lm_refuse_output(t, name)
+        return known[0]
 
-    def _lm_vector(self, t, name, size, dtype=None, out=False):
+    def _lm_vector(self, t, name, size, code=None, out=False):
         """Address of a contiguous vector argument of ``size`` values (0 for None)."""
         if t is None:
             return 0
-        self._lm_tensor(t, name)
+        known = getattr(t, "_lm", None) or self._lm_describe(t, name)
         if t.size != size or (size and max(t.shape) != size):
             raise ValueError("%s has shape %s, expected %d values" % (name, t.shape, size))
-        if size > 1 and t.strides[t.shape.index(size)] != 1:
+        if known[2] != size:
             raise ValueError("%s must be contiguous" % name)
-        if dtype is not None and t.dtype.type is not dtype:
-            raise TypeError("%s must be %s, not %s" % (name, np.dtype(dtype).name, t.dtype))
-        if out:
-            self._lm_output(t, name)
+        if code is not None and known[1] != code:
+            raise TypeError("%s must be %s, not %s" % (name, _NAMES[code], t.dtype))
+        if out and (t.rounding or known[3]):
+            self._lm_refuse_output(t, name)
         return t.gpudata
 
     @staticmethod
-    def _lm_output(t, name):
+    def _lm_refuse_output(t, name):
         if t.rounding:
             raise NotImplementedError("%s: stochastic rounding of this operator's result" % name)
-        for d, s in zip(t.shape, t.strides):
-            if d > 1 and s == 0:
-                raise ValueError("%s repeats its elements and cannot be written" % name)
+        raise ValueError("%s repeats its elements and cannot be written" % name)
 
     @staticmethod
     def _lm_span(t):
@@ -90,16 +94,19 @@ class LanguageModelOps(object):
         return (t.gpudata + size * sum(r for r in reach if r < 0),
                 t.gpudata + size * (1 + sum(r for r in reach if r > 0)))
 
-    @staticmethod
-    def _lm_params(first, second, names):
+    def _lm_params(self, first, second, names):
         """Common type code of two optional parameter vectors."""
-        for t, name in zip((first, second), names):
-            if t is not None and dtype_code(t.dtype) not in _FLOATS:
+        code = None
+        for t, name in ((first, names[0]), (second, names[1])):
+            if t is None:
+                continue
+            own = (getattr(t, "_lm", None) or self._lm_describe(t, name))[1]
+            if own not in _FLOATS:
                 raise TypeError("%s must be float32, float16 or bfloat16, not %s" % (name, t.dtype))
-        if first is not None and second is not None and first.dtype != second.dtype:
-            raise TypeError("%s and %s must have one type" % names)
-        given = first if first is not None else second
-        return rt.F32 if given is None else dtype_code(given.dtype)
+            if code is not None and own != code:
+                raise TypeError("%s and %s must have one type" % names)
+            code = own
+        return rt.F32 if code is None else code
 
     def _lm_scratch(self, nbytes):
         if not nbytes:
@@ -131,8 +138,8 @@ class LanguageModelOps(object):
         f, n = x.shape
         pdt = self._lm_params(gamma, beta, ("gamma", "beta"))
         args = (self._lm_vector(gamma, "gamma", f), self._lm_vector(beta, "beta", f), pdt,
-                self._lm_vector(mean, "mean", n, np.float32, out=True),
-                self._lm_vector(rstd, "rstd", n, np.float32, out=True))
+                self._lm_vector(mean, "mean", n, rt.F32, out=True),
+                self._lm_vector(rstd, "rstd", n, rt.F32, out=True))
         self._lm_check(x, y, gamma, beta, mean, rstd)
         self.launches += rt.ln_fprop(mx, my, *args, f, n, float(eps), self.stream)
         return y
@@ -163,7 +170,7 @@ class LanguageModelOps(object):
             if (grad_gamma is not None or grad_beta is not None) and gdt != pdt:
                 raise TypeError("gamma, grad_gamma and grad_beta must have one type")
             pdt = gdt
-        args = (self._lm_vector(mean, "mean", n, np.float32), self._lm_vector(rstd, "rstd", n, np.float32),
+        args = (self._lm_vector(mean, "mean", n, rt.F32), self._lm_vector(rstd, "rstd", n, rt.F32),
                 self._lm_vector(gamma, "gamma", f), self._lm_vector(grad_gamma, "grad_gamma", f, out=True),
                 self._lm_vector(grad_beta, "grad_beta", f, out=True))
         self._lm_check(x, delta_in, delta_out, mean, rstd, gamma, grad_gamma, grad_beta)
@@ -185,8 +192,9 @@ class LanguageModelOps(object):
             scale: factor of every value looked up
         """
         mw = self._lm_matrix(W, "W")
-        self._lm_tensor(outputs, "outputs")
-        mo = self._lm_matrix(outputs, "outputs", (W.shape[1], outputs.shape[-1]), out=True)
+        mo = self._lm_matrix(outputs, "outputs", out=True)
+        if outputs.shape[0] != W.shape[1]:
+            raise ValueError("outputs has shape %s, expected (%d, positions)" % (outputs.shape, W.shape[1]))
         if W.dtype != outputs.dtype:
             raise TypeError("W and outputs must have one type")
         n = outputs.shape[1]
@@ -198,10 +206,10 @@ class LanguageModelOps(object):
         return outputs
 
     def _lm_words(self, t, name, size):
-        self._lm_tensor(t, name)
-        if t.dtype.type is not np.int32:
+        known = getattr(t, "_lm", None) or self._lm_describe(t, name)
+        if known[1] != rt.I32:
             raise TypeError("%s must be int32, not %s" % (name, t.dtype))
-        if t.size != size or not t.is_contiguous:
+        if t.size != size or not (known[2] == size or t.is_contiguous):
             raise ValueError("%s must hold %d contiguous word numbers, got shape %s" % (name, size, t.shape))
         return t.gpudata
 
@@ -225,7 +233,9 @@ class LanguageModelOps(object):
             pad_idx: word that takes no gradient, or None
         """
         me = self._lm_matrix(error, "error")
-        mw = self._lm_matrix(dW, "dW", (dW.shape[0], error.shape[0]), out=True)
+        mw = self._lm_matrix(dW, "dW", out=True)
+        if dW.shape[1] != error.shape[0]:
+            raise ValueError("dW has shape %s, expected (vocabulary, %d)" % (dW.shape, error.shape[0]))
         f, n = error.shape
         ids = self._lm_words(inputs, "inputs", n)
         if error_t is not None:
@@ -272,15 +282,16 @@ class LanguageModelOps(object):
         mz = self._lm_matrix(logits, "logits")
         v, n = logits.shape
         md = self._lm_delta(delta, logits)
-        self._lm_tensor(top_ids, "top_ids")
-        if top_ids.dtype.type is not np.int32:
+        mi = self._lm_matrix(top_ids, "top_ids", floats=False)
+        if mi.dtype != rt.I32:
             raise TypeError("top_ids must be int32, not %s" % top_ids.dtype)
         k = top_ids.shape[0]
-        mi = self._lm_matrix(top_ids, "top_ids", (k, n), floats=False)
+        if top_ids.shape[1] != n:
+            raise ValueError("top_ids has shape %s, expected (K, %d)" % (top_ids.shape, n))
         mt = self._lm_matrix(top_logits, "top_logits", (k, n))
         if cost is None:
             raise ValueError("cost must be a tensor")
-        args = (self._lm_vector(weights, "weights", n, np.float32), self._lm_vector(cost, "cost", n, np.float32, out=True))
+        args = (self._lm_vector(weights, "weights", n, rt.F32), self._lm_vector(cost, "cost", n, rt.F32, out=True))
         self._lm_check(logits, delta, top_ids, top_logits, weights, cost)
         nbytes = rt.cost_scratch_bytes(v, n, k)
         self.launches += rt.distill(mz, md, mi, mt, *args, v, n, k, float(temperature), self._lm_scratch(nbytes), nbytes,
@@ -329,10 +340,10 @@ class LanguageModelOps(object):
         if kl_coef != 0 and ref_logp is None:
             raise ValueError("a KL term needs ref_logp")
         vec = self._lm_vector
-        args = (self._lm_words(actions, "actions", n), vec(old_logp, "old_logp", n, np.float32),
-                vec(ref_logp, "ref_logp", n, np.float32), vec(advantages, "advantages", n, np.float32),
-                vec(weights, "weights", n, np.float32), vec(cost, "cost", n, np.float32, out=True),
-                vec(logp, "logp", n, np.float32, out=True))
+        args = (self._lm_words(actions, "actions", n), vec(old_logp, "old_logp", n, rt.F32),
+                vec(ref_logp, "ref_logp", n, rt.F32), vec(advantages, "advantages", n, rt.F32),
+                vec(weights, "weights", n, rt.F32), vec(cost, "cost", n, rt.F32, out=True),
+                vec(logp, "logp", n, rt.F32, out=True))
         self._lm_check(logits, delta, actions, old_logp, ref_logp, advantages, weights, cost, logp)
         nbytes = rt.cost_scratch_bytes(v, n, 1)
         self.launches += rt.policy(mz, md, *args, v, n, float(low), float(high), float(kl_coef),
