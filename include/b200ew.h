@@ -243,9 +243,10 @@ typedef struct b200_matrix {
 /* layer normalisation of every item over its features, y = (x - mean) * rstd * gamma + beta, next to
  * the batch normalisation entry points (neon/backends/nervanagpu.py:2463-2588).  gamma and beta
  * (param_dtype), mean and rstd (f32, written) are optional.  y may be x. */
+uint64_t    b200_ln_fprop_scratch_bytes(int64_t features, int64_t items);
 b200_status b200_ln_fprop(const b200_matrix *x, const b200_matrix *y, uint64_t gamma, uint64_t beta,
                           int32_t param_dtype, uint64_t mean, uint64_t rstd, int64_t features, int64_t items,
-                          float eps, uint64_t stream, int32_t *launches);
+                          float eps, uint64_t scratch, uint64_t scratch_bytes, uint64_t stream, int32_t *launches);
 /* its gradient: delta with respect to x (may be x or the error), grad_gamma and grad_beta
  * (param_dtype, optional) summed over the items; mean and rstd as the forward call wrote them */
 uint64_t    b200_ln_bprop_scratch_bytes(int64_t features, int64_t items);

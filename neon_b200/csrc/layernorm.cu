@@ -444,182 +444,369 @@ template <bool BACK> cudaError_t launch_type(const LnP& p, bool mis, float* part
 //
 // A block takes a stripe of neighbouring items, `lanes` threads with V items each side by side and
 // its other threads down the features, so every access is a run of 32 to 128 bytes of a feature's
-// row.  The stripe is walked through three times forward (sum, centred squares, result) and twice
-// backwards.  HELD: it is copied to shared memory first, every thread's own vectors by itself, so
-// HBM is read once; a stripe that does not fit is read again, from L2 if that holds the stripes
-// under way.
-template <int V> DEV void stripe_sum(float (&v)[V], float* s, int lanes) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, tx = threadIdx.x & (lanes - 1);
+// row.  With enough stripes for the machine a block sees all features of its items: it copies the
+// stripe to shared memory (HELD; every thread its own vectors), so HBM is read once, or, where that
+// is too small, walks over it again.  With few stripes the features are split over blocks as well,
+// and a second kernel joins their sums: of a share of n_i features its mean m_i and centred squares
+// q_i, which give the item's mean sum n_i m_i / F and squares sum q_i + n_i (m_i - mean)^2.
+//
+// Neighbouring items as pairs; a single item (V = 1) is a pair with 0.
+template <int DT, int V> struct Items {
+    static constexpr int P = V > 1 ? V / 2 : 1, W = V > 1 ? 4 : 1;
+    u32 w[W];
+    DEV void load(u64 base, i64 at) { ld_w<DT, V, false>(base, at, w); }
+    DEV void load(const u32* held) { ld_raw<dt_size<DT>::value * V, false>(reinterpret_cast<const char*>(held), w); }
+    DEV f32x2 get(int l) const {
+        if constexpr (V > 1) return get2<DT>(w, l);
+        else { float z[1]; cvt_in<DT, 1>(w, z); return pair(z[0], 0.f); }
+    }
+    DEV void set(int l, f32x2 v) {
+        if constexpr (V > 1) set2<DT>(w, l, v);
+        else { float x, y; split(v, x, y); cvt_out<DT, 1, false>(&x, w, SrCtx(), nullptr); }
+    }
+    DEV void store(u64 base, i64 at) const { st_raw<dt_size<DT>::value * V>(reinterpret_cast<char*>(base) + at * dt_size<DT>::value, w); }
+};
+// One value per item of a thread, from a vector of one value per item, and back.
+template <int V> DEV void get_items(u64 base, i64 n, f32x2* v) {
+    const float* at = reinterpret_cast<const float*>(base) + n;
+    if constexpr (V > 1) {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        for (int o = 16; o >= lanes; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        for (int l = 0; l < V / 2; ++l) v[l] = pair(at[2 * l], at[2 * l + 1]);
+    } else v[0] = pair(at[0], 0.f);
+}
+template <int V> DEV void put_items(u64 base, i64 n, const f32x2* v) {
+    float* at = reinterpret_cast<float*>(base) + n;
+#pragma unroll
+    for (int l = 0; l < (V > 1 ? V / 2 : 1); ++l) {
+        float x, y;
+        split(v[l], x, y);
+        at[V > 1 ? 2 * l : 0] = x;
+        if constexpr (V > 1) at[2 * l + 1] = y;
+    }
+}
+DEV f32x2 both_of(float x) { return pair(x, x); }
+DEV f32x2 minus(f32x2 v) { float x, y; split(v, x, y); return pair(-x, -y); }
+
+// Sums over the threads of a stripe that share its items: within the warps, then by one thread per
+// value over the warps; `s` holds 17 times the stripe's items.
+enum { kColsT = 512, kColsWarps = kColsT / 32 };
+template <int V> DEV void stripe_sum(f32x2* v, float* s, int lanes) {
+    constexpr int P = V > 1 ? V / 2 : 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tx = threadIdx.x & (lanes - 1), wide = lanes * 2 * P;
+#pragma unroll
+    for (int l = 0; l < P; ++l) {
+        float x, y;
+        split(v[l], x, y);
+        for (int o = 16; o >= lanes; o >>= 1) {
+            x += __shfl_xor_sync(0xffffffffu, x, o);
+            y += __shfl_xor_sync(0xffffffffu, y, o);
+        }
+        v[l] = pair(x, y);
+    }
     __syncthreads();
     if (lane < lanes) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[(warp * lanes + tx) * V + i] = v[i];
+        for (int l = 0; l < P; ++l) *reinterpret_cast<f32x2*>(s + warp * wide + tx * 2 * P + 2 * l) = v[l];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < wide; i += kColsT) {
+        float a = 0.f;
+#pragma unroll
+        for (int w = 0; w < kColsWarps; ++w) a += s[w * wide + i];
+        s[kColsWarps * wide + i] = a;
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        float a = 0.f;
-        for (int w = 0; w < warps; ++w) a += s[(w * lanes + tx) * V + i];
-        v[i] = a;
+    for (int l = 0; l < P; ++l) v[l] = *reinterpret_cast<const f32x2*>(s + kColsWarps * wide + tx * 2 * P + 2 * l);
+}
+enum { kStripeFloats = (kColsWarps + 1) * 64 };     // at most 64 values side by side
+
+// A thread's place in its stripe, and its features: first, first + rows, ... below end.
+struct Place { int lanes, tx, ty, rows, F; i64 n; bool in; };
+template <int V> DEV Place place(i64 stripe, int lanes, i64 N, i64 F) {
+    Place q;
+    q.lanes = lanes; q.tx = threadIdx.x & (lanes - 1); q.ty = threadIdx.x / lanes; q.rows = blockDim.x / lanes; q.F = (int)F;
+    q.n = (stripe * lanes + q.tx) * V;
+    q.in = q.n < N;
+    return q;
+}
+// A thread's vectors of a stripe, copied to its own places in shared memory.
+template <int DT> DEV void hold(const u32* to, u64 base, i64 pitch, const Place& q) {
+    u32 at = (u32)__cvta_generic_to_shared(to + threadIdx.x * 4);
+    for (int f = q.ty; f < q.F; f += q.rows, at += blockDim.x * 16) copy16(at, base + (u64)((f * pitch + q.n) * dt_size<DT>::value));
+}
+template <int DT, int V, bool HELD> DEV void look(Items<DT, V>& x, const u32* held, int k, u64 base, i64 at) {
+    if constexpr (HELD) x.load(held + (k * blockDim.x + threadIdx.x) * 4);
+    else x.load(base, at);
+}
+// mean and centred squares of features [f0, f1) of the stripe's items
+template <int DT, int V, bool HELD> DEV void moments(const LnP& p, const Place& q, const u32* held, int f0, int f1, float* s, f32x2* mean, f32x2* squares) {
+    constexpr int P = Items<DT, V>::P;
+#pragma unroll
+    for (int l = 0; l < P; ++l) mean[l] = squares[l] = 0;
+    if (q.in) {
+#pragma unroll 4
+        for (int f = f0 + q.ty, k = 0; f < f1; f += q.rows, ++k) {
+            Items<DT, V> x;
+            look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
+#pragma unroll
+            for (int l = 0; l < P; ++l) mean[l] = add2(mean[l], x.get(l));
+        }
+    }
+    stripe_sum<V>(mean, s, q.lanes);
+    f32x2 less[P];
+#pragma unroll
+    for (int l = 0; l < P; ++l) {
+        mean[l] = mul2(mean[l], both_of(1.f / (float)(f1 - f0)));
+        less[l] = minus(mean[l]);
+    }
+    if (q.in) {
+#pragma unroll 4
+        for (int f = f0 + q.ty, k = 0; f < f1; f += q.rows, ++k) {
+            Items<DT, V> x;
+            look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
+#pragma unroll
+            for (int l = 0; l < P; ++l) { const f32x2 d = add2(x.get(l), less[l]); squares[l] = fma2(d, d, squares[l]); }
+        }
+    }
+    stripe_sum<V>(squares, s, q.lanes);
+}
+// 1 / sqrt(squares / F + eps), in place
+template <int P> DEV void to_rstd(f32x2 (&v)[P], float inv, float eps) {
+#pragma unroll
+    for (int l = 0; l < P; ++l) {
+        float x, y;
+        split(v[l], x, y);
+        v[l] = pair(1.f / sqrtf(x * inv + eps), 1.f / sqrtf(y * inv + eps));
     }
 }
-
-// A thread's vectors of a stripe, copied to its own places in shared memory (i: which of them).
-template <int DT> DEV void hold(u32 to, u64 base, i64 f0, i64 step, i64 pitch, i64 n, int F) {
-    for (i64 f = f0; f < F; f += step, to += blockDim.x * 16) copy16(to, base + (u64)((f * pitch + n) * dt_size<DT>::value));
-}
-template <int DT, int V, bool HELD> DEV void look(const u32* held, int i, u64 base, i64 at, float* x) {
-    if constexpr (HELD) {
-        u32 w[4];
-        ld_raw<16, false>(reinterpret_cast<const char*>(held + (i * blockDim.x + threadIdx.x) * 4), w);
-        cvt_in<DT, V>(w, x);
-    } else {
-        ld_f<DT, V, false>(base, at, x);
+template <int DT, int V, bool HELD> DEV void normalise(const LnP& p, const Place& q, const u32* held, int f0, int f1, const f32x2* mean, const f32x2* rstd) {
+    constexpr int P = Items<DT, V>::P;
+    f32x2 less[P];
+#pragma unroll
+    for (int l = 0; l < P; ++l) less[l] = minus(mean[l]);
+#pragma unroll 4
+    for (int f = f0 + q.ty, k = 0; f < f1; f += q.rows, ++k) {
+        const f32x2 g = both_of(p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f), b = both_of(p.beta ? ld_any(p.beta, f, p.pdt) : 0.f);
+        Items<DT, V> x;
+        look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
+#pragma unroll
+        for (int l = 0; l < P; ++l) x.set(l, fma2(mul2(add2(x.get(l), less[l]), rstd[l]), g, b));
+        x.store(p.out, f * p.o0 + q.n);
     }
 }
 
 template <int DT, int V, bool HELD>
-__global__ void __launch_bounds__(512) ln_fprop_cols(const __grid_constant__ LnP p, int lanes) {
+__global__ void __launch_bounds__(kColsT) ln_fprop_cols(const __grid_constant__ LnP p, int lanes) {
     extern __shared__ __align__(16) u32 held[];
-    __shared__ float s[16 * 32 * (V > 1 ? 2 : 1)];     // [warps][lanes][V]: 8 lanes of vectors, or 32 of single items
-    const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = blockDim.x / lanes, F = (int)p.F;
-    const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
-    const bool in = n < p.N;
-    const float inv = 1.f / (float)F;
-    float mean[V], rstd[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) mean[i] = rstd[i] = 0.f;
+    __shared__ __align__(16) float s[kStripeFloats];
+    const Place q = place<V>(blockIdx.x, lanes, p.N, p.F);
     if constexpr (HELD) {
-        if (in) hold<DT>((u32)__cvta_generic_to_shared(held) + threadIdx.x * 16, p.x, ty, rows, p.x0, n, F);
+        if (q.in) hold<DT>(held, p.x, p.x0, q);
         copy_commit();
         copy_wait<0>();
     }
-    if (in) {
-#pragma unroll 4
-        for (int f = ty, k = 0; f < F; f += rows, ++k) {
-            float x[V];
-            look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
+    f32x2 mean[Items<DT, V>::P], rstd[Items<DT, V>::P];
+    moments<DT, V, HELD>(p, q, held, 0, q.F, s, mean, rstd);
+    to_rstd(rstd, 1.f / (float)q.F, p.eps);
+    if (!q.in) return;
+    if (q.ty == 0) {
+        if (p.mean) put_items<V>(p.mean, q.n, mean);
+        if (p.rstd) put_items<V>(p.rstd, q.n, rstd);
+    }
+    normalise<DT, V, HELD>(p, q, held, 0, q.F, mean, rstd);
+}
+
+// part[split][0][N]: mean, part[split][1][N]: centred squares of a share of `per` features
+template <int DT, int V>
+__global__ void __launch_bounds__(kColsT) ln_split_moments(const __grid_constant__ LnP p, int lanes, int per, float* part) {
+    grid_enter();
+    __shared__ __align__(16) float s[kStripeFloats];
+    const Place q = place<V>(blockIdx.x, lanes, p.N, p.F);
+    const int f0 = blockIdx.y * per, f1 = min(f0 + per, q.F);
+    f32x2 mean[Items<DT, V>::P], squares[Items<DT, V>::P];
+    moments<DT, V, false>(p, q, nullptr, f0, f1, s, mean, squares);
+    if (!q.in || q.ty) return;
+    float* to = part + (i64)blockIdx.y * 2 * p.N;
+    put_items<V>((u64)to, q.n, mean);
+    put_items<V>((u64)(to + p.N), q.n, squares);
+}
+template <int DT, int V>
+__global__ void __launch_bounds__(kColsT) ln_split_fprop(const __grid_constant__ LnP p, int lanes, int per, const float* part) {
+    grid_enter();
+    constexpr int P = Items<DT, V>::P;
+    const Place q = place<V>(blockIdx.x, lanes, p.N, p.F);
+    if (!q.in) return;
+    const float inv = 1.f / (float)q.F;
+    f32x2 mean[P], rstd[P], m[P], m2[P];
 #pragma unroll
-            for (int i = 0; i < V; ++i) mean[i] += x[i];
+    for (int l = 0; l < P; ++l) mean[l] = rstd[l] = 0;
+    for (int k = 0; k < (int)gridDim.y; ++k) {
+        get_items<V>((u64)(part + (i64)k * 2 * p.N), q.n, m);
+        const float n = (float)(min((k + 1) * per, q.F) - k * per) * inv;
+#pragma unroll
+        for (int l = 0; l < P; ++l) mean[l] = fma2(m[l], both_of(n), mean[l]);
+    }
+    for (int k = 0; k < (int)gridDim.y; ++k) {
+        get_items<V>((u64)(part + (i64)k * 2 * p.N), q.n, m);
+        get_items<V>((u64)(part + ((i64)k * 2 + 1) * p.N), q.n, m2);
+        const float n = (float)(min((k + 1) * per, q.F) - k * per);
+#pragma unroll
+        for (int l = 0; l < P; ++l) {
+            const f32x2 d = add2(m[l], minus(mean[l]));
+            rstd[l] = fma2(mul2(d, both_of(n)), d, add2(rstd[l], m2[l]));
         }
     }
-    stripe_sum<V>(mean, s, lanes);
+    to_rstd(rstd, inv, p.eps);
+    if (q.ty == 0 && blockIdx.y == 0) {
+        if (p.mean) put_items<V>(p.mean, q.n, mean);
+        if (p.rstd) put_items<V>(p.rstd, q.n, rstd);
+    }
+    const int f0 = blockIdx.y * per;
+    normalise<DT, V, false>(p, q, nullptr, f0, min(f0 + per, q.F), mean, rstd);
+}
+
+// Sums of g and g h over features [f0, f1) of the stripe's items, and the stripe's share of the
+// parameters' gradients at those features, added to acc (`more`) or put there.
+template <int DT, int V, bool HELD> DEV void error_sums(const LnP& p, const Place& q, const u32* held, const u32* held_e, int f0, int f1,
+                                                        float* s, const f32x2* mean, const f32x2* rstd, f32x2* a, f32x2* b, float* acc, bool more) {
+    constexpr int P = Items<DT, V>::P;
+    f32x2 less[P];
 #pragma unroll
-    for (int i = 0; i < V; ++i) mean[i] *= inv;
-    if (in) {
-#pragma unroll 4
-        for (int f = ty, k = 0; f < F; f += rows, ++k) {
-            float x[V];
-            look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
+    for (int l = 0; l < P; ++l) { a[l] = b[l] = 0; less[l] = minus(mean[l]); }
+#pragma unroll 2
+    for (int f = f0 + q.ty, k = 0; f - q.ty < f1; f += q.rows, ++k) {       // all threads: the lanes of a feature add up below
+        f32x2 gg = 0, gb = 0;
+        if (q.in && f < f1) {
+            const f32x2 gamma = both_of(p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f);
+            Items<DT, V> x, e;
+            look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
+            look<DT, V, HELD>(e, held_e, k, p.e, f * p.e0 + q.n);
 #pragma unroll
-            for (int i = 0; i < V; ++i) { x[i] -= mean[i]; rstd[i] = fmaf(x[i], x[i], rstd[i]); }
+            for (int l = 0; l < P; ++l) {
+                const f32x2 h = mul2(add2(x.get(l), less[l]), rstd[l]), err = e.get(l), g = mul2(err, gamma);
+                gg = fma2(err, h, gg);
+                gb = add2(err, gb);
+                a[l] = add2(a[l], g);
+                b[l] = fma2(g, h, b[l]);
+            }
+        }
+        if (acc) {
+            float x = both(gg), y = both(gb);
+            for (int o = q.lanes >> 1; o; o >>= 1) {
+                x += __shfl_xor_sync(0xffffffffu, x, o);
+                y += __shfl_xor_sync(0xffffffffu, y, o);
+            }
+            if (q.tx == 0 && f < f1) {
+                acc[f] = (more ? acc[f] : 0.f) + x;
+                acc[q.F + f] = (more ? acc[q.F + f] : 0.f) + y;
+            }
         }
     }
-    stripe_sum<V>(rstd, s, lanes);
+    stripe_sum<V>(a, s, q.lanes);
+    stripe_sum<V>(b, s, q.lanes);
+}
+template <int DT, int V, bool HELD> DEV void put_delta(const LnP& p, const Place& q, const u32* held, const u32* held_e, int f0, int f1,
+                                                       const f32x2* mean, const f32x2* rstd, const f32x2* a, const f32x2* b) {
+    constexpr int P = Items<DT, V>::P;
+    const f32x2 inv = both_of(-1.f / (float)q.F);
+    f32x2 less[P], ma[P], mb[P];
 #pragma unroll
-    for (int i = 0; i < V; ++i) rstd[i] = 1.f / sqrtf(rstd[i] * inv + p.eps);
-    if (!in) return;
-    if (ty == 0) {
+    for (int l = 0; l < P; ++l) { less[l] = minus(mean[l]); ma[l] = mul2(a[l], inv); mb[l] = mul2(b[l], inv); }
+#pragma unroll 2
+    for (int f = f0 + q.ty, k = 0; f < f1; f += q.rows, ++k) {
+        const f32x2 gamma = both_of(p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f);
+        Items<DT, V> x, e;
+        look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
+        look<DT, V, HELD>(e, held_e, k, p.e, f * p.e0 + q.n);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (p.mean) reinterpret_cast<float*>(p.mean)[n + i] = mean[i];
-            if (p.rstd) reinterpret_cast<float*>(p.rstd)[n + i] = rstd[i];
+        for (int l = 0; l < P; ++l) {
+            const f32x2 h = mul2(add2(x.get(l), less[l]), rstd[l]);
+            x.set(l, mul2(rstd[l], fma2(h, mb[l], fma2(e.get(l), gamma, ma[l]))));
         }
-    }
-#pragma unroll 4
-    for (int f = ty, k = 0; f < F; f += rows, ++k) {
-        const float g = p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f, b = p.beta ? ld_any(p.beta, f, p.pdt) : 0.f;
-        float x[V];
-        look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = fmaf((x[i] - mean[i]) * rstd[i], g, b);
-        st_f<DT, V>(p.out, f * p.o0 + n, x);
+        x.store(p.out, f * p.o0 + q.n);
     }
 }
 
-// part[block][0][F]: the block's share of grad_gamma, part[block][1][F]: of grad_beta; a block
-// works through stripes gridDim.x apart and adds to its own shares.
+// A block works through stripes gridDim.x apart; part[block][0][F]: its share of grad_gamma,
+// part[block][1][F]: of grad_beta, gathered in shared memory if `acc_held`.
 template <int DT, int V, bool HELD>
-__global__ void __launch_bounds__(512) ln_bprop_cols(const __grid_constant__ LnP p, float* part, int lanes, i64 stripes) {
-    extern __shared__ __align__(16) u32 held[];        // x, then the error
-    __shared__ float s[16 * 32 * (V > 1 ? 2 : 1)];
-    const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = blockDim.x / lanes, F = (int)p.F;
-    const int each = (F + rows - 1) / rows;            // vectors per thread
-    const u32* held_e = held + each * blockDim.x * 4;
-    const float inv = 1.f / (float)F;
-    float* mine = part + (i64)blockIdx.x * 2 * F;
+__global__ void __launch_bounds__(kColsT) ln_bprop_cols(const __grid_constant__ LnP p, float* part, int lanes, i64 stripes, int acc_held) {
+    extern __shared__ __align__(16) u32 mem[];         // x, the error, the block's share of the gradients
+    __shared__ __align__(16) float s[kStripeFloats];
+    constexpr int P = Items<DT, V>::P;
+    const int F = (int)p.F, rows = kColsT / lanes, each = HELD ? (F + rows - 1) / rows : 0;
+    const u32 *held = mem, *held_e = mem + each * kColsT * 4;
+    float* mine = part ? part + (i64)blockIdx.x * 2 * F : nullptr;
+    float* acc = part && acc_held ? reinterpret_cast<float*>(mem + 2 * each * kColsT * 4) : mine;
     for (i64 stripe = blockIdx.x; stripe < stripes; stripe += gridDim.x) {
-        const i64 n = (stripe * lanes + tx) * V;
-        const bool in = n < p.N;
+        const Place q = place<V>(stripe, lanes, p.N, p.F);
         if constexpr (HELD) {
-            if (in) {
-                const u32 to = (u32)__cvta_generic_to_shared(held) + threadIdx.x * 16;
-                hold<DT>(to, p.x, ty, rows, p.x0, n, F);
-                hold<DT>(to + each * blockDim.x * 16, p.e, ty, rows, p.e0, n, F);
+            if (q.in) {
+                hold<DT>(held, p.x, p.x0, q);
+                hold<DT>(held_e, p.e, p.e0, q);
             }
             copy_commit();
         }
-        float mean[V], rstd[V], a[V], b[V];
+        f32x2 mean[P], rstd[P], a[P], b[P];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            mean[i] = in ? reinterpret_cast<const float*>(p.mean)[n + i] : 0.f;
-            rstd[i] = in ? reinterpret_cast<const float*>(p.rstd)[n + i] : 0.f;
-            a[i] = b[i] = 0.f;
+        for (int l = 0; l < P; ++l) mean[l] = rstd[l] = 0;
+        if (q.in) {
+            get_items<V>(p.mean, q.n, mean);
+            get_items<V>(p.rstd, q.n, rstd);
         }
         if constexpr (HELD) copy_wait<0>();
-#pragma unroll 2
-        for (int k = 0; k < each; ++k) {               // all threads: the lanes of a feature add up below
-            const int f = k * rows + ty;
-            float gg = 0.f, gb = 0.f;
-            if (in && f < F) {
-                const float gamma = p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f;
-                float x[V], e[V];
-                look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
-                look<DT, V, HELD>(held_e, k, p.e, f * p.e0 + n, e);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    x[i] = (x[i] - mean[i]) * rstd[i];
-                    gg = fmaf(e[i], x[i], gg);
-                    gb += e[i];
-                    e[i] *= gamma;
-                    a[i] += e[i];
-                    b[i] = fmaf(e[i], x[i], b[i]);
-                }
-            }
-            if (part) {
-                for (int o = lanes >> 1; o; o >>= 1) {
-                    gg += __shfl_xor_sync(0xffffffffu, gg, o);
-                    gb += __shfl_xor_sync(0xffffffffu, gb, o);
-                }
-                if (tx == 0 && f < F) {
-                    const bool more = stripe != blockIdx.x;
-                    mine[f] = (more ? mine[f] : 0.f) + gg;
-                    mine[F + f] = (more ? mine[F + f] : 0.f) + gb;
-                }
-            }
-        }
-        stripe_sum<V>(a, s, lanes);
-        stripe_sum<V>(b, s, lanes);
-        if (!in) continue;
-#pragma unroll
-        for (int i = 0; i < V; ++i) { a[i] *= inv; b[i] *= inv; }
-#pragma unroll 2
-        for (int f = ty, k = 0; f < F; f += rows, ++k) {
-            const float gamma = p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f;
-            float x[V], e[V];
-            look<DT, V, HELD>(held, k, p.x, f * p.x0 + n, x);
-            look<DT, V, HELD>(held_e, k, p.e, f * p.e0 + n, e);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                x[i] = (x[i] - mean[i]) * rstd[i];
-                e[i] = rstd[i] * ((e[i] * gamma - a[i]) - x[i] * b[i]);
-            }
-            st_f<DT, V>(p.out, f * p.o0 + n, e);
-        }
+        error_sums<DT, V, HELD>(p, q, held, held_e, 0, F, s, mean, rstd, a, b, acc, stripe != blockIdx.x);
+        if (q.in) put_delta<DT, V, HELD>(p, q, held, held_e, 0, F, mean, rstd, a, b);
     }
+    if (acc == mine) return;
+    __syncthreads();
+    for (int f = threadIdx.x; f < 2 * F; f += kColsT) mine[f] = acc[f];
+}
+
+// sums[split][0][N]: of g, sums[split][1][N]: of g h over a share of `per` features;
+// part[stripe][2][F] as above, every feature by one block
+template <int DT, int V>
+__global__ void __launch_bounds__(kColsT) ln_split_sums(const __grid_constant__ LnP p, int lanes, int per, float* sums, float* part) {
+    grid_enter();
+    __shared__ __align__(16) float s[kStripeFloats];
+    constexpr int P = Items<DT, V>::P;
+    const Place q = place<V>(blockIdx.x, lanes, p.N, p.F);
+    const int f0 = blockIdx.y * per, f1 = min(f0 + per, q.F);
+    f32x2 mean[P], rstd[P], a[P], b[P];
+#pragma unroll
+    for (int l = 0; l < P; ++l) mean[l] = rstd[l] = 0;
+    if (q.in) {
+        get_items<V>(p.mean, q.n, mean);
+        get_items<V>(p.rstd, q.n, rstd);
+    }
+    error_sums<DT, V, false>(p, q, nullptr, nullptr, f0, f1, s, mean, rstd, a, b, part ? part + (i64)blockIdx.x * 2 * p.F : nullptr, false);
+    if (!q.in || q.ty) return;
+    float* to = sums + (i64)blockIdx.y * 2 * p.N;
+    put_items<V>((u64)to, q.n, a);
+    put_items<V>((u64)(to + p.N), q.n, b);
+}
+template <int DT, int V>
+__global__ void __launch_bounds__(kColsT) ln_split_delta(const __grid_constant__ LnP p, int lanes, int per, const float* sums) {
+    grid_enter();
+    constexpr int P = Items<DT, V>::P;
+    const Place q = place<V>(blockIdx.x, lanes, p.N, p.F);
+    if (!q.in) return;
+    f32x2 mean[P], rstd[P], a[P], b[P], x[P];
+    get_items<V>(p.mean, q.n, mean);
+    get_items<V>(p.rstd, q.n, rstd);
+#pragma unroll
+    for (int l = 0; l < P; ++l) a[l] = b[l] = 0;
+    for (int k = 0; k < (int)gridDim.y; ++k) {
+        get_items<V>((u64)(sums + (i64)k * 2 * p.N), q.n, x);
+#pragma unroll
+        for (int l = 0; l < P; ++l) a[l] = add2(a[l], x[l]);
+        get_items<V>((u64)(sums + ((i64)k * 2 + 1) * p.N), q.n, x);
+#pragma unroll
+        for (int l = 0; l < P; ++l) b[l] = add2(b[l], x[l]);
+    }
+    const int f0 = blockIdx.y * per;
+    put_delta<DT, V, false>(p, q, nullptr, nullptr, f0, min(f0 + per, q.F), mean, rstd, a, b);
 }
 
 // Whether the matrices have their items next to each other; `wide`: in whole 16-byte vectors.
@@ -633,39 +820,87 @@ bool cols_fit(const b200_matrix* const* m, int count, i64 N, bool& wide) {
     return true;
 }
 
-// Stripes of 128 bytes, or down to 32 bytes where wider ones would leave SMs without a block, or
-// would not fit twice into an SM's shared memory.
-template <int DT, int V, bool BACK, bool HELD> cudaError_t launch_cols_of(const LnP& p, int lanes, int smem, float* part, int* parts, cudaStream_t s) {
-    const i64 stripes = (p.N + (i64)lanes * V - 1) / ((i64)lanes * V);
-    if constexpr (BACK) {
-        i64 grid = resident_blocks(ln_bprop_cols<DT, V, HELD>, 512, smem);
-        if (!grid) return cudaErrorInvalidConfiguration;
-        if (grid > stripes) grid = stripes;
-        if (part && grid > most_parts(p.F)) grid = most_parts(p.F);
-        *parts = (int)grid;
-        ln_bprop_cols<DT, V, HELD><<<(unsigned)grid, 512, smem, s>>>(p, part, lanes, stripes);
-    } else {
-        if (!resident_blocks(ln_fprop_cols<DT, V, HELD>, 512, smem)) return cudaErrorInvalidConfiguration;
-        ln_fprop_cols<DT, V, HELD><<<(unsigned)stripes, 512, smem, s>>>(p, lanes);
+// How a call in this order is cut.  Stripes of 128 bytes, or down to 32 bytes where wider ones would
+// leave SMs without a block or would not fit twice into an SM's shared memory; below 148 stripes of
+// 32 bytes, the features in shares of at least 4 per thread, at most 64 of them.
+enum { kMaxSplits = 64 };
+struct Cols { int lanes, splits, per, held; i64 stripes; };
+Cols cols_plan(i64 F, i64 N, int size, int V, bool back) {          // size: bytes of a thread's items
+    Cols c;
+    c.lanes = 128 / size > 32 ? 32 : 128 / size;
+    auto stripes = [&](int l) { return (N + (i64)l * V - 1) / ((i64)l * V); };
+    while (c.lanes > 1 && c.lanes * size > 32 && stripes(c.lanes) < 2 * 148) c.lanes /= 2;
+    c.splits = 1; c.per = (int)F; c.held = 0;
+    c.stripes = stripes(c.lanes);
+    if (c.stripes < 148) {
+        i64 splits = 2 * 148 / c.stripes, most = F / (4 * (kColsT / c.lanes));
+        if (splits > most) splits = most;
+        if (splits > kMaxSplits) splits = kMaxSplits;
+        if (splits > 1) {
+            c.per = (int)((F + splits - 1) / splits);
+            c.splits = (int)((F + c.per - 1) / c.per);
+            return c;
+        }
     }
+    if (V > 1) {
+        auto bytes = [&](int l) { return (F + kColsT / l - 1) / (kColsT / l) * kColsT * 16 * (back ? 2 : 1); };
+        while (c.lanes > 2 && bytes(c.lanes) > 100 * 1024) c.lanes /= 2;
+        if (bytes(c.lanes) <= 200 * 1024) c.held = (int)bytes(c.lanes);
+        c.stripes = stripes(c.lanes);
+    }
+    return c;
+}
+// Scratch of the split form, in front of the gradients' shares.
+inline i64 split_bytes(i64 N) { return N < 148 * 64 ? (kMaxSplits * 8 * N + 255) / 256 * 256 : 0; }
+
+template <int DT, int V, bool HELD> cudaError_t launch_cols_back(const LnP& p, const Cols& c, float* part, int* parts, cudaStream_t s) {
+    const int acc = part && p.F <= 4096 && c.held + 8 * p.F <= 216 * 1024 ? (int)(8 * p.F) : 0, smem = c.held + acc;
+    i64 grid = resident_blocks(ln_bprop_cols<DT, V, HELD>, kColsT, smem);
+    if (!grid) return cudaErrorInvalidConfiguration;
+    if (grid > c.stripes) grid = c.stripes;
+    if (part && grid > most_parts(p.F)) grid = most_parts(p.F);
+    *parts = (int)grid;
+    ln_bprop_cols<DT, V, HELD><<<(unsigned)grid, kColsT, smem, s>>>(p, part, c.lanes, c.stripes, acc != 0);
     return cudaGetLastError();
 }
-template <int DT, int V, bool BACK> cudaError_t launch_cols(const LnP& p, float* part, int* parts, cudaStream_t s) {
-    constexpr int size = dt_size<DT>::value * V;
-    int lanes = 128 / size > 32 ? 32 : 128 / size;
-    while (lanes * size > 32 && lanes > 1 && (p.N + (i64)lanes * V - 1) / ((i64)lanes * V) < 2 * 148) lanes /= 2;
-    if constexpr (V > 1) {
-        auto bytes = [&](int l) { return (p.F + 512 / l - 1) / (512 / l) * 512 * 16 * (BACK ? 2 : 1); };
-        while (lanes > 2 && bytes(lanes) > 100 * 1024) lanes /= 2;
-        if (bytes(lanes) <= 216 * 1024) return launch_cols_of<DT, V, BACK, true>(p, lanes, (int)bytes(lanes), part, parts, s);
+template <int DT, int V, bool BACK> cudaError_t launch_cols(const LnP& p, char* scratch, float* part, int* parts, int& launches, cudaStream_t s) {
+    const Cols c = cols_plan(p.F, p.N, dt_size<DT>::value * V, V, BACK);
+    float* sums = reinterpret_cast<float*>(scratch);
+    const dim3 grid((unsigned)c.stripes, (unsigned)c.splits);
+    if (c.splits > 1) {
+        launches += 2;
+        cudaError_t e;
+        if constexpr (BACK) {
+            *parts = (int)c.stripes;
+            e = launch_dependent(ln_split_sums<DT, V>, grid, kColsT, 0, s, p, c.lanes, c.per, sums, part);
+            if (e == cudaSuccess) e = launch_dependent(ln_split_delta<DT, V>, grid, kColsT, 0, s, p, c.lanes, c.per, (const float*)sums);
+        } else {
+            e = launch_dependent(ln_split_moments<DT, V>, grid, kColsT, 0, s, p, c.lanes, c.per, sums);
+            if (e == cudaSuccess) e = launch_dependent(ln_split_fprop<DT, V>, grid, kColsT, 0, s, p, c.lanes, c.per, (const float*)sums);
+        }
+        return e;
     }
-    return launch_cols_of<DT, V, BACK, false>(p, lanes, 0, part, parts, s);
+    ++launches;
+    if constexpr (BACK) {
+        if constexpr (V > 1) if (c.held) return launch_cols_back<DT, V, true>(p, c, part, parts, s);
+        return launch_cols_back<DT, V, false>(p, c, part, parts, s);
+    } else {
+        if constexpr (V > 1) {
+            if (c.held) {
+                if (!resident_blocks(ln_fprop_cols<DT, V, true>, kColsT, c.held)) return cudaErrorInvalidConfiguration;
+                ln_fprop_cols<DT, V, true><<<(unsigned)c.stripes, kColsT, c.held, s>>>(p, c.lanes);
+                return cudaGetLastError();
+            }
+        }
+        ln_fprop_cols<DT, V, false><<<(unsigned)c.stripes, kColsT, 0, s>>>(p, c.lanes);
+        return cudaGetLastError();
+    }
 }
-template <bool BACK> cudaError_t launch_cols_type(const LnP& p, bool wide, float* part, int* parts, cudaStream_t s) {
+template <bool BACK> cudaError_t launch_cols_type(const LnP& p, bool wide, char* scratch, float* part, int* parts, int& launches, cudaStream_t s) {
     switch (p.dt) {
-    case B200_F32: return wide ? launch_cols<F32, 4, BACK>(p, part, parts, s) : launch_cols<F32, 1, BACK>(p, part, parts, s);
-    case B200_F16: return wide ? launch_cols<F16, 8, BACK>(p, part, parts, s) : launch_cols<F16, 1, BACK>(p, part, parts, s);
-    default: return wide ? launch_cols<BF16, 8, BACK>(p, part, parts, s) : launch_cols<BF16, 1, BACK>(p, part, parts, s);
+    case B200_F32: return wide ? launch_cols<F32, 4, BACK>(p, scratch, part, parts, launches, s) : launch_cols<F32, 1, BACK>(p, scratch, part, parts, launches, s);
+    case B200_F16: return wide ? launch_cols<F16, 8, BACK>(p, scratch, part, parts, launches, s) : launch_cols<F16, 1, BACK>(p, scratch, part, parts, launches, s);
+    default: return wide ? launch_cols<BF16, 8, BACK>(p, scratch, part, parts, launches, s) : launch_cols<BF16, 1, BACK>(p, scratch, part, parts, launches, s);
     }
 }
 
@@ -681,9 +916,14 @@ b200_matrix vec(uint64_t ptr, int dt) { b200_matrix m; m.ptr = ptr; m.s0 = 1; m.
 
 }  // namespace
 
+extern "C" uint64_t b200_ln_fprop_scratch_bytes(int64_t features, int64_t items) {
+    return features < 1 || items < 1 ? 0 : (uint64_t)split_bytes(items);
+}
+
 extern "C" b200_status b200_ln_fprop(const b200_matrix* x, const b200_matrix* y, uint64_t gamma, uint64_t beta,
                                      int32_t param_dtype, uint64_t mean, uint64_t rstd, int64_t features,
-                                     int64_t items, float eps, uint64_t stream, int32_t* launches) {
+                                     int64_t items, float eps, uint64_t scratch, uint64_t scratch_bytes,
+                                     uint64_t stream, int32_t* launches) {
     const char* where = "b200_ln_fprop";
     if (launches) *launches = 0;
     if (!x || !y) return refuse(where, "null matrix");
@@ -693,6 +933,8 @@ extern "C" b200_status b200_ln_fprop(const b200_matrix* x, const b200_matrix* y,
     if (!(eps >= 0.f)) return refuse(where, "eps must not be negative");
     if (items == 0) return B200_OK;
     if (!x->ptr || !y->ptr) return refuse(where, "null device pointer");
+    const uint64_t need = b200_ln_fprop_scratch_bytes(features, items);
+    if (scratch_bytes < need || (need && (!scratch || scratch % 256))) return refuse(where, "scratch too small or misaligned");
     if (!same(*x, *y) && meet(*x, features, items, *y, features, items))
         return refuse(where, "y may be x itself or apart from it, not a shifted view of it");
     if (!aligned(x->ptr, x->dtype) || !aligned(y->ptr, y->dtype) || !aligned(gamma | beta, param_dtype) ||
@@ -719,22 +961,24 @@ extern "C" b200_status b200_ln_fprop(const b200_matrix* x, const b200_matrix* y,
     cudaError_t e = cudaSuccess;
     const b200_matrix* all[2] = {x, y};
     bool mis, wide;
+    int count = 1;
     if (rows_fit(all, 2, features, mis)) {
         e = launch_type<false>(p, mis, nullptr, nullptr, s);
     } else if (cols_fit(all, 2, items, wide)) {
-        e = launch_cols_type<false>(p, wide, nullptr, nullptr, s);
+        count = 0;
+        e = launch_cols_type<false>(p, wide, reinterpret_cast<char*>(scratch), nullptr, nullptr, count, s);
     } else {
         ln_fprop_any<<<blocks_for(items), 256, 0, s>>>(p);
         e = cudaGetLastError();
     }
-    if (launches) *launches = 1;
+    if (launches) *launches = count;
     return cuda_status(where, e);
 }
 
 extern "C" uint64_t b200_ln_bprop_scratch_bytes(int64_t features, int64_t items) {
     if (features < 1 || items < 1) return 0;
     const i64 parts = most_parts(features), want = items < 32 ? 32 : (items + 7) / 8 * 8;
-    return (uint64_t)((want < parts ? want : parts) * 8 * features);
+    return (uint64_t)(split_bytes(items) + (want < parts ? want : parts) * 8 * features);
 }
 
 extern "C" b200_status b200_ln_bprop(const b200_matrix* delta, const b200_matrix* error, const b200_matrix* x,
@@ -787,9 +1031,14 @@ extern "C" b200_status b200_ln_bprop(const b200_matrix* delta, const b200_matrix
     bool mis, wide;
     const bool rows = rows_fit(all, 3, features, mis);
     if (rows || cols_fit(all, 3, items, wide)) {
-        float* part = grad_gamma || grad_beta ? reinterpret_cast<float*>(scratch) : nullptr;
+        char* at = reinterpret_cast<char*>(scratch);
+        float* part = grad_gamma || grad_beta ? reinterpret_cast<float*>(at + split_bytes(items)) : nullptr;
         int parts = 0;
-        err = rows ? launch_type<true>(p, mis, part, &parts, s) : launch_cols_type<true>(p, wide, part, &parts, s);
+        if (rows) err = launch_type<true>(p, mis, part, &parts, s);
+        else {
+            count = 0;
+            err = launch_cols_type<true>(p, wide, at, part, &parts, count, s);
+        }
         if (part && err == cudaSuccess) {
             ln_sum_parts<<<(unsigned)((2 * features + 7) / 8), 1024, 0, s>>>(part, parts, features, grad_gamma, grad_beta, param_dtype);
             err = cudaGetLastError();

@@ -141,7 +141,8 @@ class LanguageModelOps(object):
                 self._lm_vector(mean, "mean", n, rt.F32, out=True),
                 self._lm_vector(rstd, "rstd", n, rt.F32, out=True))
         self._lm_check(x, y, gamma, beta, mean, rstd)
-        self.launches += rt.ln_fprop(mx, my, *args, f, n, float(eps), self.stream)
+        nbytes = rt.ln_fprop_scratch_bytes(f, n)
+        self.launches += rt.ln_fprop(mx, my, *args, f, n, float(eps), self._lm_scratch(nbytes), nbytes, self.stream)
         return y
 
     def compound_bprop_ln(self, delta_out, grad_gamma, grad_beta, delta_in, x, mean, rstd, gamma):

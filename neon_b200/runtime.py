@@ -85,7 +85,9 @@ SIGNATURES = {
     "b200_dimshuffle": (i32, [u64, u64, i32, i32, P(C.c_int64), P(C.c_int64), P(C.c_int64), u64]),
     "b200_compensated_sum": (i32, [u64, u64, u64, i32, u64, C.c_float, C.c_float, i32, u64]),
     "b200_log2_hist": (i32, [u64, i32, u64, u64, i32, i32, u64]),
-    "b200_ln_fprop": (i32, [P(Matrix), P(Matrix), u64, u64, i32, u64, u64, C.c_int64, C.c_int64, C.c_float, u64, P(i32)]),
+    "b200_ln_fprop_scratch_bytes": (u64, [C.c_int64, C.c_int64]),
+    "b200_ln_fprop": (i32, [P(Matrix), P(Matrix), u64, u64, i32, u64, u64, C.c_int64, C.c_int64, C.c_float, u64, u64, u64,
+                            P(i32)]),
     "b200_ln_bprop_scratch_bytes": (u64, [C.c_int64, C.c_int64]),
     "b200_ln_bprop": (i32, [P(Matrix), P(Matrix), P(Matrix), u64, u64, u64, u64, u64, i32, C.c_int64, C.c_int64,
                             u64, u64, u64, P(i32)]),
@@ -389,10 +391,15 @@ def log2_hist(src, dtype, count, hist, nbins, offset, stream=0):
     check(lib().b200_log2_hist(src, dtype, count, hist, nbins, offset, stream))
 
 
-def ln_fprop(x, y, gamma, beta, param_dtype, mean, rstd, features, items, eps, stream=0):
+def ln_fprop_scratch_bytes(features, items):
+    return int(lib().b200_ln_fprop_scratch_bytes(features, items))
+
+
+def ln_fprop(x, y, gamma, beta, param_dtype, mean, rstd, features, items, eps, scratch, scratch_bytes, stream=0):
     """Layer normalisation (matrices as ``Matrix``); returns the number of kernels launched."""
     n = i32(0)
-    check(lib().b200_ln_fprop(x, y, gamma, beta, param_dtype, mean, rstd, features, items, eps, stream, n))
+    check(lib().b200_ln_fprop(x, y, gamma, beta, param_dtype, mean, rstd, features, items, eps, scratch, scratch_bytes,
+                              stream, n))
     return n.value
 
 

@@ -149,17 +149,17 @@ def test_entry_points_refuse_null_and_misaligned(be):
     m = rt.Matrix(1 << 20, 1, 8, rt.F32, 0)
     odd = rt.Matrix((1 << 20) + 2, 1, 8, rt.F32, 0)
     far = rt.Matrix(1 << 30, 1, 8, rt.F32, 0)
-    assert lib.b200_ln_fprop(None, m, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 0, None) == -1
-    assert lib.b200_ln_fprop(odd, far, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 0, None) == -1 and "misaligned" in rt.last_error()
-    assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 0, 4, 1e-5, 0, None) == -1
-    assert lib.b200_ln_fprop(m, far, 0, 0, rt.I32, 0, 0, 8, 4, 1e-5, 0, None) == -7
-    assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 8, -1, 1e-5, 0, None) == -1
+    assert lib.b200_ln_fprop(None, m, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 0, 0, 0, None) == -1
+    assert lib.b200_ln_fprop(odd, far, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 0, 0, 0, None) == -1 and "misaligned" in rt.last_error()
+    assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 0, 4, 1e-5, 0, 0, 0, None) == -1
+    assert lib.b200_ln_fprop(m, far, 0, 0, rt.I32, 0, 0, 8, 4, 1e-5, 0, 0, 0, None) == -7
+    assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 8, -1, 1e-5, 0, 0, 0, None) == -1
     assert lib.b200_lut_bprop(1 << 22, m, far, 8, 8, 4, -1, 1.0, 0.0, 0, 0, 0, None) == -1 and "scratch" in rt.last_error()
     assert lib.b200_distill(m, None, None, m, 0, 1 << 25, 8, 4, 2, 1.0, 0, 0, 0, None) == -1
     assert lib.b200_policy(m, None, 0, 0, 0, 0, 0, 1 << 25, 0, 8, 4, 0.2, 0.2, 0.0, 0, 0, 0, None) == -1
     if rt.device_count() == 0:                       # a good call reports the missing device
         n = C.c_int32(5)
-        assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 0, n) == -2 and n.value == 0
+        assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 1 << 40, 1 << 30, 0, n) == -2 and n.value == 0
 
 
 def test_scratch_of_the_table_gradient_is_bounded():
