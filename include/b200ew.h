@@ -262,11 +262,13 @@ b200_status b200_lut_fprop(uint64_t ids, const b200_matrix *table, const b200_ma
 /* its gradient, replacing compound_bprop_lut (neon/backends/nervanagpu.py): dtable[v] = beta *
  * dtable[v] + alpha * (sum of error[:, n] over the positions n that hold v), for every row of
  * dtable; word pad_idx (-1: none) and numbers outside the table collect nothing.  The same bits in
- * every run. */
+ * every run.  error_t (may be null) is a (positions, features) buffer that receives the error
+ * transposed when its features are not neighbours; without it the strided error is read. */
 uint64_t    b200_lut_bprop_scratch_bytes(int64_t words, int64_t features, int64_t positions);
-b200_status b200_lut_bprop(uint64_t ids, const b200_matrix *error, const b200_matrix *dtable, int64_t words,
-                           int64_t features, int64_t positions, int64_t pad_idx, float alpha, float beta,
-                           uint64_t scratch, uint64_t scratch_bytes, uint64_t stream, int32_t *launches);
+b200_status b200_lut_bprop(uint64_t ids, const b200_matrix *error, const b200_matrix *error_t,
+                           const b200_matrix *dtable, int64_t words, int64_t features, int64_t positions,
+                           int64_t pad_idx, float alpha, float beta, uint64_t scratch, uint64_t scratch_bytes,
+                           uint64_t stream, int32_t *launches);
 
 /* distillation from a teacher's `top` largest logits (any float type) at the words top_ids (int32),
  * both (top, items): cost[n] = weights[n] T^2 KL(softmax(top_logits / T) || softmax(logits / T)), and

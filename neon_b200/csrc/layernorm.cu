@@ -731,7 +731,7 @@ template <int DT, int V, bool HELD> DEV void put_delta(const LnP& p, const Place
 // A block works through stripes gridDim.x apart; part[block][0][F]: its share of grad_gamma,
 // part[block][1][F]: of grad_beta, gathered in shared memory if `acc_held`.
 template <int DT, int V, bool HELD>
-__global__ void __launch_bounds__(kColsT) ln_bprop_cols(const __grid_constant__ LnP p, float* part, int lanes, i64 stripes, int acc_held) {
+__global__ void __launch_bounds__(kColsT, 2) ln_bprop_cols(const __grid_constant__ LnP p, float* part, int lanes, i64 stripes, int acc_held) {
     extern __shared__ __align__(16) u32 mem[];         // x, the error, the block's share of the gradients
     __shared__ __align__(16) float s[kStripeFloats];
     constexpr int P = Items<DT, V>::P;

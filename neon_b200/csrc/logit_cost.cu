@@ -885,7 +885,7 @@ extern "C" b200_status b200_distill(const b200_matrix* logits, const b200_matrix
     if (!logits || !top_ids || !top_logits) return refuse(where, "null matrix");
     const b200_matrix none = vec(0, logits->dtype), *d = delta ? delta : &none;
     const b200_matrix in[1] = {vec(weights, B200_F32)}, out[1] = {vec(cost, B200_F32)};
-    if (!(temperature > 0.f) || !std::isfinite(temperature) || !std::isfinite(1.f / temperature))
+    if (!(temperature > 0.f) || !std::isfinite(temperature) || !std::isfinite(1.5f / temperature))
         return refuse(where, "the temperature must be positive and finite");
     if (top < 1 || top > kMaxTop) return refuse(where, "between 1 and 1024 entries per item");
     if (int32_t st = check(where, logits, d, words, items, in, 1, out, 1)) return st;

@@ -564,9 +564,9 @@ extern "C" uint64_t b200_lut_bprop_scratch_bytes(int64_t words, int64_t features
     return (uint64_t)plan(words, features, positions).bytes;
 }
 
-extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, const b200_matrix* dtable, int64_t words,
-                                      int64_t features, int64_t positions, int64_t pad_idx, float alpha, float beta,
-                                      uint64_t scratch, uint64_t scratch_bytes, uint64_t stream, int32_t* launches) {
+extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, const b200_matrix* error_t,
+                                      const b200_matrix* dtable, int64_t words, int64_t features, int64_t positions, int64_t pad_idx,
+                                      float alpha, float beta, uint64_t scratch, uint64_t scratch_bytes, uint64_t stream, int32_t* launches) {
     const char* where = "b200_lut_bprop";
     if (launches) *launches = 0;
     if (!error || !dtable) return refuse(where, "null matrix");
@@ -578,6 +578,15 @@ extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, co
     if (positions && (meet(*dtable, words, features, *error, features, positions) ||
                       meet(*dtable, words, features, vec(ids, B200_I32), positions, 1)))
         return refuse(where, "the gradient shares memory with the error or the word numbers");
+    if (error_t) {
+        const b200_matrix words_given = vec(ids, B200_I32);
+        if (error_t->dtype != error->dtype) return refuse(where, "the error and its transposed buffer must have one type", B200_ERR_UNSUPPORTED);
+        if (positions && !error_t->ptr) return refuse(where, "null device pointer");
+        if (!aligned(error_t->ptr, error_t->dtype)) return refuse(where, "misaligned pointer");
+        if (meet(*error_t, positions, features, *error, features, positions) || meet(*error_t, positions, features, *dtable, words, features) ||
+            meet(*error_t, positions, features, words_given, positions, 1))
+            return refuse(where, "the buffer for the transposed error must lie apart from the other arguments");
+    }
     const Plan q = plan(words, features, positions);
     if (!scratch || scratch % 256 || scratch_bytes < (uint64_t)q.bytes) return refuse(where, "scratch too small or misaligned");
     DeviceScope scope;
@@ -586,6 +595,14 @@ extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, co
     char* base = reinterpret_cast<char*>(scratch);
     auto ints = [base](i64 off) { return reinterpret_cast<int*>(base + off); };
     int count = 0, from = 0;
+    b200_matrix turned = *error;
+    if (error_t && error->s0 != 1 && features > 1 && positions > 1) {
+        const int64_t shape[2] = {positions, features}, to[2] = {error_t->s0, error_t->s1}, as[2] = {error->s1, error->s0};
+        if (b200_status st = b200_dimshuffle(error_t->ptr, error->ptr, (int32_t)esize(error->dtype), 2, shape, to, as, stream)) return st;
+        turned.ptr = error_t->ptr; turned.s0 = error_t->s1; turned.s1 = error_t->s0;
+        ++count;
+    }
+    error = &turned;
     SortP t;
     t.ids = reinterpret_cast<const int*>(ids); t.hist = ints(q.hist);
     t.N = (int)positions; t.V = (int)words; t.tiles = (int)q.tiles;

@@ -84,16 +84,6 @@ class LanguageModelOps(object):
             raise NotImplementedError("%s: stochastic rounding of this operator's result" % name)
         raise ValueError("%s repeats its elements and cannot be written" % name)
 
-    @staticmethod
-    def _lm_span(t):
-        """First byte and one past the last byte that a tensor reaches."""
-        if not t.size:
-            return 0, 0
-        reach = [(d - 1) * s for d, s in zip(t.shape, t.strides)]
-        size = t.dtype.itemsize
-        return (t.gpudata + size * sum(r for r in reach if r < 0),
-                t.gpudata + size * (1 + sum(r for r in reach if r > 0)))
-
     def _lm_params(self, first, second, names):
         """Common type code of two optional parameter vectors."""
         code = None
@@ -133,7 +123,7 @@ class LanguageModelOps(object):
         """
         mx = self._lm_matrix(x, "x")
         my = self._lm_matrix(y, "y", x.shape, out=True)
-        if x.dtype != y.dtype:
+        if mx.dtype != my.dtype:
             raise TypeError("x and y must have one type")
         f, n = x.shape
         pdt = self._lm_params(gamma, beta, ("gamma", "beta"))
@@ -160,7 +150,7 @@ class LanguageModelOps(object):
         mx = self._lm_matrix(x, "x")
         me = self._lm_matrix(delta_in, "delta_in", x.shape)
         md = self._lm_matrix(delta_out, "delta_out", x.shape, out=True)
-        if x.dtype != delta_in.dtype or x.dtype != delta_out.dtype:
+        if mx.dtype != me.dtype or mx.dtype != md.dtype:
             raise TypeError("x, delta_in and delta_out must have one type")
         if mean is None or rstd is None:
             raise ValueError("the backward pass needs the forward pass's mean and rstd")
@@ -196,7 +186,7 @@ class LanguageModelOps(object):
         mo = self._lm_matrix(outputs, "outputs", out=True)
         if outputs.shape[0] != W.shape[1]:
             raise ValueError("outputs has shape %s, expected (%d, positions)" % (outputs.shape, W.shape[1]))
-        if W.dtype != outputs.dtype:
+        if mw.dtype != mo.dtype:
             raise TypeError("W and outputs must have one type")
         n = outputs.shape[1]
         ids = self._lm_words(inputs, "inputs", n)
@@ -239,24 +229,16 @@ class LanguageModelOps(object):
             raise ValueError("dW has shape %s, expected (vocabulary, %d)" % (dW.shape, error.shape[0]))
         f, n = error.shape
         ids = self._lm_words(inputs, "inputs", n)
+        mt = None
         if error_t is not None:
-            self._lm_matrix(error_t, "error_t", (n, f), out=True)
-            if error_t.dtype != error.dtype:
+            mt = self._lm_matrix(error_t, "error_t", (n, f), out=True)
+            if mt.dtype != me.dtype:
                 raise TypeError("error and error_t must have one type")
-            for t, name in ((error, "error"), (dW, "dW"), (inputs, "inputs")):
-                lo, hi = self._lm_span(t)
-                first, last = self._lm_span(error_t)
-                if lo < last and first < hi:
-                    raise ValueError("error_t must lie apart from %s" % name)
         self._lm_check(inputs, error, error_t, dW)
-        pad = -1 if pad_idx is None else int(pad_idx)
-        nbytes = rt.lut_bprop_scratch_bytes(dW.shape[0], f, max(n, 1))
-        scratch = self._lm_scratch(nbytes)
-        if error_t is not None and n > 1 and f > 1 and error.strides[0] != 1:
-            self.copy_transpose(error, error_t)
-            me = rt.Matrix(error_t.gpudata, error_t.strides[1], error_t.strides[0], me.dtype, 0)
-        self.launches += rt.lut_bprop(ids, me, mw, dW.shape[0], f, n, pad, float(alpha), float(beta), scratch, nbytes,
-                                      self.stream)
+        v = dW.shape[0]
+        nbytes = rt.lut_bprop_scratch_bytes(v, f, n or 1)
+        self.launches += rt.lut_bprop(ids, me, mt, mw, v, f, n, -1 if pad_idx is None else int(pad_idx), float(alpha),
+                                      float(beta), self._lm_scratch(nbytes), nbytes, self.stream)
         return dW
 
     # ------------------------------------------------------------------ costs on logits
@@ -303,7 +285,7 @@ class LanguageModelOps(object):
         if delta is None:
             return _NONE
         md = self._lm_matrix(delta, "delta", logits.shape, out=True)
-        if delta.dtype != logits.dtype:
+        if md.dtype != logits._lm[1]:
             raise TypeError("logits and delta must have one type")
         return md
 

@@ -93,7 +93,7 @@ SIGNATURES = {
                             u64, u64, u64, P(i32)]),
     "b200_lut_fprop": (i32, [u64, P(Matrix), P(Matrix), C.c_int64, C.c_int64, C.c_int64, C.c_float, u64]),
     "b200_lut_bprop_scratch_bytes": (u64, [C.c_int64, C.c_int64, C.c_int64]),
-    "b200_lut_bprop": (i32, [u64, P(Matrix), P(Matrix), C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_float,
+    "b200_lut_bprop": (i32, [u64, P(Matrix), P(Matrix), P(Matrix), C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_float,
                              C.c_float, u64, u64, u64, P(i32)]),
     "b200_cost_scratch_bytes": (u64, [C.c_int64, C.c_int64, C.c_int64]),
     "b200_distill": (i32, [P(Matrix), P(Matrix), P(Matrix), P(Matrix), u64, u64, C.c_int64, C.c_int64, C.c_int64,
@@ -423,9 +423,10 @@ def lut_bprop_scratch_bytes(words, features, positions):
     return int(lib().b200_lut_bprop_scratch_bytes(words, features, positions))
 
 
-def lut_bprop(ids, error, dtable, words, features, positions, pad_idx, alpha, beta, scratch, scratch_bytes, stream=0):
+def lut_bprop(ids, error, error_t, dtable, words, features, positions, pad_idx, alpha, beta, scratch, scratch_bytes,
+              stream=0):
     n = i32(0)
-    check(lib().b200_lut_bprop(ids, error, dtable, words, features, positions, pad_idx, alpha, beta, scratch,
+    check(lib().b200_lut_bprop(ids, error, error_t, dtable, words, features, positions, pad_idx, alpha, beta, scratch,
                                scratch_bytes, stream, n))
     return n.value
 

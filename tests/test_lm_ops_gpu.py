@@ -205,7 +205,7 @@ def words(rng, v, n):
 
 
 LUT_SIZES = [(1, 1, 1), (5, 3, 40), (100, 64, 1), (300, 33, 500), (1000, 128, 4096), (511, 40, 5000), (512, 16, 9000),
-             (50000, 8, 300), (20, 1000, 70), (3, 256, 20000)]
+             (50000, 8, 300), (20, 1000, 70), (3, 256, 20000), (300000, 5, 9000)]
 
 
 @pytest.mark.parametrize("v,f,n", LUT_SIZES)
@@ -563,3 +563,135 @@ def test_operators_recorded_and_replayed(b200):
     for m, w in zip(models, want):
         for k in w:
             assert np.array_equal(m.d[k].get(), w[k]), k
+
+
+# ---------------------------------------------------------------- other things a caller may do
+def test_offsets_beyond_32_bits(b200):
+    """Matrices of more than 2^31 elements: their last items have the values that the same items
+    have in a small matrix, and so has the element behind them."""
+    be = b200
+    f, n, tail = 16384, 135000, 3
+    assert f * n > 2 ** 31
+    x, gamma, beta, e = ln_inputs(f, tail, bf16, np.float32)
+    big, err = be.empty((n, f), dtype=bf16), be.empty((n, f), dtype=bf16)
+    big[:] = 0.5
+    err[:] = 0.25
+    big[n - tail:] = np.ascontiguousarray(x.T)
+    err[n - tail:] = np.ascontiguousarray(e.T)
+    mean, rstd, g, b = be.empty((1, n)), be.empty((1, n)), vector(be, gamma), vector(be, beta)
+    out = be.empty((n, f), dtype=bf16)
+    be.compound_fprop_ln(big.T, mean, rstd, g, b, out.T)
+    got = {"y": out[n - tail:].get().T, "mean": mean.get()[:, -tail:], "rstd": rstd.get()[:, -tail:]}
+    compare(got, ref.ln_fprop(x, gamma, beta, 1e-5, bf16))
+    gg, gb = be.empty((f, 1)), be.empty((f, 1))
+    be.compound_bprop_ln(out.T, gg, gb, err.T, big.T, mean, rstd, g)
+    want = ref.ln_bprop(e, x, got["mean"], got["rstd"], gamma, bf16, np.float32)
+    ref.check("delta", out[n - tail:].get().T, want["delta"])
+    total = 0.25 * (n - tail) + want["grad_beta"][0]
+    ref.check("grad_beta", gb.get(), (total, ref.depth(n) * ref.U * (0.25 * n + np.abs(e.astype(np.float64)).sum(1, keepdims=True))))
+
+    ids = np.zeros(n, np.int32)
+    ids[-tail:] = [1, 2, 0]
+    w = np.random.RandomState(0).standard_normal((3, f)).astype(bf16)
+    dev = be.array(ids.reshape(1, n), dtype=np.int32)
+    be.compound_fprop_lut(dev, be.array(w, dtype=bf16), out.T, scale=0.5)
+    ref.check("out", out[n - tail:].get().T, ref.lut_fprop(ids[-tail:], w, 0.5, bf16)["out"])
+    dw = be.empty((3, f))
+    be.compound_bprop_lut(1, dev, err.T, None, dw, pad_idx=0)
+    ref.check("dW", dw.get()[1:], tuple(a[1:] for a in ref.lut_bprop(ids[-tail:], e, dw.get(), 0, 1.0, 0.0, np.float32)["dW"]))
+
+    z, act, old, new_ref, adv, weights = policy_inputs(f, tail, bf16)
+    big[n - tail:] = np.ascontiguousarray(z.T)
+    row = lambda a: np.concatenate([np.zeros((1, n - tail)), a], axis=1)                        # noqa: E731
+    cost, logp = be.empty((1, n)), be.empty((1, n))
+    be.compound_policy(big.T, be.array(row(act), dtype=np.int32), vector(be, row(old)), vector(be, row(adv)), cost, out.T,
+                       logp=logp, ref_logp=vector(be, row(new_ref)), clip=(0.2, 0.28), kl_coef=0.05)
+    got = {"cost": cost.get()[:, -tail:], "logp": logp.get()[:, -tail:], "delta": out[n - tail:].get().T}
+    compare(got, ref.policy(z, act, old, new_ref, adv, None, 0.2, 0.28, 0.05, bf16))
+    z, tids, top, w = distill_inputs(f, tail, 3, bf16)
+    big[n - tail:] = np.ascontiguousarray(z.T)
+    w = row(w)
+    w[0, :4] = 0
+    many = lambda a: np.concatenate([np.zeros((3, n - tail), a.dtype), a], axis=1)              # noqa: E731
+    be.compound_distill(big.T, be.array(many(tids), dtype=np.int32), be.array(many(top), dtype=bf16), cost, big.T,
+                        vector(be, w), 2.0)
+    compare({"cost": cost.get()[:, -tail:], "delta": big[n - tail:].get().T}, ref.distill(z, tids, top, w[:, -tail:], 2.0, bf16))
+    assert (big[0:4].get().astype(np.float32) == 0).all()
+
+
+def test_calls_queued_one_behind_the_other(b200):
+    """Calls that reuse the backend's scratch, without waiting between them, and op-tree statements."""
+    be = b200
+    rng = np.random.RandomState(2)
+    v, f, n = 900, 96, 3000
+    want, held = [], []
+    for k in range(6):
+        ids = words(rng, v, n)
+        e = rng.standard_normal((f, n)).astype(np.float32)
+        dw, total = be.empty((v, f)), be.empty((1, 1))
+        dev, err = be.array(ids.reshape(1, n), dtype=np.int32), be.array(e)
+        held.append((dw, total, dev, err, be.empty((n, f))))
+        want.append((ref.lut_bprop(ids, e, np.zeros((v, f)), None, 1.0, 0.0, np.float32)["dW"], e))
+    x, gamma, beta, e2 = ln_inputs(700, 40, np.float32, np.float32)
+    hx, hy = Held(be, x, np.float32, "cols"), Held(be, nan_like(x.shape), np.float32, "cols")
+    g, b = vector(be, gamma), vector(be, beta)
+    for dw, total, dev, err, error_t in held:
+        be.compound_bprop_lut(1, dev, err, error_t, dw)
+        total[:] = be.sum(dw)
+        be.compound_fprop_ln(hx.view, None, None, g, b, hy.view)
+    for (dw, total, dev, err, error_t), (value, e) in zip(held, want):
+        ref.check("dW", dw.get(), value)
+        assert abs(float(total.get()[0, 0]) - e.astype(np.float64).sum()) < 1e-5 * np.abs(e).sum()
+    ref.check("y", hy.get(), ref.ln_fprop(x, gamma, beta, 1e-5, np.float32)["y"])
+
+
+def test_checked_mode(b200):
+    be = b200
+    x, gamma, beta, e = ln_inputs(40, 6, np.float32, np.float32)
+    be.check_bounds = True
+    try:
+        got = run_ln(be, x, gamma, beta, e, np.float32, np.float32, "pitched")
+        compare(got, want_ln(x, gamma, beta, e, got, np.float32, np.float32))
+    finally:
+        be.check_bounds = False
+
+
+@pytest.mark.parametrize("f,n", [(2048, 5000), (1001, 3000), (96, 20000), (300, 12000), (5000, 700)])
+@pytest.mark.parametrize("order", ["rows", "cols"])
+def test_layer_norm_many_items(b200, f, n, order):
+    """More items than are under way at once: every block and group takes several."""
+    x, gamma, beta, e = ln_inputs(f, n, bf16, np.float32)
+    got = run_ln(b200, x, gamma, beta, e, bf16, np.float32, order)
+    compare(got, want_ln(x, gamma, beta, e, got, bf16, np.float32))
+
+
+@pytest.mark.parametrize("v,n", [(700, 6000), (3001, 3000), (20000, 900), (60000, 350)])
+def test_costs_many_items(b200, v, n):
+    """Several rows per block, masked ones among them, and a check of whole items by their sums: the
+    gradient of an item adds up to zero."""
+    be = b200
+    rng = np.random.RandomState(v)
+    z = (rng.standard_normal((n, v)) * 2).astype(np.float32)
+    ids = np.sort(rng.randint(0, v, (n, 5)), axis=1).astype(np.int32)
+    top = rng.standard_normal((n, 5)).astype(np.float32)
+    w = (rng.rand(1, n) < 0.7).astype(np.float32)
+    act = rng.randint(-1, v, (1, n)).astype(np.int32)
+    z[w[0] == 0, 3] = np.nan
+    cost, delta = be.array(nan_like((1, n))), be.array(nan_like((n, v)))
+    zt, wt = be.array(z), be.array(w)
+    be.compound_distill(zt.T, be.array(ids, dtype=np.int32).T, be.array(top).T, cost, delta.T, wt, 2.0)
+    some = rng.permutation(n)[:40]
+    want = ref.distill(z[some].T, ids[some].T, top[some].T, w[:, some], 2.0, np.float32)
+    got, got_cost = delta.get(), cost.get()
+    compare({"cost": got_cost[:, some], "delta": got[some].T}, want)
+    assert (got[w[0] == 0] == 0).all() and (got_cost[w == 0] == 0).all()
+    # a sum of v roundings of values of at most 2 w, half of which is the teacher's
+    assert np.abs(got.sum(axis=1, dtype=np.float64)).max() < 4 * (ref.depth(v) + 64) * ref.U + 64 * ref.EXP
+    old, adv = rng.standard_normal((1, n)).astype(np.float32) - 8, rng.standard_normal((1, n)).astype(np.float32)
+    be.compound_policy(zt.T, be.array(act, dtype=np.int32), be.array(old), be.array(adv), cost, delta.T, weights=wt)
+    got, got_cost = delta.get(), cost.get()
+    none = (w[0] == 0) | (act[0] < 0)
+    assert (got[none] == 0).all() and (got_cost[0, none] == 0).all()
+    live = [i for i in some if not none[i]]
+    want = ref.policy(z[live].T, act[:, live], old[:, live], None, adv[:, live], w[:, live], 0.2, 0.2, 0.0, np.float32)
+    compare({"cost": got_cost[:, live], "delta": got[live].T}, want)
