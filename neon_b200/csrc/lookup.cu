@@ -16,6 +16,8 @@
 
 #include "nn_common.cuh"
 
+#include <algorithm>
+
 using namespace nn;
 
 namespace {
@@ -310,6 +312,7 @@ struct SumP {
     i64 F, L;                             // L sorted places per chunk
     float* part;                          // [chunk][2][F]: 0 continues an earlier chunk, 1 begins here and goes on
     float alpha, beta;
+    int parts;                            // pieces that rows are cleared in
 };
 
 template <int V> DEV void put_dw(const SumP& p, i64 v, int f, const float* sum) {
@@ -333,27 +336,46 @@ template <int V> DEV void put_dw(const SumP& p, i64 v, int f, const float* sum) 
     for (int i = 0; i < V; ++i) if (f + i < p.F) st_any(p.w, at + i * p.w1, p.wdt, r[i]);
 }
 
+// Clears (or scales) the rows of words that have no position: a warp takes 32 words and a part of
+// their features at a time.  Rows that start off a 16-byte boundary are cleared in whole vectors too.
+template <int DT> DEV void clear_part(u64 base, i64 row, int from, int to) {
+    constexpr int V = 16 / dt_size<DT>::value;
+    const u32 none[4] = {0, 0, 0, 0};
+    const int mis = (int)((base / dt_size<DT>::value + (u64)(row + from)) % V), many = to - from;
+    for (int f = (int)(threadIdx.x & 31) * V - mis; f < many; f += 32 * V) put_part<DT, V>(base, row + from, f, many, none);
+}
+DEV void fill_words(const SumP& p, i64 warp, i64 warps) {
+    const int lane = threadIdx.x & 31, F = (int)p.F, per = (F + p.parts - 1) / p.parts;
+    const i64 groups = ((i64)p.V + 31) / 32;
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (i64 task = warp; task < groups * p.parts; task += warps) {
+        const i64 v0 = task / p.parts * 32;
+        const int from = (int)(task % p.parts) * per, to = min(from + per, F);
+        unsigned none = __ballot_sync(0xffffffffu, v0 + lane < p.V && p.start[v0 + lane] == p.start[v0 + lane + 1]);
+        while (none) {
+            const i64 v = v0 + __ffs(none) - 1;
+            none &= none - 1;
+            if (p.beta == 0.f && p.w1 == 1) {
+                if (p.wdt == F32) clear_part<F32>(p.w, v * p.w0, from, to);
+                else clear_part<F16>(p.w, v * p.w0, from, to);          // 16 bits of zero, of either type
+            } else {
+                for (int f = from + lane; f < to; f += 32) put_dw<1>(p, v, f, zero);
+            }
+        }
+    }
+}
+
 // The first `sum_blocks` blocks: a thread adds up V features of the places of one chunk, in their
 // order; neighbouring threads take neighbouring features.  Eight places are under way at a time, and
 // the numbers of the next eight are read meanwhile.  V > 1: the error's features are next to each
 // other; `aligned`: its positions start on 16-byte boundaries.
-// The other blocks: a warp looks at 32 words and clears (or scales) those that have no position.
+// The other blocks see to the words without a position.
 template <int DT, int V>
 __global__ void __launch_bounds__(256) lut_chunks(const __grid_constant__ SumP p, i64 chunks, int nvec, int aligned, unsigned sum_blocks) {
     grid_enter();
     const int F = (int)p.F;
     if (blockIdx.x >= sum_blocks) {
-        const int lane = threadIdx.x & 31;
-        const i64 step = (i64)(gridDim.x - sum_blocks) * 8 * 32;
-        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        for (i64 v0 = ((i64)(blockIdx.x - sum_blocks) * 8 + (threadIdx.x >> 5)) * 32; v0 < p.V; v0 += step) {
-            unsigned none = __ballot_sync(0xffffffffu, v0 + lane < p.V && p.start[v0 + lane] == p.start[v0 + lane + 1]);
-            while (none) {
-                const i64 v = v0 + __ffs(none) - 1;
-                none &= none - 1;
-                for (int f = lane * 4; f < F; f += 128) put_dw<4>(p, v, f, zero);
-            }
-        }
+        fill_words(p, (i64)(blockIdx.x - sum_blocks) * 8 + (threadIdx.x >> 5), (i64)(gridDim.x - sum_blocks) * 8);
         return;
     }
     constexpr int U = 8, W = V == 1 ? 1 : 4;
@@ -483,9 +505,12 @@ __global__ void __launch_bounds__(256) lut_cross(const __grid_constant__ SumP p,
     }
 }
 
-template <int DT, int V> cudaError_t launch_chunks(const SumP& p, i64 chunks, bool aligned, cudaStream_t s) {
+template <int DT, int V> cudaError_t launch_chunks(SumP p, i64 chunks, bool aligned, cudaStream_t s) {
     const i64 nvec = (p.F + V - 1) / V, sums = (chunks * nvec + 255) / 256;
-    i64 fill = p.beta == 1.f ? 0 : ((i64)p.V + 255) / 256;
+    // rows of few words are cut, down to 512 features, so that there is a warp for every 16 SM slots
+    const i64 groups = ((i64)p.V + 31) / 32;
+    p.parts = (int)std::min<i64>((148 * 32 + groups - 1) / groups, (p.F + 511) / 512);
+    i64 fill = p.beta == 1.f ? 0 : (groups * p.parts + 7) / 8;
     if (fill > 148 * 16) fill = 148 * 16;
     if (!(sums + fill)) return cudaSuccess;
     return launch_dependent(lut_chunks<DT, V>, dim3((unsigned)(sums + fill)), 256, 0, s, p, chunks, (int)nvec, (int)aligned, (unsigned)sums);
@@ -629,7 +654,7 @@ extern "C" b200_status b200_lut_bprop(uint64_t ids, const b200_matrix* error, co
     p.e = error->ptr; p.e0 = error->s0; p.e1 = error->s1; p.edt = error->dtype;
     p.w = dtable->ptr; p.w0 = dtable->s0; p.w1 = dtable->s1; p.wdt = dtable->dtype;
     p.V = (int)words; p.L = q.L; p.F = features; p.part = reinterpret_cast<float*>(base + q.part);
-    p.alpha = alpha; p.beta = beta;
+    p.alpha = alpha; p.beta = beta; p.parts = 1;
     p.wide = features % 8 == 0 && dtable->s1 == 1 && dtable->ptr % 16 == 0 && dtable->s0 % 8 == 0;
     if (e == cudaSuccess)
         e = launch_dependent(sort_starts, dim3((unsigned)((words + 256) / 256)), 256, 0, s, p.key, (int)positions, ints(q.start), (int)words);
