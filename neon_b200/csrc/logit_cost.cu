@@ -245,10 +245,11 @@ __global__ void __launch_bounds__(256) cost_any(const __grid_constant__ CostP p)
 // vectors start at the 128-byte boundary at or before the row, `mis` words early, so that a warp's
 // accesses are whole lines whatever the row's length; those without a word of the row are left out.
 //
-// What bounds it: the second read.  At 50257 x 2048 bf16 it takes 95 us where one read and one write
-// of HBM need 64; without any arithmetic it still takes 85, without the gradient 46.  Rows kept in
-// shared memory from one walk to the other (in clusters where they are wide) were measured too, and
-// slower (98 and 681 us at 131072 x 4096, against 95 and 440): too few rows are under way then.
+// What bounds it: instructions, and the second read.  At 50257 x 2048 bf16 one read and one write of
+// HBM take 64 us, this takes 82, of which the first walk, the costs without a gradient, 43.  The loops
+// are written for few instructions: constant distances (T is a constant), no checks but in the steps
+// that hold an end of the row.  Rows kept in shared memory from one walk to the other (in clusters
+// where they are wide) were measured too and are slower, 98 us here: too few rows are under way.
 DEV u32 max_pair(u32 a, u32 b, int dt) {              // NaN is passed over
     u32 r;
     if (dt == F16) asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -317,19 +318,25 @@ template <int DT> DEV void mask_end(u32* w, int f, int words) {
     }
 }
 
-template <bool POLICY, int DT, int RING, int MAXT, int MINB>
-__global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ CostP p) {
-    constexpr int SZ = dt_size<DT>::value, V = 16 / SZ, LV = SZ == 4 ? 2 : 3, U = 4;
+// One of a step's copies, OFF bytes from the first: constant distances keep the address arithmetic,
+// which counts here, out of the loops.
+template <int OFF> DEV void copy16_at(u32 to, u64 from) {
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %2], 16;" :: "r"(to), "l"(from), "n"(OFF) : "memory");
+}
+
+template <bool POLICY, int DT, int RING, int T, int MINB>
+__global__ void __launch_bounds__(T, MINB) cost_rows(const __grid_constant__ CostP p) {
+    constexpr int SZ = dt_size<DT>::value, V = 16 / SZ, LV = SZ == 4 ? 2 : 3, U = 4, STEP = U * T, JUMP = T * 16;
+    constexpr int WARPS = T / 32;
     // [RING][U][T] vectors, then the entries [2][3][K4].  These, and what is [2] below, alternate from
     // item to item; the barriers of the item in between keep two uses of one half apart.
     extern __shared__ __align__(16) u32 mem[];
     __shared__ float2 red[2][32];
     __shared__ Item shared_item[2];
     __shared__ float shared_word[2];
-    const int tid = threadIdx.x, T = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = T >> 5;
-    const int jump = T * 16;                           // bytes from one of a thread's vectors to the next
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int K4 = (p.K + 3) / 4 * 4, walks = p.d ? 2 : 1;
-    float* entries = reinterpret_cast<float*>(mem + RING * U * T * 4);
+    float* entries = reinterpret_cast<float*>(mem + RING * STEP * 4);
     char* mine = reinterpret_cast<char*>(mem) + tid * 16;
     const u32 mine32 = (u32)__cvta_generic_to_shared(mine);
     auto mis_of = [&](i64 n) { return (int)(p.z / SZ + (u64)(n * p.z1)) & (128 / SZ - 1); };
@@ -337,11 +344,13 @@ __global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ 
     auto weight_at = [&](i64 n) { return n < p.N ? weight_of(p, n) : 0.f; };
     auto action_at = [&](i64 n) { return POLICY && n < p.N ? reinterpret_cast<const int*>(p.actions)[n] : 0; };
 
-    // ---- what the copies are at: row, walk, first vector of the step
+    // ---- what the copies are at: row, walk, first vector of the step, this thread's address in it
     i64 fn = blockIdx.x;
-    int fwalk = 0, fk = 0, ffirst = 0, fnvec = 0, fslot = 0, fa = action_at(fn);
+    int fwalk = 0, fk = 0, ffirst = 0, fnvec = 0, fa = action_at(fn);
     float fw = weight_at(fn);
-    u64 frow = 0;
+    u64 frow = 0, from = 0;
+    u32 fto = mine32;
+    bool live = false;
     auto enter = [&]() {                               // row fn or the first after it that is not skipped
         for (;;) {
             const bool skip = skipped<POLICY>(p, fw, fa);
@@ -350,27 +359,37 @@ __global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ 
             if (fn >= p.N || !skip) break;
             fn += gridDim.x;
         }
+        live = fn < p.N;
         const int mis = mis_of(fn);
         ffirst = mis >> LV;
         fnvec = (p.V + mis + V - 1) >> LV;
-        frow = p.z + (u64)((fn * p.z1 - mis) * SZ) + (u64)tid * 16;
+        from = frow = p.z + (u64)((fn * p.z1 - mis) * SZ) + (u64)tid * 16;
         fwalk = fk = 0;
     };
     enter();
     auto fetch = [&]() {
-        if (fn < p.N) {
-            const u32 to = mine32 + fslot * U * jump;
-            const u64 from = frow + (u64)fk * 16;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (fk + u * T + tid >= ffirst && fk + u * T + tid < fnvec) copy16(to + u * jump, from + (u32)(u * jump));
-            fk += U * T;
+        if (live) {
+            if (fk + STEP <= fnvec && fk >= ffirst) {
+                copy16_at<0>(fto, from);
+                copy16_at<JUMP>(fto, from);
+                copy16_at<2 * JUMP>(fto, from);
+                copy16_at<3 * JUMP>(fto, from);
+            } else {
+                const int k = fk + tid;
+                if (k >= ffirst && k < fnvec) copy16_at<0>(fto, from);
+                if (k + T < fnvec) copy16_at<JUMP>(fto, from);
+                if (k + 2 * T < fnvec) copy16_at<2 * JUMP>(fto, from);
+                if (k + 3 * T < fnvec) copy16_at<3 * JUMP>(fto, from);
+            }
+            fk += STEP;
+            from += U * JUMP;
             if (fk >= fnvec) {
                 fk = 0;
+                from = frow;
                 if (++fwalk == walks) { fn += gridDim.x; enter(); }
             }
         }
-        fslot = fslot == RING - 1 ? 0 : fslot + 1;
+        fto = fto == mine32 + (RING - 1) * U * JUMP ? mine32 : fto + U * JUMP;
         copy_commit();
     };
 #pragma unroll
@@ -385,7 +404,15 @@ __global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ 
         next_t = entry_top(p, blockIdx.x, tid);
         if (next_id >= 0 && next_id < p.V) next_z = ld_any(p.z, blockIdx.x * p.z1 + next_id, DT);
     }
-    int turn = 0, slot = 0;
+    int turn = 0;
+    const char* at = mine;                             // the step that is read next
+    auto arrive = [&]() {
+        fetch();
+        copy_wait<RING - 1>();
+        const char* here = at;
+        at = at == mine + (RING - 1) * U * JUMP ? mine : at + U * JUMP;
+        return here;
+    };
     for (i64 n = blockIdx.x; n < p.N; n += gridDim.x) {
         const float w_item = next_w;
         const int a_item = next_a, id_item = next_id;
@@ -399,7 +426,7 @@ __global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ 
         }
         const bool skip = skipped<POLICY>(p, w_item, a_item);
         Item it = {0.f, 0.f, 1};
-        const int mis = mis_of(n), kfirst = mis >> LV, nvec = (p.V + mis + V - 1) >> LV;
+        const int mis = mis_of(n), kfirst = mis >> LV, nvec = (p.V + mis + V - 1) >> LV, whole = (p.V + mis) >> LV;
         const i64 drow = n * p.d1;
         float at_word = 0.f;
         Entries e;
@@ -413,7 +440,7 @@ __global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ 
             int used = 0;
             if (POLICY) {
                 if (warp == 0) chosen = read_chosen(p, n, a_item, w_item);
-            }            else if (ahead) {
+            } else if (ahead) {
                 if (tid < p.K) {
                     put_entry(p, e, tid, id_item, t_item, z_item);
                     used = entry_used(p, id_item, t_item);
@@ -423,39 +450,44 @@ __global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ 
                 used = read_entries(p, n, e);
             }
             Running r = {-INFINITY, 0, 0};
-            for (int k0 = 0; k0 < nvec; k0 += U * T) {
-                fetch();
-                copy_wait<RING - 1>();
-                const char* at = mine + slot * U * jump;
-                slot = slot == RING - 1 ? 0 : slot + 1;
-                const int k = k0 + tid;
-                u32 w[U][4];
+            for (int k0 = 0; k0 < nvec; k0 += STEP) {
+                const char* here = arrive();
+                // steps with a vector that is not all the row's go one by one, and stop behind the row
+                if (k0 + STEP <= whole && (k0 || warp || !mis)) {
+                    u32 w[U][4];
 #pragma unroll
-                for (int u = 0; u < U; ++u) ld_raw<16, false>(at + u * jump, w[u]);
-                if (k0 + U * T >= nvec || k <= kfirst) {        // the row's ends, and vectors around it
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int ku = k + u * T;
-                        if (ku <= kfirst || ku >= nvec - 1) mask_end<DT>(w[u], ku * V - mis, p.V);
+                    for (int u = 0; u < U; ++u) ld_raw<16, false>(here + u * JUMP, w[u]);
+                    take<DT, U>(r, w, p.c);
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u < U && k0 + u * T < nvec; ++u, here += JUMP) {
+                        const int k = k0 + u * T + tid;
+                        u32 w[1][4];
+                        ld_raw<16, false>(here, w[0]);
+                        if (k <= kfirst || k >= nvec - 1) mask_end<DT>(w[0], k * V - mis, p.V);
+                        take<DT, 1>(r, w, p.c);
                     }
                 }
-                take<DT, U>(r, w, p.c);
             }
             // one maximum and sum for the row
             float m = warp_max(r.m), s = warp_sum(both(add2(r.a, r.b)) * exp_of(r.m, usable(m), p.c));
-            if (lane == 0) red[turn][warp] = make_float2(m, s);
             int any = 0;
-            if (POLICY) __syncthreads();
-            else any = __syncthreads_or(used);
-            const float2 part = lane < warps ? red[turn][lane] : make_float2(-INFINITY, 0.f);
-            m = warp_max(part.x);
-            s = warp_sum(part.y * exp_of(part.x, usable(m), p.c));
+            if constexpr (WARPS > 1) {
+                if (lane == 0) red[turn][warp] = make_float2(m, s);
+                if (POLICY) __syncthreads();
+                else any = __syncthreads_or(used);
+                const float2 part = lane < WARPS ? red[turn][lane] : make_float2(-INFINITY, 0.f);
+                m = warp_max(part.x);
+                s = warp_sum(part.y * exp_of(part.x, usable(m), p.c));
+            } else {
+                any = __any_sync(0xffffffffu, used);
+            }
             if (POLICY) {
                 if (warp == 0) {
                     it = policy_item(p, n, m, s, chosen, tid == 0, at_word);
-                    if (lane == 0) { shared_item[turn] = it; shared_word[turn] = at_word; }
+                    if (WARPS > 1 && lane == 0) { shared_item[turn] = it; shared_word[turn] = at_word; }
                 }
-                if (p.d) {
+                if (WARPS > 1 && p.d) {
                     __syncthreads();
                     it = shared_item[turn];
                     at_word = shared_word[turn];
@@ -471,29 +503,29 @@ __global__ void __launch_bounds__(MAXT, MINB) cost_rows(const __grid_constant__ 
         if (mine_too && after < p.N) next_z = next_id >= 0 && next_id < p.V ? ld_any(p.z, after * p.z1 + next_id, DT) : 0.f;
         if (p.d) {
             char* to = reinterpret_cast<char*>(p.d) + (drow - mis) * SZ + tid * 16;
-            for (int k0 = 0; k0 < nvec; k0 += U * T, to += U * jump) {
-                const char* at = mine + slot * U * jump;
-                if (!skip) {
-                    fetch();
-                    copy_wait<RING - 1>();
-                    slot = slot == RING - 1 ? 0 : slot + 1;
-                }
-                const int k = k0 + tid;
-                const bool ends = k0 + U * T >= nvec || k <= kfirst;
-                u32 w[U][4];
+            for (int k0 = 0; k0 < nvec; k0 += STEP, to += U * JUMP) {
+                const char* here = skip ? mine : arrive();
+                if (k0 + STEP <= whole && (k0 || warp || !mis) && !it.dead) {
+                    u32 w[U][4];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (it.dead) w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;
-                    else {
-                        ld_raw<16, false>(at + u * jump, w[u]);
+                    for (int u = 0; u < U; ++u) ld_raw<16, false>(here + u * JUMP, w[u]);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
                         give<DT>(w[u], it, p.c);
+                        st_raw<16>(to + u * JUMP, w[u]);
                     }
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int ku = k + u * T;
-                    if (ends && (ku <= kfirst || ku >= nvec - 1)) put_part<DT, V>(p.d, drow, ku * V - mis, p.V, w[u]);
-                    else st_raw<16>(to + u * jump, w[u]);
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u < U && k0 + u * T < nvec; ++u, here += JUMP) {
+                        const int k = k0 + u * T + tid;
+                        u32 w[4] = {0, 0, 0, 0};
+                        if (!it.dead) {
+                            ld_raw<16, false>(here, w);
+                            give<DT>(w, it, p.c);
+                        }
+                        if (k <= kfirst || k >= nvec - 1) put_part<DT, V>(p.d, drow, k * V - mis, p.V, w);
+                        else st_raw<16>(to + u * JUMP, w);
+                    }
                 }
             }
             if (POLICY) {                              // by the thread that wrote the word's vector
@@ -804,26 +836,27 @@ template <bool POLICY> cudaError_t launch_any(const CostP& p, cudaStream_t s) {
 
 // How many threads a row gets, and with them how many rows are under way: small blocks keep more
 // rows of an SM at different points of their way, but a row stays in L2 between its two walks only
-// if the rows under way hold no more than some 60 MB.  Measured, us: 8192 words bf16 x 16384, 128
-// threads 130, 256 151; 50257 bf16 x 2048, 256 threads 95, 512 101; 32768 f32 x 4096 (128 KB), 256
-// threads 217, 512 189; 131072 bf16 x 4096, 512 threads 490, 1024 440.
-template <bool POLICY, int DT, int RING, int MAXT, int MINB> cudaError_t launch_rows_of(const CostP& p, cudaStream_t s) {
-    constexpr int V = 16 / dt_size<DT>::value, U = 4;
-    const bool even = p.z % 128 == 0 && p.z1 % (8 * V) == 0;        // every row starts on a boundary
-    const i64 nvec = ((i64)p.V + (even ? 0 : 8 * V - 1) + V - 1) / V, steps = (nvec + U * MAXT - 1) / (U * MAXT);
-    const int T = (int)((nvec + U * steps - 1) / (U * steps) + 31) / 32 * 32;
-    const int smem = RING * U * T * 16 + (POLICY ? 0 : 24 * ((p.K + 3) / 4 * 4));
-    const i64 most = resident_blocks(cost_rows<POLICY, DT, RING, MAXT, MINB>, T, smem);
+// if the rows under way do: the smallest block with which they hold no more than 50 MB, or any if
+// all logits together hold no more than 66.  Measured, us, blocks per SM in brackets: 32768 words
+// bf16 x 4096 (64 KB a row), 128 threads (8) 127, 256 (3) 99; 50257 bf16 x 2048, 256 (3) 82, 256 (4)
+// 89, 512 (2) 102; 32768 f32 x 4096, 256 (3) 228, 512 (2) 210; 131072 bf16 x 4096, 512 (2) 489, 1024
+// (1) 412; 32003 f16 x 1000, 128 (8) 30, 256 (4) 37.  Rows of up to 8 KB are a warp's: 4001 bf16 x
+// 16384, 32 threads 54, 128 85.
+template <bool POLICY, int DT, int RING, int T, int MINB> cudaError_t launch_rows_of(const CostP& p, cudaStream_t s) {
+    const int smem = RING * 4 * T * 16 + (POLICY ? 0 : 24 * ((p.K + 3) / 4 * 4));
+    const i64 most = resident_blocks(cost_rows<POLICY, DT, RING, T, MINB>, T, smem);
     if (!most) return cudaErrorInvalidConfiguration;
-    cost_rows<POLICY, DT, RING, MAXT, MINB><<<(unsigned)(p.N < most ? p.N : most), T, smem, s>>>(p);
+    cost_rows<POLICY, DT, RING, T, MINB><<<(unsigned)(p.N < most ? p.N : most), T, smem, s>>>(p);
     return cudaGetLastError();
 }
 template <bool POLICY, int DT> cudaError_t launch_rows(const CostP& p, cudaStream_t s) {
     const i64 bytes = (i64)p.V * dt_size<DT>::value;
-    if (bytes > 160 * 1024) return launch_rows_of<POLICY, DT, 3, 1024, 1>(p, s);
-    if (bytes > 110 * 1024) return launch_rows_of<POLICY, DT, 3, 512, 2>(p, s);
-    if (bytes > 32 * 1024) return launch_rows_of<POLICY, DT, 3, 256, 4>(p, s);
-    return launch_rows_of<POLICY, DT, 3, 128, 8>(p, s);
+    auto fits = [&](int per_sm) { return p.N * bytes <= 66 * 1000 * 1000 || 148 * per_sm * bytes <= 50 * 1000 * 1000; };
+    if (bytes <= 8 * 1024) return launch_rows_of<POLICY, DT, 3, 32, 24>(p, s);
+    if (fits(8)) return launch_rows_of<POLICY, DT, 2, 128, 8>(p, s);
+    if (fits(3)) return launch_rows_of<POLICY, DT, 3, 256, 3>(p, s);
+    if (fits(2)) return launch_rows_of<POLICY, DT, 3, 512, 2>(p, s);
+    return launch_rows_of<POLICY, DT, 3, 1024, 1>(p, s);
 }
 
 template <bool POLICY, int DT> cudaError_t launch_cols_width(const CostP& p, char* scratch, int& launches, cudaStream_t s) {
