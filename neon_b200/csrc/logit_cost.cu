@@ -576,7 +576,7 @@ template <int DT, int V> struct Pairs {
 };
 
 template <int DT, int V>
-__global__ void __launch_bounds__(kColThreads) cost_cols_stats(const __grid_constant__ ColsP p) {
+__global__ void __launch_bounds__(kColThreads, 4) cost_cols_stats(const __grid_constant__ ColsP p) {
     grid_enter();
     constexpr int U = 4, P = Pairs<DT, V>::P;
     __shared__ float2 red[kColThreads * V];
@@ -774,20 +774,26 @@ template <bool POLICY, int DT, int V> cudaError_t launch_cols(const CostP& all, 
         while (p.lanes > 1 && p.lanes * V * size > 32 && (i64)p.lanes * V / 2 >= c.N) p.lanes /= 2;
         const int wide = p.lanes * V, rows = kColThreads / p.lanes;
         const i64 across = (c.N + wide - 1) / wide;
-        i64 splits = (148 * 8 + across - 1) / across, most = ((i64)c.V + rows * 4 - 1) / (rows * 4);
-        if (splits > kSplits) splits = kSplits;
-        if (splits > most) splits = most;
-        p.rows = (int)(((i64)c.V + splits - 1) / splits);
-        p.splits = (int)(((i64)c.V + p.rows - 1) / p.rows);
+        // shares of the vocabulary: the first kernel's blocks all resident at once, the third's a
+        // quarter as long, since nothing has to be joined there
+        const i64 most = ((i64)c.V + rows * 4 - 1) / (rows * 4), room = resident_blocks(cost_cols_stats<DT, V>, kColThreads, 0);
+        if (!room) return cudaErrorInvalidConfiguration;
+        auto cut = [&](i64 splits) {
+            if (splits > most) splits = most;
+            if (splits < 1) splits = 1;
+            p.rows = (int)(((i64)c.V + splits - 1) / splits);
+            return (unsigned)(((i64)c.V + p.rows - 1) / p.rows);
+        };
         p.part = reinterpret_cast<float2*>(scratch);
         p.item = reinterpret_cast<float4*>(scratch + 8 * kSplits * slice);
         p.grad = reinterpret_cast<float*>(scratch + (8 * kSplits + 16) * slice);
-        const dim3 grid((unsigned)across, (unsigned)p.splits);
-        cudaError_t e = launch_dependent(cost_cols_stats<DT, V>, grid, kColThreads, 0, s, p);
+        p.splits = (int)cut(room / across < kSplits ? room / across : kSplits);
+        cudaError_t e = launch_dependent(cost_cols_stats<DT, V>, dim3((unsigned)across, (unsigned)p.splits), kColThreads, 0, s, p);
         if (e == cudaSuccess) e = launch_dependent(cost_cols_items<POLICY>, dim3((unsigned)c.N), 32, POLICY ? 0 : 12 * ((c.K + 3) / 4 * 4), s, p);
         launches += 2;
         if (e == cudaSuccess && c.d) {
-            e = launch_dependent(cost_cols_delta<DT, V>, grid, kColThreads, 0, s, p);
+            const unsigned shares = cut(4 * room / across < 65535 ? 4 * room / across : 65535);
+            e = launch_dependent(cost_cols_delta<DT, V>, dim3((unsigned)across, shares), kColThreads, 0, s, p);
             if (e == cudaSuccess) e = launch_dependent(cost_cols_put<POLICY>, dim3((unsigned)((c.N * c.K + 255) / 256)), 256, 0, s, p);
             launches += 2;
         }
