@@ -442,46 +442,87 @@ template <bool BACK> cudaError_t launch_type(const LnP& p, bool mis, float* part
 
 // ---- items next to each other (their stride is 1; neon's own order)
 //
-// A block takes a stripe of neighbouring items, `lanes` threads with V items each side by side and
-// its other threads down the features, so every access is a run of 32 to 128 bytes of a feature's
-// row.  With enough stripes for the machine a block sees all features of its items: it copies the
-// stripe to shared memory (HELD; every thread its own vectors), so HBM is read once, or, where that
-// is too small, walks over it again.  With few stripes the features are split over blocks as well,
-// and a second kernel joins their sums: of a share of n_i features its mean m_i and centred squares
-// q_i, which give the item's mean sum n_i m_i / F and squares sum q_i + n_i (m_i - mean)^2.
+// A block takes a stripe of neighbouring items, `lanes` threads side by side and its other threads
+// down the features, so every access is a run of 32 to 128 bytes of a feature's row.  With enough
+// stripes for the machine a block sees all features of its items: it copies the stripe to shared
+// memory (HELD; every thread its own vectors), so HBM is read once, or, where that is too small,
+// walks over it again.  With few stripes the features are split over blocks as well, and a second
+// kernel joins their sums: of a share of n_i features its mean m_i and centred squares q_i, which
+// give the item's mean sum n_i m_i / F and squares sum q_i + n_i (m_i - mean)^2.
 //
-// Neighbouring items as pairs; a single item (V = 1) is a pair with 0.
+// What bounds them: the instructions of an element (conversion, the sums, the result), with a
+// stripe's three phases in turn; the loops have constant distances for that (76 -> 69 us, backwards
+// 179 -> 152 us at 1024 x 65536 bf16, 60 % and 41 % of the copy rate, and 21 us backwards at
+// 1001 x 4096 f32).  Rows that are not whole 16-byte vectors go item by item: 82 and 199 us at
+// 1001 x 32767 bf16, four items a thread, against 103 and 317 us with one.
+//
+// A thread's place in its stripe: its V items, next to each other from n on, or, where the rows do
+// not consist of whole 16-byte vectors (V = -4), four of them `lanes` apart, of which `count` exist;
+// and its features: ty, ty + rows, ... below F.
+struct Place { int lanes, tx, ty, rows, F, count; i64 n; bool in; };
+enum { kColsT = 512, kColsWarps = kColsT / 32 };
+template <int V> struct Width { static constexpr int P = (V > 0 ? V : -V) / 2; };
+template <int V> DEV Place place(i64 stripe, int lanes, i64 N, i64 F) {
+    Place q;
+    q.lanes = lanes; q.tx = threadIdx.x & (lanes - 1); q.ty = threadIdx.x / lanes; q.rows = kColsT / lanes; q.F = (int)F;
+    q.n = V > 0 ? (stripe * lanes + q.tx) * V : stripe * lanes * -V + q.tx;
+    q.in = q.n < N;
+    q.count = V > 0 ? V : 0;
+    if constexpr (V < 0) {
+#pragma unroll
+        for (int l = 0; l < -V; ++l) q.count += q.n + l * lanes < N;
+    }
+    return q;
+}
+// A thread's items of one feature, as pairs.
 template <int DT, int V> struct Items {
-    static constexpr int P = V > 1 ? V / 2 : 1, W = V > 1 ? 4 : 1;
-    u32 w[W];
-    DEV void load(u64 base, i64 at) { ld_w<DT, V, false>(base, at, w); }
-    DEV void load(const u32* held) { ld_raw<dt_size<DT>::value * V, false>(reinterpret_cast<const char*>(held), w); }
-    DEV f32x2 get(int l) const {
-        if constexpr (V > 1) return get2<DT>(w, l);
-        else { float z[1]; cvt_in<DT, 1>(w, z); return pair(z[0], 0.f); }
+    static constexpr int P = Width<V>::P;
+    u32 w[4];
+    DEV void load(u64 base, i64 at, const Place&) { ld_w<DT, V, false>(base, at, w); }
+    DEV void load(const u32* held) { ld_raw<16, false>(reinterpret_cast<const char*>(held), w); }
+    DEV f32x2 get(int l) const { return get2<DT>(w, l); }
+    DEV void set(int l, f32x2 v) { set2<DT>(w, l, v); }
+    DEV void store(u64 base, i64 at, const Place&) const { st_raw<16>(reinterpret_cast<char*>(base) + at * dt_size<DT>::value, w); }
+};
+template <int DT> struct Items<DT, -4> {
+    static constexpr int P = Width<-4>::P;
+    float v[2 * P];
+    DEV void load(u64 base, i64 at, const Place& q) {
+#pragma unroll
+        for (int l = 0; l < 2 * P; ++l) {                                   // (no branches: the first exists)
+            const float x = ld_any(base, at + (l < q.count ? l * q.lanes : 0), DT);
+            v[l] = l < q.count ? x : 0.f;
+        }
     }
-    DEV void set(int l, f32x2 v) {
-        if constexpr (V > 1) set2<DT>(w, l, v);
-        else { float x, y; split(v, x, y); cvt_out<DT, 1, false>(&x, w, SrCtx(), nullptr); }
+    DEV f32x2 get(int l) const { return pair(v[2 * l], v[2 * l + 1]); }
+    DEV void set(int l, f32x2 x) { split(x, v[2 * l], v[2 * l + 1]); }
+    DEV void store(u64 base, i64 at, const Place& q) const {
+#pragma unroll
+        for (int l = 0; l < 2 * P; ++l)
+            if (l < q.count) st_any(base, at + l * q.lanes, DT, v[l]);
     }
-    DEV void store(u64 base, i64 at) const { st_raw<dt_size<DT>::value * V>(reinterpret_cast<char*>(base) + at * dt_size<DT>::value, w); }
 };
 // One value per item of a thread, from a vector of one value per item, and back.
-template <int V> DEV void get_items(u64 base, i64 n, f32x2* v) {
-    const float* at = reinterpret_cast<const float*>(base) + n;
-    if constexpr (V > 1) {
+template <int V> DEV void get_items(u64 base, const Place& q, f32x2* v) {
+    const float* at = reinterpret_cast<const float*>(base) + q.n;
 #pragma unroll
-        for (int l = 0; l < V / 2; ++l) v[l] = pair(at[2 * l], at[2 * l + 1]);
-    } else v[0] = pair(at[0], 0.f);
+    for (int l = 0; l < Width<V>::P; ++l) {
+        if constexpr (V > 0) v[l] = pair(at[2 * l], at[2 * l + 1]);
+        else {
+            const float x = at[2 * l < q.count ? 2 * l * q.lanes : 0], y = at[2 * l + 1 < q.count ? (2 * l + 1) * q.lanes : 0];
+            v[l] = pair(2 * l < q.count ? x : 0.f, 2 * l + 1 < q.count ? y : 0.f);
+        }
+    }
 }
-template <int V> DEV void put_items(u64 base, i64 n, const f32x2* v) {
-    float* at = reinterpret_cast<float*>(base) + n;
+template <int V> DEV void put_items(u64 base, const Place& q, const f32x2* v) {
+    float* at = reinterpret_cast<float*>(base) + q.n;
+    const int step = V > 0 ? 1 : q.lanes;
 #pragma unroll
-    for (int l = 0; l < (V > 1 ? V / 2 : 1); ++l) {
+    for (int l = 0; l < Width<V>::P; ++l) {
         float x, y;
         split(v[l], x, y);
-        at[V > 1 ? 2 * l : 0] = x;
-        if constexpr (V > 1) at[2 * l + 1] = y;
+        if (2 * l < q.count) at[2 * l * step] = x;
+        if (2 * l + 1 < q.count) at[(2 * l + 1) * step] = y;
     }
 }
 DEV f32x2 both_of(float x) { return pair(x, x); }
@@ -489,9 +530,8 @@ DEV f32x2 minus(f32x2 v) { float x, y; split(v, x, y); return pair(-x, -y); }
 
 // Sums over the threads of a stripe that share its items: within the warps, then by one thread per
 // value over the warps; `s` holds 17 times the stripe's items.
-enum { kColsT = 512, kColsWarps = kColsT / 32 };
 template <int V> DEV void stripe_sum(f32x2* v, float* s, int lanes) {
-    constexpr int P = V > 1 ? V / 2 : 1;
+    constexpr int P = Width<V>::P;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tx = threadIdx.x & (lanes - 1), wide = lanes * 2 * P;
 #pragma unroll
     for (int l = 0; l < P; ++l) {
@@ -519,25 +559,16 @@ template <int V> DEV void stripe_sum(f32x2* v, float* s, int lanes) {
 #pragma unroll
     for (int l = 0; l < P; ++l) v[l] = *reinterpret_cast<const f32x2*>(s + kColsWarps * wide + tx * 2 * P + 2 * l);
 }
-enum { kStripeFloats = (kColsWarps + 1) * 64 };     // at most 64 values side by side
+enum { kStripeFloats = (kColsWarps + 1) * 128 };     // at most 128 items side by side
 
-// A thread's place in its stripe, and its features: first, first + rows, ... below end.
-struct Place { int lanes, tx, ty, rows, F; i64 n; bool in; };
-template <int V> DEV Place place(i64 stripe, int lanes, i64 N, i64 F) {
-    Place q;
-    q.lanes = lanes; q.tx = threadIdx.x & (lanes - 1); q.ty = threadIdx.x / lanes; q.rows = blockDim.x / lanes; q.F = (int)F;
-    q.n = (stripe * lanes + q.tx) * V;
-    q.in = q.n < N;
-    return q;
-}
 // A thread's vectors of a stripe, copied to its own places in shared memory.
 template <int DT> DEV void hold(const u32* to, u64 base, i64 pitch, const Place& q) {
     u32 at = (u32)__cvta_generic_to_shared(to + threadIdx.x * 4);
-    for (int f = q.ty; f < q.F; f += q.rows, at += blockDim.x * 16) copy16(at, base + (u64)((f * pitch + q.n) * dt_size<DT>::value));
+    for (int f = q.ty; f < q.F; f += q.rows, at += kColsT * 16) copy16(at, base + (u64)((f * pitch + q.n) * dt_size<DT>::value));
 }
-template <int DT, int V, bool HELD> DEV void look(Items<DT, V>& x, const u32* held, int k, u64 base, i64 at) {
-    if constexpr (HELD) x.load(held + (k * blockDim.x + threadIdx.x) * 4);
-    else x.load(base, at);
+template <int DT, int V, bool HELD> DEV void look(Items<DT, V>& x, const u32* held, int k, u64 base, i64 at, const Place& q) {
+    if constexpr (HELD) x.load(held + (k * kColsT + threadIdx.x) * 4);
+    else x.load(base, at, q);
 }
 // mean and centred squares of features [f0, f1) of the stripe's items
 template <int DT, int V, bool HELD> DEV void moments(const LnP& p, const Place& q, const u32* held, int f0, int f1, float* s, f32x2* mean, f32x2* squares) {
@@ -548,7 +579,7 @@ template <int DT, int V, bool HELD> DEV void moments(const LnP& p, const Place& 
 #pragma unroll 4
         for (int f = f0 + q.ty, k = 0; f < f1; f += q.rows, ++k) {
             Items<DT, V> x;
-            look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
+            look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n, q);
 #pragma unroll
             for (int l = 0; l < P; ++l) mean[l] = add2(mean[l], x.get(l));
         }
@@ -564,7 +595,7 @@ template <int DT, int V, bool HELD> DEV void moments(const LnP& p, const Place& 
 #pragma unroll 4
         for (int f = f0 + q.ty, k = 0; f < f1; f += q.rows, ++k) {
             Items<DT, V> x;
-            look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
+            look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n, q);
 #pragma unroll
             for (int l = 0; l < P; ++l) { const f32x2 d = add2(x.get(l), less[l]); squares[l] = fma2(d, d, squares[l]); }
         }
@@ -589,18 +620,19 @@ template <int DT, int V, bool HELD> DEV void normalise(const LnP& p, const Place
     for (int f = f0 + q.ty, k = 0; f < f1; f += q.rows, ++k) {
         const f32x2 g = both_of(p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f), b = both_of(p.beta ? ld_any(p.beta, f, p.pdt) : 0.f);
         Items<DT, V> x;
-        look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
+        look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n, q);
 #pragma unroll
         for (int l = 0; l < P; ++l) x.set(l, fma2(mul2(add2(x.get(l), less[l]), rstd[l]), g, b));
-        x.store(p.out, f * p.o0 + q.n);
+        x.store(p.out, f * p.o0 + q.n, q);
     }
 }
 
-template <int DT, int V, bool HELD>
+// (LANES: the stripe's width where it is known to the compiler, or 0)
+template <int DT, int V, bool HELD, int LANES>
 __global__ void __launch_bounds__(kColsT) ln_fprop_cols(const __grid_constant__ LnP p, int lanes) {
     extern __shared__ __align__(16) u32 held[];
     __shared__ __align__(16) float s[kStripeFloats];
-    const Place q = place<V>(blockIdx.x, lanes, p.N, p.F);
+    const Place q = place<V>(blockIdx.x, LANES ? LANES : lanes, p.N, p.F);
     if constexpr (HELD) {
         if (q.in) hold<DT>(held, p.x, p.x0, q);
         copy_commit();
@@ -611,8 +643,8 @@ __global__ void __launch_bounds__(kColsT) ln_fprop_cols(const __grid_constant__ 
     to_rstd(rstd, 1.f / (float)q.F, p.eps);
     if (!q.in) return;
     if (q.ty == 0) {
-        if (p.mean) put_items<V>(p.mean, q.n, mean);
-        if (p.rstd) put_items<V>(p.rstd, q.n, rstd);
+        if (p.mean) put_items<V>(p.mean, q, mean);
+        if (p.rstd) put_items<V>(p.rstd, q, rstd);
     }
     normalise<DT, V, HELD>(p, q, held, 0, q.F, mean, rstd);
 }
@@ -628,28 +660,29 @@ __global__ void __launch_bounds__(kColsT) ln_split_moments(const __grid_constant
     moments<DT, V, false>(p, q, nullptr, f0, f1, s, mean, squares);
     if (!q.in || q.ty) return;
     float* to = part + (i64)blockIdx.y * 2 * p.N;
-    put_items<V>((u64)to, q.n, mean);
-    put_items<V>((u64)(to + p.N), q.n, squares);
+    put_items<V>((u64)to, q, mean);
+    put_items<V>((u64)(to + p.N), q, squares);
 }
 template <int DT, int V>
 __global__ void __launch_bounds__(kColsT) ln_split_fprop(const __grid_constant__ LnP p, int lanes, int per, const float* part) {
     grid_enter();
     constexpr int P = Items<DT, V>::P;
     const Place q = place<V>(blockIdx.x, lanes, p.N, p.F);
-    if (!q.in) return;
+    __shared__ __align__(16) float s[kStripeFloats];
     const float inv = 1.f / (float)q.F;
     f32x2 mean[P], rstd[P], m[P], m2[P];
 #pragma unroll
     for (int l = 0; l < P; ++l) mean[l] = rstd[l] = 0;
-    for (int k = 0; k < (int)gridDim.y; ++k) {
-        get_items<V>((u64)(part + (i64)k * 2 * p.N), q.n, m);
+    for (int k = q.ty; k < (int)gridDim.y && q.in; k += q.rows) {           // the stripe's threads take a share each
+        get_items<V>((u64)(part + (i64)k * 2 * p.N), q, m);
         const float n = (float)(min((k + 1) * per, q.F) - k * per) * inv;
 #pragma unroll
         for (int l = 0; l < P; ++l) mean[l] = fma2(m[l], both_of(n), mean[l]);
     }
-    for (int k = 0; k < (int)gridDim.y; ++k) {
-        get_items<V>((u64)(part + (i64)k * 2 * p.N), q.n, m);
-        get_items<V>((u64)(part + ((i64)k * 2 + 1) * p.N), q.n, m2);
+    stripe_sum<V>(mean, s, q.lanes);
+    for (int k = q.ty; k < (int)gridDim.y && q.in; k += q.rows) {
+        get_items<V>((u64)(part + (i64)k * 2 * p.N), q, m);
+        get_items<V>((u64)(part + ((i64)k * 2 + 1) * p.N), q, m2);
         const float n = (float)(min((k + 1) * per, q.F) - k * per);
 #pragma unroll
         for (int l = 0; l < P; ++l) {
@@ -657,19 +690,23 @@ __global__ void __launch_bounds__(kColsT) ln_split_fprop(const __grid_constant__
             rstd[l] = fma2(mul2(d, both_of(n)), d, add2(rstd[l], m2[l]));
         }
     }
+    stripe_sum<V>(rstd, s, q.lanes);
+    if (!q.in) return;
     to_rstd(rstd, inv, p.eps);
     if (q.ty == 0 && blockIdx.y == 0) {
-        if (p.mean) put_items<V>(p.mean, q.n, mean);
-        if (p.rstd) put_items<V>(p.rstd, q.n, rstd);
+        if (p.mean) put_items<V>(p.mean, q, mean);
+        if (p.rstd) put_items<V>(p.rstd, q, rstd);
     }
     const int f0 = blockIdx.y * per;
     normalise<DT, V, false>(p, q, nullptr, f0, min(f0 + per, q.F), mean, rstd);
 }
 
 // Sums of g and g h over features [f0, f1) of the stripe's items, and the stripe's share of the
-// parameters' gradients at those features, added to acc (`more`) or put there.
+// parameters' gradients at those features, added (`more`) to what is there or put there: in `own`,
+// two sums for every feature of every thread, or, over all items of the stripe, in acc.
 template <int DT, int V, bool HELD> DEV void error_sums(const LnP& p, const Place& q, const u32* held, const u32* held_e, int f0, int f1,
-                                                        float* s, const f32x2* mean, const f32x2* rstd, f32x2* a, f32x2* b, float* acc, bool more) {
+                                                        float* s, const f32x2* mean, const f32x2* rstd, f32x2* a, f32x2* b,
+                                                        float* acc, f32x2* own, bool more) {
     constexpr int P = Items<DT, V>::P;
     f32x2 less[P];
 #pragma unroll
@@ -680,8 +717,8 @@ template <int DT, int V, bool HELD> DEV void error_sums(const LnP& p, const Plac
         if (q.in && f < f1) {
             const f32x2 gamma = both_of(p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f);
             Items<DT, V> x, e;
-            look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
-            look<DT, V, HELD>(e, held_e, k, p.e, f * p.e0 + q.n);
+            look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n, q);
+            look<DT, V, HELD>(e, held_e, k, p.e, f * p.e0 + q.n, q);
 #pragma unroll
             for (int l = 0; l < P; ++l) {
                 const f32x2 h = mul2(add2(x.get(l), less[l]), rstd[l]), err = e.get(l), g = mul2(err, gamma);
@@ -691,7 +728,11 @@ template <int DT, int V, bool HELD> DEV void error_sums(const LnP& p, const Plac
                 b[l] = fma2(g, h, b[l]);
             }
         }
-        if (acc) {
+        if (own) {
+            f32x2& sum = own[k * kColsT + threadIdx.x];
+            const f32x2 v = pair(both(gg), both(gb));
+            sum = more ? add2(sum, v) : v;
+        } else if (acc) {
             float x = both(gg), y = both(gb);
             for (int o = q.lanes >> 1; o; o >>= 1) {
                 x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -717,28 +758,31 @@ template <int DT, int V, bool HELD> DEV void put_delta(const LnP& p, const Place
     for (int f = f0 + q.ty, k = 0; f < f1; f += q.rows, ++k) {
         const f32x2 gamma = both_of(p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f);
         Items<DT, V> x, e;
-        look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n);
-        look<DT, V, HELD>(e, held_e, k, p.e, f * p.e0 + q.n);
+        look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n, q);
+        look<DT, V, HELD>(e, held_e, k, p.e, f * p.e0 + q.n, q);
 #pragma unroll
         for (int l = 0; l < P; ++l) {
             const f32x2 h = mul2(add2(x.get(l), less[l]), rstd[l]);
             x.set(l, mul2(rstd[l], fma2(h, mb[l], fma2(e.get(l), gamma, ma[l]))));
         }
-        x.store(p.out, f * p.o0 + q.n);
+        x.store(p.out, f * p.o0 + q.n, q);
     }
 }
 
 // A block works through stripes gridDim.x apart; part[block][0][F]: its share of grad_gamma,
-// part[block][1][F]: of grad_beta, gathered in shared memory if `acc_held`.
-template <int DT, int V, bool HELD>
-__global__ void __launch_bounds__(kColsT, 2) ln_bprop_cols(const __grid_constant__ LnP p, float* part, int lanes, i64 stripes, int acc_held) {
-    extern __shared__ __align__(16) u32 mem[];         // x, the error, the block's share of the gradients
+// part[block][1][F]: of grad_beta, gathered in shared memory, per thread if `own_sums`, per
+// feature if `acc_held`.
+template <int DT, int V, bool HELD, int LANES>
+__global__ void __launch_bounds__(kColsT, 2) ln_bprop_cols(const __grid_constant__ LnP p, float* part, int width, i64 stripes, int own_sums, int acc_held) {
+    extern __shared__ __align__(16) u32 mem[];         // x, the error, the threads' shares of the gradients
     __shared__ __align__(16) float s[kStripeFloats];
     constexpr int P = Items<DT, V>::P;
-    const int F = (int)p.F, rows = kColsT / lanes, each = HELD ? (F + rows - 1) / rows : 0;
+    const int lanes = LANES ? LANES : width, F = (int)p.F, rows = kColsT / lanes, each = (F + rows - 1) / rows;
     const u32 *held = mem, *held_e = mem + each * kColsT * 4;
     float* mine = part ? part + (i64)blockIdx.x * 2 * F : nullptr;
-    float* acc = part && acc_held ? reinterpret_cast<float*>(mem + 2 * each * kColsT * 4) : mine;
+    u32* behind = mem + (HELD ? 2 * each * kColsT * 4 : 0);
+    f32x2* own = own_sums ? reinterpret_cast<f32x2*>(behind) : nullptr;
+    float* acc = acc_held ? reinterpret_cast<float*>(behind) : mine;
     for (i64 stripe = blockIdx.x; stripe < stripes; stripe += gridDim.x) {
         const Place q = place<V>(stripe, lanes, p.N, p.F);
         if constexpr (HELD) {
@@ -752,16 +796,25 @@ __global__ void __launch_bounds__(kColsT, 2) ln_bprop_cols(const __grid_constant
 #pragma unroll
         for (int l = 0; l < P; ++l) mean[l] = rstd[l] = 0;
         if (q.in) {
-            get_items<V>(p.mean, q.n, mean);
-            get_items<V>(p.rstd, q.n, rstd);
+            get_items<V>(p.mean, q, mean);
+            get_items<V>(p.rstd, q, rstd);
         }
         if constexpr (HELD) copy_wait<0>();
-        error_sums<DT, V, HELD>(p, q, held, held_e, 0, F, s, mean, rstd, a, b, acc, stripe != blockIdx.x);
+        error_sums<DT, V, HELD>(p, q, held, held_e, 0, F, s, mean, rstd, a, b, acc, own, stripe != blockIdx.x);
         if (q.in) put_delta<DT, V, HELD>(p, q, held, held_e, 0, F, mean, rstd, a, b);
     }
-    if (acc == mine) return;
+    if (!own && !acc_held) return;
     __syncthreads();
-    for (int f = threadIdx.x; f < 2 * F; f += kColsT) mine[f] = acc[f];
+    for (int f = threadIdx.x; f < F; f += kColsT) {
+        if (!own) {
+            mine[f] = acc[f];
+            mine[F + f] = acc[F + f];
+            continue;
+        }
+        f32x2 sum = 0;
+        for (int t = 0; t < lanes; ++t) sum = add2(sum, own[f / rows * kColsT + f % rows * lanes + t]);
+        split(sum, mine[f], mine[F + f]);
+    }
 }
 
 // sums[split][0][N]: of g, sums[split][1][N]: of g h over a share of `per` features;
@@ -777,34 +830,38 @@ __global__ void __launch_bounds__(kColsT) ln_split_sums(const __grid_constant__ 
 #pragma unroll
     for (int l = 0; l < P; ++l) mean[l] = rstd[l] = 0;
     if (q.in) {
-        get_items<V>(p.mean, q.n, mean);
-        get_items<V>(p.rstd, q.n, rstd);
+        get_items<V>(p.mean, q, mean);
+        get_items<V>(p.rstd, q, rstd);
     }
-    error_sums<DT, V, false>(p, q, nullptr, nullptr, f0, f1, s, mean, rstd, a, b, part ? part + (i64)blockIdx.x * 2 * p.F : nullptr, false);
+    error_sums<DT, V, false>(p, q, nullptr, nullptr, f0, f1, s, mean, rstd, a, b,
+                             part ? part + (i64)blockIdx.x * 2 * p.F : nullptr, nullptr, false);
     if (!q.in || q.ty) return;
     float* to = sums + (i64)blockIdx.y * 2 * p.N;
-    put_items<V>((u64)to, q.n, a);
-    put_items<V>((u64)(to + p.N), q.n, b);
+    put_items<V>((u64)to, q, a);
+    put_items<V>((u64)(to + p.N), q, b);
 }
 template <int DT, int V>
 __global__ void __launch_bounds__(kColsT) ln_split_delta(const __grid_constant__ LnP p, int lanes, int per, const float* sums) {
     grid_enter();
     constexpr int P = Items<DT, V>::P;
     const Place q = place<V>(blockIdx.x, lanes, p.N, p.F);
-    if (!q.in) return;
+    __shared__ __align__(16) float s[kStripeFloats];
     f32x2 mean[P], rstd[P], a[P], b[P], x[P];
-    get_items<V>(p.mean, q.n, mean);
-    get_items<V>(p.rstd, q.n, rstd);
 #pragma unroll
     for (int l = 0; l < P; ++l) a[l] = b[l] = 0;
-    for (int k = 0; k < (int)gridDim.y; ++k) {
-        get_items<V>((u64)(sums + (i64)k * 2 * p.N), q.n, x);
+    for (int k = q.ty; k < (int)gridDim.y && q.in; k += q.rows) {
+        get_items<V>((u64)(sums + (i64)k * 2 * p.N), q, x);
 #pragma unroll
         for (int l = 0; l < P; ++l) a[l] = add2(a[l], x[l]);
-        get_items<V>((u64)(sums + ((i64)k * 2 + 1) * p.N), q.n, x);
+        get_items<V>((u64)(sums + ((i64)k * 2 + 1) * p.N), q, x);
 #pragma unroll
         for (int l = 0; l < P; ++l) b[l] = add2(b[l], x[l]);
     }
+    stripe_sum<V>(a, s, q.lanes);
+    stripe_sum<V>(b, s, q.lanes);
+    if (!q.in) return;
+    get_items<V>(p.mean, q, mean);
+    get_items<V>(p.rstd, q, rstd);
     const int f0 = blockIdx.y * per;
     put_delta<DT, V, false>(p, q, nullptr, nullptr, f0, min(f0 + per, q.F), mean, rstd, a, b);
 }
@@ -822,18 +879,19 @@ bool cols_fit(const b200_matrix* const* m, int count, i64 N, bool& wide) {
 
 // How a call in this order is cut.  Stripes of 128 bytes, or down to 32 bytes where wider ones would
 // leave SMs without a block or would not fit twice into an SM's shared memory; below 148 stripes of
-// 32 bytes, the features in shares of at least 4 per thread, at most 64 of them.
+// 32 bytes, the features in shares of at least 4 vectors per thread, at most 64 of them.
 enum { kMaxSplits = 64 };
 struct Cols { int lanes, splits, per, held; i64 stripes; };
-Cols cols_plan(i64 F, i64 N, int size, int V, bool back) {          // size: bytes of a thread's items
+Cols cols_plan(i64 F, i64 N, int esize, int V, bool back) {
     Cols c;
-    c.lanes = 128 / size > 32 ? 32 : 128 / size;
-    auto stripes = [&](int l) { return (N + (i64)l * V - 1) / ((i64)l * V); };
+    const int items = V > 0 ? V : -V, size = items * esize;             // a thread's
+    c.lanes = V > 0 ? 128 / size : 32;
+    auto stripes = [&](int l) { return (N + (i64)l * items - 1) / ((i64)l * items); };
     while (c.lanes > 1 && c.lanes * size > 32 && stripes(c.lanes) < 2 * 148) c.lanes /= 2;
     c.splits = 1; c.per = (int)F; c.held = 0;
     c.stripes = stripes(c.lanes);
     if (c.stripes < 148) {
-        i64 splits = 2 * 148 / c.stripes, most = F / (4 * (kColsT / c.lanes));
+        i64 splits = 2 * 148 / c.stripes, most = F / ((V > 0 ? 4 : 1) * (kColsT / c.lanes));
         if (splits > most) splits = most;
         if (splits > kMaxSplits) splits = kMaxSplits;
         if (splits > 1) {
@@ -844,27 +902,46 @@ Cols cols_plan(i64 F, i64 N, int size, int V, bool back) {          // size: byt
     }
     if (V > 1) {
         auto bytes = [&](int l) { return (F + kColsT / l - 1) / (kColsT / l) * kColsT * 16 * (back ? 2 : 1); };
-        while (c.lanes > 2 && bytes(c.lanes) > 100 * 1024) c.lanes /= 2;
-        if (bytes(c.lanes) <= 200 * 1024) c.held = (int)bytes(c.lanes);
-        c.stripes = stripes(c.lanes);
+        const i64 room = (back ? 86 : 100) * 1024;     // backwards, half as much again for the gradients' shares is wanted too
+        int lanes = c.lanes;
+        while (lanes > 2 && bytes(lanes) > room) lanes /= 2;
+        if (bytes(lanes) <= 200 * 1024) {
+            c.lanes = lanes;
+            c.held = (int)bytes(lanes);
+            c.stripes = stripes(lanes);
+        }
     }
     return c;
 }
 // Scratch of the split form, in front of the gradients' shares.
 inline i64 split_bytes(i64 N) { return N < 148 * 64 ? (kMaxSplits * 8 * N + 255) / 256 * 256 : 0; }
 
-template <int DT, int V, bool HELD> cudaError_t launch_cols_back(const LnP& p, const Cols& c, float* part, int* parts, cudaStream_t s) {
-    const int acc = part && p.F <= 4096 && c.held + 8 * p.F <= 216 * 1024 ? (int)(8 * p.F) : 0, smem = c.held + acc;
-    i64 grid = resident_blocks(ln_bprop_cols<DT, V, HELD>, kColsT, smem);
+template <int DT, int V, bool HELD, int LANES> cudaError_t launch_cols_back(const LnP& p, const Cols& c, float* part, int* parts, cudaStream_t s) {
+    const i64 rows = kColsT / c.lanes, own = (p.F + rows - 1) / rows * kColsT * 8;
+    const bool own_sums = part && c.held + own <= 216 * 1024;
+    const bool acc_held = part && !own_sums && p.F <= 4096 && c.held + 8 * p.F <= 216 * 1024;
+    const int smem = c.held + (own_sums ? (int)own : acc_held ? (int)(8 * p.F) : 0);
+    auto kernel = ln_bprop_cols<DT, V, HELD, LANES>;
+    i64 grid = resident_blocks(kernel, kColsT, smem);
     if (!grid) return cudaErrorInvalidConfiguration;
     if (grid > c.stripes) grid = c.stripes;
     if (part && grid > most_parts(p.F)) grid = most_parts(p.F);
     *parts = (int)grid;
-    ln_bprop_cols<DT, V, HELD><<<(unsigned)grid, kColsT, smem, s>>>(p, part, c.lanes, c.stripes, acc != 0);
+    kernel<<<(unsigned)grid, kColsT, smem, s>>>(p, part, c.lanes, c.stripes, own_sums, acc_held);
     return cudaGetLastError();
 }
+template <int DT, int V, bool HELD, int LANES> cudaError_t launch_cols_forward(const LnP& p, const Cols& c, cudaStream_t s) {
+    auto kernel = ln_fprop_cols<DT, V, HELD, LANES>;
+    if (!resident_blocks(kernel, kColsT, c.held)) return cudaErrorInvalidConfiguration;
+    kernel<<<(unsigned)c.stripes, kColsT, c.held, s>>>(p, c.lanes);
+    return cudaGetLastError();
+}
+template <int DT, int V, bool BACK, bool HELD, int LANES> cudaError_t launch_cols_one(const LnP& p, const Cols& c, float* part, int* parts, cudaStream_t s) {
+    if constexpr (BACK) return launch_cols_back<DT, V, HELD, LANES>(p, c, part, parts, s);
+    else return launch_cols_forward<DT, V, HELD, LANES>(p, c, s);
+}
 template <int DT, int V, bool BACK> cudaError_t launch_cols(const LnP& p, char* scratch, float* part, int* parts, int& launches, cudaStream_t s) {
-    const Cols c = cols_plan(p.F, p.N, dt_size<DT>::value * V, V, BACK);
+    const Cols c = cols_plan(p.F, p.N, dt_size<DT>::value, V, BACK);
     float* sums = reinterpret_cast<float*>(scratch);
     const dim3 grid((unsigned)c.stripes, (unsigned)c.splits);
     if (c.splits > 1) {
@@ -881,26 +958,18 @@ template <int DT, int V, bool BACK> cudaError_t launch_cols(const LnP& p, char* 
         return e;
     }
     ++launches;
-    if constexpr (BACK) {
-        if constexpr (V > 1) if (c.held) return launch_cols_back<DT, V, true>(p, c, part, parts, s);
-        return launch_cols_back<DT, V, false>(p, c, part, parts, s);
-    } else {
-        if constexpr (V > 1) {
-            if (c.held) {
-                if (!resident_blocks(ln_fprop_cols<DT, V, true>, kColsT, c.held)) return cudaErrorInvalidConfiguration;
-                ln_fprop_cols<DT, V, true><<<(unsigned)c.stripes, kColsT, c.held, s>>>(p, c.lanes);
-                return cudaGetLastError();
-            }
-        }
-        ln_fprop_cols<DT, V, false><<<(unsigned)c.stripes, kColsT, 0, s>>>(p, c.lanes);
-        return cudaGetLastError();
+    if constexpr (V > 1) {
+        if (c.held && c.lanes == 8) return launch_cols_one<DT, V, BACK, true, 8>(p, c, part, parts, s);
+        if (c.held && c.lanes == 4) return launch_cols_one<DT, V, BACK, true, 4>(p, c, part, parts, s);
+        if (c.held && c.lanes == 2) return launch_cols_one<DT, V, BACK, true, 2>(p, c, part, parts, s);
     }
+    return launch_cols_one<DT, V, BACK, false, 0>(p, c, part, parts, s);
 }
 template <bool BACK> cudaError_t launch_cols_type(const LnP& p, bool wide, char* scratch, float* part, int* parts, int& launches, cudaStream_t s) {
     switch (p.dt) {
-    case B200_F32: return wide ? launch_cols<F32, 4, BACK>(p, scratch, part, parts, launches, s) : launch_cols<F32, 1, BACK>(p, scratch, part, parts, launches, s);
-    case B200_F16: return wide ? launch_cols<F16, 8, BACK>(p, scratch, part, parts, launches, s) : launch_cols<F16, 1, BACK>(p, scratch, part, parts, launches, s);
-    default: return wide ? launch_cols<BF16, 8, BACK>(p, scratch, part, parts, launches, s) : launch_cols<BF16, 1, BACK>(p, scratch, part, parts, launches, s);
+    case B200_F32: return wide ? launch_cols<F32, 4, BACK>(p, scratch, part, parts, launches, s) : launch_cols<F32, -4, BACK>(p, scratch, part, parts, launches, s);
+    case B200_F16: return wide ? launch_cols<F16, 8, BACK>(p, scratch, part, parts, launches, s) : launch_cols<F16, -4, BACK>(p, scratch, part, parts, launches, s);
+    default: return wide ? launch_cols<BF16, 8, BACK>(p, scratch, part, parts, launches, s) : launch_cols<BF16, -4, BACK>(p, scratch, part, parts, launches, s);
     }
 }
 
