@@ -690,9 +690,7 @@ __global__ void __launch_bounds__(32) cost_cols_items(const __grid_constant__ Co
     if (c.d && lane == 0) p.item[n] = make_float4(it.m, it.scale, it.dead ? 1.f : 0.f, 0.f);
 }
 
-template <int DT, int V>
-__global__ void __launch_bounds__(kColThreads) cost_cols_delta(const __grid_constant__ ColsP p) {
-    grid_enter();
+template <int DT, int V> DEV void cols_delta(const ColsP& p, int lo, int hi) {
     constexpr int U = 4, P = Pairs<DT, V>::P;
     const int lanes = p.lanes, tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = kColThreads / lanes;
     const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
@@ -714,7 +712,6 @@ __global__ void __launch_bounds__(kColThreads) cost_cols_delta(const __grid_cons
             alive[l % (V > 1 ? 4 : 1)] = (a.z != 0.f ? 0u : 0xffffu) | (b.z != 0.f ? 0u : 0xffff0000u);
         }
     }
-    const int lo = blockIdx.y * p.rows, hi = min(lo + p.rows, p.c.V);
     for (int v0 = lo + ty; v0 < hi; v0 += rows * U) {
         Pairs<DT, V> z[U];
 #pragma unroll
@@ -738,7 +735,24 @@ __global__ void __launch_bounds__(kColThreads) cost_cols_delta(const __grid_cons
     }
 }
 
-template <bool POLICY>
+// The policy cost's one entry of an item is put by the block that has its word.
+template <bool POLICY, int DT, int V>
+__global__ void __launch_bounds__(kColThreads) cost_cols_delta(const __grid_constant__ ColsP p) {
+    grid_enter();
+    const int lo = blockIdx.y * p.rows, hi = min(lo + p.rows, p.c.V);
+    cols_delta<DT, V>(p, lo, hi);
+    if constexpr (POLICY) {
+        __syncthreads();                               // after the gradients of all words
+        const int wide = p.lanes * V;
+        for (int i = threadIdx.x; i < wide; i += kColThreads) {
+            const i64 n = (i64)blockIdx.x * wide + i;
+            if (n >= p.c.N || p.item[n].z != 0.f) continue;
+            const int id = reinterpret_cast<const int*>(p.c.actions)[n];
+            if (id >= lo && id < hi) st_any(p.c.d, id * p.c.d0 + n * p.c.d1, DT, p.grad[n]);
+        }
+    }
+}
+
 __global__ void __launch_bounds__(256) cost_cols_put(const __grid_constant__ ColsP p) {
     grid_enter();
     const CostP& c = p.c;
@@ -746,9 +760,8 @@ __global__ void __launch_bounds__(256) cost_cols_put(const __grid_constant__ Col
     const int k = (int)(at / c.N);
     const i64 n = at - k * c.N;
     if (k >= c.K || p.item[n].z != 0.f) return;
-    const int id = POLICY ? reinterpret_cast<const int*>(c.actions)[n] : *(reinterpret_cast<const int*>(c.ids) + k * c.i0 + n * c.i1);
-    if (id < 0 || id >= c.V) return;
-    if (!POLICY && ld_any(c.top, k * c.t0 + n * c.t1, c.tdt) == -INFINITY) return;
+    const int id = *(reinterpret_cast<const int*>(c.ids) + k * c.i0 + n * c.i1);
+    if (id < 0 || id >= c.V || ld_any(c.top, k * c.t0 + n * c.t1, c.tdt) == -INFINITY) return;
     st_any(c.d, id * c.d0 + n * c.d1, c.dt, p.grad[at]);
 }
 
@@ -781,7 +794,8 @@ template <bool POLICY, int DT, int V> cudaError_t launch_cols(const CostP& all, 
         auto cut = [&](i64 splits) {
             if (splits > most) splits = most;
             if (splits < 1) splits = 1;
-            p.rows = (int)(((i64)c.V + splits - 1) / splits);
+            const i64 step = rows * 4, each = ((i64)c.V + splits - 1) / splits;
+            p.rows = (int)((each + step - 1) / step * step);            // whole steps of all threads
             return (unsigned)(((i64)c.V + p.rows - 1) / p.rows);
         };
         p.part = reinterpret_cast<float2*>(scratch);
@@ -793,9 +807,12 @@ template <bool POLICY, int DT, int V> cudaError_t launch_cols(const CostP& all, 
         launches += 2;
         if (e == cudaSuccess && c.d) {
             const unsigned shares = cut(4 * room / across < 65535 ? 4 * room / across : 65535);
-            e = launch_dependent(cost_cols_delta<DT, V>, dim3((unsigned)across, shares), kColThreads, 0, s, p);
-            if (e == cudaSuccess) e = launch_dependent(cost_cols_put<POLICY>, dim3((unsigned)((c.N * c.K + 255) / 256)), 256, 0, s, p);
-            launches += 2;
+            e = launch_dependent(cost_cols_delta<POLICY, DT, V>, dim3((unsigned)across, shares), kColThreads, 0, s, p);
+            ++launches;
+            if (!POLICY && e == cudaSuccess) {
+                e = launch_dependent(cost_cols_put, dim3((unsigned)((c.N * c.K + 255) / 256)), 256, 0, s, p);
+                ++launches;
+            }
         }
         if (e != cudaSuccess) return e;
     }
