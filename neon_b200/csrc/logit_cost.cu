@@ -560,77 +560,130 @@ struct ColsP {
 };
 enum { kSplits = 64, kColThreads = 256 };
 
-// neighbouring items of a word's row as pairs of fp32; a single item is a pair with -inf
+// neighbouring items of a word's row as pairs of fp32
 template <int DT, int V> struct Pairs {
-    static constexpr int P = V > 1 ? V / 2 : 1;
-    u32 w[V > 1 ? 4 : 1];
+    static constexpr int P = V / 2;
+    u32 w[4];
     DEV void load(u64 base, i64 at) { ld_w<DT, V, false>(base, at, w); }
     DEV void none() {
 #pragma unroll
         for (u32& x : w) x = DT == F32 ? 0xff800000u : DT == F16 ? 0xfc00fc00u : 0xff80ff80u;
     }
-    DEV f32x2 get(int l) const {
-        if constexpr (V > 1) return get2<DT>(w, l);
-        else { float z[1]; cvt_in<DT, 1>(w, z); return pair(z[0], -INFINITY); }
-    }
+    DEV f32x2 get(int l) const { return get2<DT>(w, l); }
 };
+// A single item's words first, first + step, ... below end (rows that are not whole 16-byte
+// vectors): eight under way, two in a pair.
+enum { kSingle = 8 };
+template <int DT> DEV void single_words(u64 base, i64 pitch, i64 n, int first, int step, int end, float* z) {
+#pragma unroll
+    for (int u = 0; u < kSingle; ++u) z[u] = first + u * step < end ? ld_any(base, (i64)(first + u * step) * pitch + n, DT) : -INFINITY;
+}
+template <int DT> DEV void single_stats(const ColsP& p, i64 n, int first, int step, int end, float& m, float& sum) {
+    const float c = p.c.c;
+    const f32x2 c2 = pair(c, c);
+    f32x2 s = 0, less = 0;
+    m = -INFINITY;
+    for (int v0 = first; v0 < end; v0 += kSingle * step) {
+        float z[kSingle];
+        single_words<DT>(p.c.z, p.c.z0, n, v0, step, end, z);
+        float a = z[0];
+#pragma unroll
+        for (int u = 1; u < kSingle; ++u) a = fmaxf(a, z[u]);
+        if (a > m) {
+            const float by = exp_of(m, usable(a), c);
+            s = mul2(s, pair(by, by));
+            m = a;
+            less = pair(-usable(a), -usable(a));
+        }
+#pragma unroll
+        for (int u = 0; u < kSingle; u += 2) {
+            float x, y;
+            split(mul2(add2(pair(z[u], z[u + 1]), less), c2), x, y);
+            s = add2(s, pair(ex2_approx(x), ex2_approx(y)));
+        }
+    }
+    sum = both(s);
+}
+template <int DT> DEV void single_delta(const ColsP& p, i64 n, int first, int step, int end) {
+    const float4 it = p.item[n];
+    const f32x2 c2 = pair(p.c.c, p.c.c), less = pair(-it.x, -it.x), scale = pair(it.y, it.y);
+    for (int v0 = first; v0 < end; v0 += kSingle * step) {
+        float z[kSingle];
+        single_words<DT>(p.c.z, p.c.z0, n, v0, step, end, z);
+#pragma unroll
+        for (int u = 0; u < kSingle; u += 2) {
+            float x, y;
+            split(mul2(add2(pair(z[u], z[u + 1]), less), c2), x, y);
+            split(mul2(scale, pair(ex2_approx(x), ex2_approx(y))), x, y);
+            const i64 v = v0 + u * step;
+            if (v < end) st_any(p.c.d, v * p.c.d0 + n, DT, it.z != 0.f ? 0.f : x);
+            if (v + step < end) st_any(p.c.d, (v + step) * p.c.d0 + n, DT, it.z != 0.f ? 0.f : y);
+        }
+    }
+}
 
 template <int DT, int V>
 __global__ void __launch_bounds__(kColThreads, 4) cost_cols_stats(const __grid_constant__ ColsP p) {
     grid_enter();
-    constexpr int U = 4, P = Pairs<DT, V>::P;
     __shared__ float2 red[kColThreads * V];
     const int lanes = p.lanes, tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = kColThreads / lanes;
     const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
     const bool in = n < p.c.N;
-    const float c = p.c.c;
-    const f32x2 c2 = pair(c, c);
-    float m[2 * P];
-    f32x2 s[P], less[P];
-#pragma unroll
-    for (int l = 0; l < P; ++l) { m[2 * l] = m[2 * l + 1] = -INFINITY; s[l] = less[l] = 0; }
     const int lo = blockIdx.y * p.rows, hi = min(lo + p.rows, p.c.V);
-    if (in) {
-        for (int v0 = lo + ty; v0 < hi; v0 += rows * U) {
-            Pairs<DT, V> z[U];
+    const float c = p.c.c;
+    if constexpr (V == 1) {
+        float m = -INFINITY, sum = 0.f;
+        if (in) single_stats<DT>(p, n, lo + ty, rows, hi, m, sum);
+        red[ty * lanes + tx] = make_float2(m, sum);
+    } else {
+        constexpr int U = 4, P = Pairs<DT, V>::P;
+        const f32x2 c2 = pair(c, c);
+        float m[2 * P];
+        f32x2 s[P], less[P];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (v0 + u * rows < hi) z[u].load(p.c.z, (i64)(v0 + u * rows) * p.c.z0 + n);
-                else z[u].none();
-            }
-#pragma unroll
-            for (int l = 0; l < P; ++l) {
-                float a = -INFINITY, b = -INFINITY;    // the largest of the step
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    float x, y;
-                    split(z[u].get(l), x, y);
-                    a = fmaxf(a, x);
-                    b = fmaxf(b, y);
-                }
-                if (a > m[2 * l] || b > m[2 * l + 1]) {
-                    a = fmaxf(a, m[2 * l]);
-                    b = fmaxf(b, m[2 * l + 1]);
-                    s[l] = mul2(s[l], pair(exp_of(m[2 * l], usable(a), c), exp_of(m[2 * l + 1], usable(b), c)));
-                    m[2 * l] = a;
-                    m[2 * l + 1] = b;
-                    less[l] = pair(-usable(a), -usable(b));
-                }
+        for (int l = 0; l < P; ++l) { m[2 * l] = m[2 * l + 1] = -INFINITY; s[l] = less[l] = 0; }
+        if (in) {
+            for (int v0 = lo + ty; v0 < hi; v0 += rows * U) {
+                Pairs<DT, V> z[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    float x, y;
-                    split(mul2(add2(z[u].get(l), less[l]), c2), x, y);
-                    s[l] = add2(s[l], pair(ex2_approx(x), ex2_approx(y)));
+                    if (v0 + u * rows < hi) z[u].load(p.c.z, (i64)(v0 + u * rows) * p.c.z0 + n);
+                    else z[u].none();
+                }
+#pragma unroll
+                for (int l = 0; l < P; ++l) {
+                    float a = -INFINITY, b = -INFINITY;    // the largest of the step
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        float x, y;
+                        split(z[u].get(l), x, y);
+                        a = fmaxf(a, x);
+                        b = fmaxf(b, y);
+                    }
+                    if (a > m[2 * l] || b > m[2 * l + 1]) {
+                        a = fmaxf(a, m[2 * l]);
+                        b = fmaxf(b, m[2 * l + 1]);
+                        s[l] = mul2(s[l], pair(exp_of(m[2 * l], usable(a), c), exp_of(m[2 * l + 1], usable(b), c)));
+                        m[2 * l] = a;
+                        m[2 * l + 1] = b;
+                        less[l] = pair(-usable(a), -usable(b));
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        float x, y;
+                        split(mul2(add2(z[u].get(l), less[l]), c2), x, y);
+                        s[l] = add2(s[l], pair(ex2_approx(x), ex2_approx(y)));
+                    }
                 }
             }
         }
-    }
 #pragma unroll
-    for (int l = 0; l < P; ++l) {
-        float x, y;
-        split(s[l], x, y);
-        red[(ty * lanes + tx) * V + 2 * l] = make_float2(m[2 * l], x);
-        if constexpr (V > 1) red[(ty * lanes + tx) * V + 2 * l + 1] = make_float2(m[2 * l + 1], y);
+        for (int l = 0; l < P; ++l) {
+            float x, y;
+            split(s[l], x, y);
+            red[(ty * lanes + tx) * V + 2 * l] = make_float2(m[2 * l], x);
+            red[(ty * lanes + tx) * V + 2 * l + 1] = make_float2(m[2 * l + 1], y);
+        }
     }
     __syncthreads();
     const int wide = lanes * V;
@@ -691,46 +744,50 @@ __global__ void __launch_bounds__(32) cost_cols_items(const __grid_constant__ Co
 }
 
 template <int DT, int V> DEV void cols_delta(const ColsP& p, int lo, int hi) {
-    constexpr int U = 4, P = Pairs<DT, V>::P;
     const int lanes = p.lanes, tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, rows = kColThreads / lanes;
     const i64 n = ((i64)blockIdx.x * lanes + tx) * V;
     if (n >= p.c.N) return;
-    const f32x2 c2 = pair(p.c.c, p.c.c);
-    f32x2 less[P], scale[P];
-    u32 alive[V > 1 ? 4 : 1];                          // bits of the stored elements of items that are not dead
+    if constexpr (V == 1) {
+        single_delta<DT>(p, n, lo + ty, rows, hi);
+        return;
+    } else {
+        constexpr int U = 4, P = Pairs<DT, V>::P;
+        const f32x2 c2 = pair(p.c.c, p.c.c);
+        f32x2 less[P], scale[P];
+        u32 alive[4];                                  // bits of the stored elements of items that are not dead
 #pragma unroll
-    for (u32& x : alive) x = 0;
+        for (u32& x : alive) x = 0;
 #pragma unroll
-    for (int l = 0; l < P; ++l) {
-        const float4 a = p.item[n + 2 * l], b = V > 1 ? p.item[n + 2 * l + 1] : a;
-        less[l] = pair(-a.x, -b.x);
-        scale[l] = pair(a.y, b.y);
-        if (DT == F32 || V == 1) {
-            alive[V > 1 ? 2 * l : 0] = a.z != 0.f ? 0u : ~0u;
-            if (V > 1) alive[(2 * l + 1) % (V > 1 ? 4 : 1)] = b.z != 0.f ? 0u : ~0u;
-        } else {
-            alive[l % (V > 1 ? 4 : 1)] = (a.z != 0.f ? 0u : 0xffffu) | (b.z != 0.f ? 0u : 0xffff0000u);
-        }
-    }
-    for (int v0 = lo + ty; v0 < hi; v0 += rows * U) {
-        Pairs<DT, V> z[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) if (v0 + u * rows < hi) z[u].load(p.c.z, (i64)(v0 + u * rows) * p.c.z0 + n);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (v0 + u * rows >= hi) break;
-            u32 w[V > 1 ? 4 : 1];
-#pragma unroll
-            for (int l = 0; l < P; ++l) {
-                float x, y;
-                split(mul2(add2(z[u].get(l), less[l]), c2), x, y);
-                const f32x2 g = mul2(scale[l], pair(ex2_approx(x), ex2_approx(y)));
-                if constexpr (V > 1) set2<DT>(w, l, g);
-                else { split(g, x, y); cvt_out<DT, 1, false>(&x, w, SrCtx(), nullptr); }
+        for (int l = 0; l < P; ++l) {
+            const float4 a = p.item[n + 2 * l], b = p.item[n + 2 * l + 1];
+            less[l] = pair(-a.x, -b.x);
+            scale[l] = pair(a.y, b.y);
+            if (DT == F32) {
+                alive[2 * l % 4] = a.z != 0.f ? 0u : ~0u;
+                alive[(2 * l + 1) % 4] = b.z != 0.f ? 0u : ~0u;
+            } else {
+                alive[l % 4] = (a.z != 0.f ? 0u : 0xffffu) | (b.z != 0.f ? 0u : 0xffff0000u);
             }
+        }
+        for (int v0 = lo + ty; v0 < hi; v0 += rows * U) {
+            Pairs<DT, V> z[U];
 #pragma unroll
-            for (int i = 0; i < (V > 1 ? 4 : 1); ++i) w[i] &= alive[i];
-            st_raw<dt_size<DT>::value * V>(reinterpret_cast<char*>(p.c.d) + ((i64)(v0 + u * rows) * p.c.d0 + n) * dt_size<DT>::value, w);
+            for (int u = 0; u < U; ++u) if (v0 + u * rows < hi) z[u].load(p.c.z, (i64)(v0 + u * rows) * p.c.z0 + n);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (v0 + u * rows >= hi) break;
+                u32 w[4];
+#pragma unroll
+                for (int l = 0; l < P; ++l) {
+                    float x, y;
+                    split(mul2(add2(z[u].get(l), less[l]), c2), x, y);
+                    const f32x2 g = mul2(scale[l], pair(ex2_approx(x), ex2_approx(y)));
+                    set2<DT>(w, l, g);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] &= alive[i];
+                st_raw<dt_size<DT>::value * V>(reinterpret_cast<char*>(p.c.d) + ((i64)(v0 + u * rows) * p.c.d0 + n) * dt_size<DT>::value, w);
+            }
         }
     }
 }
@@ -789,12 +846,12 @@ template <bool POLICY, int DT, int V> cudaError_t launch_cols(const CostP& all, 
         const i64 across = (c.N + wide - 1) / wide;
         // shares of the vocabulary: the first kernel's blocks all resident at once, the third's a
         // quarter as long, since nothing has to be joined there
-        const i64 most = ((i64)c.V + rows * 4 - 1) / (rows * 4), room = resident_blocks(cost_cols_stats<DT, V>, kColThreads, 0);
+        const i64 step = rows * (V > 1 ? 4 : (int)kSingle), most = ((i64)c.V + step - 1) / step, room = resident_blocks(cost_cols_stats<DT, V>, kColThreads, 0);
         if (!room) return cudaErrorInvalidConfiguration;
         auto cut = [&](i64 splits) {
             if (splits > most) splits = most;
             if (splits < 1) splits = 1;
-            const i64 step = rows * 4, each = ((i64)c.V + splits - 1) / splits;
+            const i64 each = ((i64)c.V + splits - 1) / splits;
             p.rows = (int)((each + step - 1) / step * step);            // whole steps of all threads
             return (unsigned)(((i64)c.V + p.rows - 1) / p.rows);
         };
@@ -825,7 +882,7 @@ b200_matrix vec(uint64_t ptr, int dt) { b200_matrix m; m.ptr = ptr; m.s0 = 1; m.
 // item that are read, `out` those that are written (cost first).
 int32_t check(const char* where, const b200_matrix* z, const b200_matrix* d, i64 V, i64 N, const b200_matrix* in, int n_in,
               const b200_matrix* out, int n_out) {
-    if (V < 1 || V > 0x7fffffff) return refuse(where, "between 1 and 2^31 - 1 words");
+    if (V < 1 || V > (1 << 30)) return refuse(where, "between 1 and 2^30 words");
     if (N < 0 || N > 0x7fffffff) return refuse(where, "between 0 and 2^31 - 1 items");
     if (!is_float(z->dtype) || (d->ptr && d->dtype != z->dtype))
         return refuse(where, "only f32, f16 and bf16, the same for logits and delta", B200_ERR_UNSUPPORTED);

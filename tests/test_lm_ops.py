@@ -157,6 +157,10 @@ def test_entry_points_refuse_null_and_misaligned(be):
     assert lib.b200_lut_bprop(1 << 22, m, None, far, 8, 8, 4, -1, 1.0, 0.0, 0, 0, 0, None) == -1 and "scratch" in rt.last_error()
     assert lib.b200_distill(m, None, None, m, 0, 1 << 25, 8, 4, 2, 1.0, 0, 0, 0, None) == -1
     assert lib.b200_policy(m, None, 0, 0, 0, 0, 0, 1 << 25, 0, 8, 4, 0.2, 0.2, 0.0, 0, 0, 0, None) == -1
+    wide = rt.Matrix(1 << 40, 4, 1, rt.F32, 0)           # words that would pass 32 bits while a kernel steps over them
+    assert lib.b200_policy(wide, None, 1 << 20, 1 << 21, 0, 1 << 22, 0, 1 << 25, 0, (1 << 30) + 1, 4, 0.2, 0.2, 0.0, 0, 0, 0, None) == -1 \
+        and "2^30 words" in rt.last_error()
+    assert lib.b200_ln_fprop(wide, wide, 0, 0, rt.F32, 0, 0, (1 << 30) + 1, 4, 1e-5, 0, 0, 0, None) == -1 and "2^30" in rt.last_error()
     if rt.device_count() == 0:                       # a good call reports the missing device
         n = C.c_int32(5)
         assert lib.b200_ln_fprop(m, far, 0, 0, rt.F32, 0, 0, 8, 4, 1e-5, 1 << 40, 1 << 30, 0, n) == -2 and n.value == 0
