@@ -695,3 +695,26 @@ def test_costs_many_items(b200, v, n):
     live = [i for i in some if not none[i]]
     want = ref.policy(z[live].T, act[:, live], old[:, live], None, adv[:, live], w[:, live], 0.2, 0.2, 0.0, np.float32)
     compare({"cost": got_cost[:, live], "delta": got[live].T}, want)
+
+
+# whole vectors and not, the gradients' shares per thread, per feature and in the scratch, and split features
+@pytest.mark.parametrize("f,n", [(64, 30001), (301, 4097), (1001, 20001), (5000, 5001), (4500, 6000), (700, 24000), (12572, 47),
+                                 (9000, 130)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: np.dtype(d).name)
+def test_layer_norm_items_next_to_each_other(b200, f, n, dtype):
+    x, gamma, beta, e = ln_inputs(f, n, dtype, np.float32)
+    got = run_ln(b200, x, gamma, beta, e, dtype, np.float32, "cols")
+    compare(got, want_ln(x, gamma, beta, e, got, dtype, np.float32))
+
+
+@pytest.mark.parametrize("v,n", [(9000, 333), (2003, 2001), (2003, 2008), (40, 9001)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: np.dtype(d).name)
+def test_costs_items_next_to_each_other(b200, v, n, dtype):
+    z, ids, top, w = distill_inputs(v, n, 6, dtype)
+    w[0, ::5] = 0
+    compare(run_distill(b200, z, ids, top, w, 1.5, dtype, "cols"), ref.distill(z, ids, top, w, 1.5, dtype))
+    z, act, old, new_ref, adv, w = policy_inputs(v, n, dtype)
+    act[0, ::7] = -1
+    for inplace in (False, True):
+        got = run_policy(b200, z, act, old, new_ref, adv, w, dtype, "cols", inplace=inplace)
+        compare(got, ref.policy(z, act, old, new_ref, adv, w, 0.2, 0.28, 0.05, dtype))
