@@ -445,16 +445,18 @@ template <bool BACK> cudaError_t launch_type(const LnP& p, bool mis, float* part
 // A block takes a stripe of neighbouring items, `lanes` threads side by side and its other threads
 // down the features, so every access is a run of 32 to 128 bytes of a feature's row.  With enough
 // stripes for the machine a block sees all features of its items: it copies the stripe to shared
-// memory (HELD; every thread its own vectors), so HBM is read once, or, where that is too small,
-// walks over it again.  With few stripes the features are split over blocks as well, and a second
+// memory (HELD; every thread its own vectors), so HBM is read once, and puts the next stripe's
+// vectors into the places as it reads them for the last time; where the memory is too small, it
+// walks over the stripe again.  With few stripes the features are split over blocks as well, and a second
 // kernel joins their sums: of a share of n_i features its mean m_i and centred squares q_i, which
 // give the item's mean sum n_i m_i / F and squares sum q_i + n_i (m_i - mean)^2.
 //
 // What bounds them: the instructions of an element (conversion, the sums, the result), with a
-// stripe's three phases in turn; the loops have constant distances for that (76 -> 69 us, backwards
-// 179 -> 152 us at 1024 x 65536 bf16, 60 % and 41 % of the copy rate, and 21 us backwards at
-// 1001 x 4096 f32).  Rows that are not whole 16-byte vectors go item by item: 82 and 199 us at
-// 1001 x 32767 bf16, four items a thread, against 103 and 317 us with one.
+// stripe's phases in turn; the loops have constant distances for that (backwards 179 -> 152 us at
+// 1024 x 65536 bf16) and the next stripe is under way meanwhile (152 -> 134 us; forwards 70 us, 59 %
+// of the copy rate against 47 %; backwards at 1001 x 4096 f32 21 us).  Rows that are not whole
+// 16-byte vectors go item by item: 81 and 199 us at 1001 x 32767 bf16, four items a thread, against
+// 103 and 317 us with one.
 //
 // A thread's place in its stripe: its V items, next to each other from n on, or, where the rows do
 // not consist of whole 16-byte vectors (V = -4), four of them `lanes` apart, of which `count` exist;
@@ -566,6 +568,10 @@ template <int DT> DEV void hold(const u32* to, u64 base, i64 pitch, const Place&
     u32 at = (u32)__cvta_generic_to_shared(to + threadIdx.x * 4);
     for (int f = q.ty; f < q.F; f += q.rows, at += kColsT * 16) copy16(at, base + (u64)((f * pitch + q.n) * dt_size<DT>::value));
 }
+// The place of one such vector, read for the last time, filled with the next stripe's.
+template <int DT> DEV void refill(const u32* to, int k, u64 base, i64 at) {
+    copy16((u32)__cvta_generic_to_shared(to + (k * kColsT + threadIdx.x) * 4), base + (u64)(at * dt_size<DT>::value));
+}
 template <int DT, int V, bool HELD> DEV void look(Items<DT, V>& x, const u32* held, int k, u64 base, i64 at, const Place& q) {
     if constexpr (HELD) x.load(held + (k * kColsT + threadIdx.x) * 4);
     else x.load(base, at, q);
@@ -611,7 +617,8 @@ template <int P> DEV void to_rstd(f32x2 (&v)[P], float inv, float eps) {
         v[l] = pair(1.f / sqrtf(x * inv + eps), 1.f / sqrtf(y * inv + eps));
     }
 }
-template <int DT, int V, bool HELD> DEV void normalise(const LnP& p, const Place& q, const u32* held, int f0, int f1, const f32x2* mean, const f32x2* rstd) {
+template <int DT, int V, bool HELD> DEV void normalise(const LnP& p, const Place& q, const u32* held, int f0, int f1, const f32x2* mean, const f32x2* rstd,
+                                                       i64 next = -1) {
     constexpr int P = Items<DT, V>::P;
     f32x2 less[P];
 #pragma unroll
@@ -621,6 +628,7 @@ template <int DT, int V, bool HELD> DEV void normalise(const LnP& p, const Place
         const f32x2 g = both_of(p.gamma ? ld_any(p.gamma, f, p.pdt) : 1.f), b = both_of(p.beta ? ld_any(p.beta, f, p.pdt) : 0.f);
         Items<DT, V> x;
         look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n, q);
+        if constexpr (HELD) if (next >= 0) refill<DT>(held, k, p.x, f * p.x0 + next);
 #pragma unroll
         for (int l = 0; l < P; ++l) x.set(l, fma2(mul2(add2(x.get(l), less[l]), rstd[l]), g, b));
         x.store(p.out, f * p.o0 + q.n, q);
@@ -629,24 +637,30 @@ template <int DT, int V, bool HELD> DEV void normalise(const LnP& p, const Place
 
 // (LANES: the stripe's width where it is known to the compiler, or 0)
 template <int DT, int V, bool HELD, int LANES>
-__global__ void __launch_bounds__(kColsT) ln_fprop_cols(const __grid_constant__ LnP p, int lanes) {
+__global__ void __launch_bounds__(kColsT, 2) ln_fprop_cols(const __grid_constant__ LnP p, int lanes, i64 stripes) {
     extern __shared__ __align__(16) u32 held[];
     __shared__ __align__(16) float s[kStripeFloats];
-    const Place q = place<V>(blockIdx.x, LANES ? LANES : lanes, p.N, p.F);
+    Place q = place<V>(blockIdx.x, LANES ? LANES : lanes, p.N, p.F);
     if constexpr (HELD) {
         if (q.in) hold<DT>(held, p.x, p.x0, q);
         copy_commit();
-        copy_wait<0>();
     }
-    f32x2 mean[Items<DT, V>::P], rstd[Items<DT, V>::P];
-    moments<DT, V, HELD>(p, q, held, 0, q.F, s, mean, rstd);
-    to_rstd(rstd, 1.f / (float)q.F, p.eps);
-    if (!q.in) return;
-    if (q.ty == 0) {
-        if (p.mean) put_items<V>(p.mean, q, mean);
-        if (p.rstd) put_items<V>(p.rstd, q, rstd);
+    for (i64 stripe = blockIdx.x; stripe < stripes; stripe += gridDim.x) {
+        const Place after = place<V>(stripe + gridDim.x, LANES ? LANES : lanes, p.N, p.F);
+        if constexpr (HELD) copy_wait<0>();
+        f32x2 mean[Items<DT, V>::P], rstd[Items<DT, V>::P];
+        moments<DT, V, HELD>(p, q, held, 0, q.F, s, mean, rstd);
+        to_rstd(rstd, 1.f / (float)q.F, p.eps);
+        if (q.in) {
+            if (q.ty == 0) {
+                if (p.mean) put_items<V>(p.mean, q, mean);
+                if (p.rstd) put_items<V>(p.rstd, q, rstd);
+            }
+            normalise<DT, V, HELD>(p, q, held, 0, q.F, mean, rstd, after.in ? after.n : -1);
+        }
+        if constexpr (HELD) copy_commit();
+        q = after;
     }
-    normalise<DT, V, HELD>(p, q, held, 0, q.F, mean, rstd);
 }
 
 // part[split][0][N]: mean, part[split][1][N]: centred squares of a share of `per` features
@@ -748,7 +762,7 @@ template <int DT, int V, bool HELD> DEV void error_sums(const LnP& p, const Plac
     stripe_sum<V>(b, s, q.lanes);
 }
 template <int DT, int V, bool HELD> DEV void put_delta(const LnP& p, const Place& q, const u32* held, const u32* held_e, int f0, int f1,
-                                                       const f32x2* mean, const f32x2* rstd, const f32x2* a, const f32x2* b) {
+                                                       const f32x2* mean, const f32x2* rstd, const f32x2* a, const f32x2* b, i64 next = -1) {
     constexpr int P = Items<DT, V>::P;
     const f32x2 inv = both_of(-1.f / (float)q.F);
     f32x2 less[P], ma[P], mb[P];
@@ -760,6 +774,12 @@ template <int DT, int V, bool HELD> DEV void put_delta(const LnP& p, const Place
         Items<DT, V> x, e;
         look<DT, V, HELD>(x, held, k, p.x, f * p.x0 + q.n, q);
         look<DT, V, HELD>(e, held_e, k, p.e, f * p.e0 + q.n, q);
+        if constexpr (HELD) {
+            if (next >= 0) {
+                refill<DT>(held, k, p.x, f * p.x0 + next);
+                refill<DT>(held_e, k, p.e, f * p.e0 + next);
+            }
+        }
 #pragma unroll
         for (int l = 0; l < P; ++l) {
             const f32x2 h = mul2(add2(x.get(l), less[l]), rstd[l]);
@@ -783,15 +803,16 @@ __global__ void __launch_bounds__(kColsT, 2) ln_bprop_cols(const __grid_constant
     u32* behind = mem + (HELD ? 2 * each * kColsT * 4 : 0);
     f32x2* own = own_sums ? reinterpret_cast<f32x2*>(behind) : nullptr;
     float* acc = acc_held ? reinterpret_cast<float*>(behind) : mine;
-    for (i64 stripe = blockIdx.x; stripe < stripes; stripe += gridDim.x) {
-        const Place q = place<V>(stripe, lanes, p.N, p.F);
-        if constexpr (HELD) {
-            if (q.in) {
-                hold<DT>(held, p.x, p.x0, q);
-                hold<DT>(held_e, p.e, p.e0, q);
-            }
-            copy_commit();
+    Place q = place<V>(blockIdx.x, lanes, p.N, p.F);
+    if constexpr (HELD) {
+        if (q.in) {
+            hold<DT>(held, p.x, p.x0, q);
+            hold<DT>(held_e, p.e, p.e0, q);
         }
+        copy_commit();
+    }
+    for (i64 stripe = blockIdx.x; stripe < stripes; stripe += gridDim.x) {
+        const Place after = place<V>(stripe + gridDim.x, lanes, p.N, p.F);
         f32x2 mean[P], rstd[P], a[P], b[P];
 #pragma unroll
         for (int l = 0; l < P; ++l) mean[l] = rstd[l] = 0;
@@ -801,7 +822,9 @@ __global__ void __launch_bounds__(kColsT, 2) ln_bprop_cols(const __grid_constant
         }
         if constexpr (HELD) copy_wait<0>();
         error_sums<DT, V, HELD>(p, q, held, held_e, 0, F, s, mean, rstd, a, b, acc, own, stripe != blockIdx.x);
-        if (q.in) put_delta<DT, V, HELD>(p, q, held, held_e, 0, F, mean, rstd, a, b);
+        if (q.in) put_delta<DT, V, HELD>(p, q, held, held_e, 0, F, mean, rstd, a, b, after.in ? after.n : -1);
+        if constexpr (HELD) copy_commit();
+        q = after;
     }
     if (!own && !acc_held) return;
     __syncthreads();
@@ -932,8 +955,9 @@ template <int DT, int V, bool HELD, int LANES> cudaError_t launch_cols_back(cons
 }
 template <int DT, int V, bool HELD, int LANES> cudaError_t launch_cols_forward(const LnP& p, const Cols& c, cudaStream_t s) {
     auto kernel = ln_fprop_cols<DT, V, HELD, LANES>;
-    if (!resident_blocks(kernel, kColsT, c.held)) return cudaErrorInvalidConfiguration;
-    kernel<<<(unsigned)c.stripes, kColsT, c.held, s>>>(p, c.lanes);
+    const i64 most = resident_blocks(kernel, kColsT, c.held);
+    if (!most) return cudaErrorInvalidConfiguration;
+    kernel<<<(unsigned)(c.stripes < most ? c.stripes : most), kColsT, c.held, s>>>(p, c.lanes, c.stripes);
     return cudaGetLastError();
 }
 template <int DT, int V, bool BACK, bool HELD, int LANES> cudaError_t launch_cols_one(const LnP& p, const Cols& c, float* part, int* parts, cudaStream_t s) {
