@@ -223,15 +223,36 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_fprop_rows(const __grid_constan
     }
 }
 
-// One barrier per item, for both sums at once.
-// part[block][0][F]: the block's share of grad_gamma, part[block][1][F]: of grad_beta.
-template <int DT, int NV, int RING, bool MIS, int MAXT, int MINB>
+// Two sums over the threads of a cluster of two blocks, known to all of them: each block's are put
+// into both blocks' shared memory by the first warp, which alone has to wait at the barrier for its
+// earlier stores.  The halves of s alternate as for group_sum2.
+DEV float2 pair_sum2(float a, float b, float2* s, float2* both_blocks, int& turn, u32 rank) {
+    const float2 v = group_sum2(a, b, s, turn, blockDim.x, 1);
+    float2* slot = both_blocks + turn * 2;
+    if (threadIdx.x < 2) {
+        dsmem_st(&slot[rank].x, threadIdx.x, __float_as_uint(v.x));
+        dsmem_st(&slot[rank].y, threadIdx.x, __float_as_uint(v.y));
+    }
+    cluster_barrier_warp0_releases();
+    return make_float2(slot[0].x + slot[1].x, slot[0].y + slot[1].y);
+}
+
+// One barrier per item, for both sums at once.  Items too wide for a block's registers are a pair of
+// blocks' (PAIR: a cluster of 2), which exchange their sums behind it.
+// part[block][0][F]: the block's share of grad_gamma, part[block][1][F]: of grad_beta; one for a pair.
+//
+// What bounds it: instructions, at the few warps that fit beside the gradients' sums.  4096 x 32768
+// bf16 takes 152 us, 82 % of the copy rate, 1024 x 65536 76, 16384 x 8192 in pairs 255, where one
+// block of 1024 threads, which spills, took 409.
+template <int DT, int NV, int RING, bool MIS, int MAXT, int MINB, bool PAIR>
 __global__ void __launch_bounds__(MAXT, MINB) ln_bprop_rows(const __grid_constant__ LnP p, float* part, int T) {
     constexpr int V = 16 / dt_size<DT>::value, W = 4;
     extern __shared__ __align__(16) u32 ring[];        // [RING][2][NV][blockDim.x][W]
-    __shared__ float2 s[64];
-    const int F = (int)p.F, group = threadIdx.x / T, me = threadIdx.x % T, groups = blockDim.x / T;
-    const i64 step = (i64)gridDim.x * groups, first = (i64)blockIdx.x * groups + group;
+    __shared__ float2 s[64], both_blocks[4];
+    const int rank = PAIR ? (int)cluster_rank() : 0;   // T: threads per item, of a pair both blocks'
+    const int F = (int)p.F, group = PAIR ? 0 : threadIdx.x / T, me = PAIR ? rank * (T / 2) + threadIdx.x : threadIdx.x % T;
+    const int groups = PAIR ? 1 : blockDim.x / T, own = PAIR ? blockIdx.x / 2 : blockIdx.x;
+    const i64 step = (i64)(PAIR ? gridDim.x / 2 : gridDim.x) * groups, first = (i64)own * groups + group;
     int mis = 0;
     if constexpr (MIS) mis = (int)((p.x / dt_size<DT>::value + (u64)(first * p.x1)) % V);
     const u32 mine = (u32)__cvta_generic_to_shared(ring) + threadIdx.x * 16, slot = blockDim.x * 16;
@@ -249,6 +270,7 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bprop_rows(const __grid_constan
     };
 #pragma unroll
     for (int k = 0; k < RING - 1; ++k) fetch(first + k * step, k);
+    if constexpr (PAIR) cluster_barrier();             // the other block is there
     f32x2 gamma[NV][V / 2], gg[NV][V / 2], gb[NV][V / 2];
     load_params<V, NV>(p.gamma, p.pdt, 1.f, me, T, mis, F, gamma);
 #pragma unroll
@@ -286,7 +308,9 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bprop_rows(const __grid_constan
                 b2 = fma2(g[j][k], h[j][k], b2);
             }
         }
-        const float2 ab = group_sum2(both(a2), both(b2), s, turn, T, 1);
+        float2 ab;
+        if constexpr (PAIR) ab = pair_sum2(both(a2), both(b2), s, both_blocks, turn, rank);
+        else ab = group_sum2(both(a2), both(b2), s, turn, T, 1);
         const f32x2 a = pair(-ab.x * inv, -ab.x * inv), b = pair(-ab.y * inv, -ab.y * inv);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -302,7 +326,7 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bprop_rows(const __grid_constan
         rstd = rstd_next;
     }
     if (!part) return;
-    if (T == 32) {
+    if (!PAIR && T == 32) {
         // the warps of a block one after the other, where the ring was: all copies have been read
         float* acc = reinterpret_cast<float*>(ring);   // [2][F], F <= 32 NV V
         for (int g = 0; g < groups; ++g) {
@@ -328,7 +352,7 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bprop_rows(const __grid_constan
         for (int f = threadIdx.x; f < 2 * F; f += blockDim.x) part[(i64)blockIdx.x * 2 * F + f] = acc[f];
         return;
     }
-    float* to = part + (i64)blockIdx.x * 2 * F;
+    float* to = part + (i64)own * 2 * F;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -392,13 +416,32 @@ inline i64 most_parts(i64 F) {
     return fit > 2048 ? 2048 : fit < 8 ? 8 : fit;
 }
 
+// Backwards, wide items: a pair of blocks of T threads per item.
+template <int DT, int NV, int RING, bool MIS, int MAXT>
+cudaError_t launch_pairs(const LnP& p, int T, float* part, int* parts, cudaStream_t s) {
+    auto kernel = ln_bprop_rows<DT, NV, RING, MIS, MAXT, 1, true>;
+    const int smem = RING * 2 * NV * T * 16;
+    i64 grid = resident_blocks(kernel, T, smem) / 2;
+    if (!grid) return cudaErrorInvalidConfiguration;
+    if (grid > p.N) grid = p.N;
+    if (part && grid > most_parts(p.F)) grid = most_parts(p.F);
+    if (MIS) grid = grid < 8 ? 8 : grid / 8 * 8;
+    *parts = (int)grid;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)grid * 2); c.blockDim = dim3(T); c.dynamicSmemBytes = smem; c.stream = s;
+    cudaLaunchAttribute a;
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = 2; a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    c.attrs = &a; c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, p, part, 2 * T);
+}
 // One kernel of either direction: T threads per item; a block is one group, or 8 warps that are
 // groups of their own (4 where there are few items).  `parts`: the blocks, whose shares lie in `part`.
 template <int DT, int NV, int RING, bool MIS, int MAXT, int MINB, bool BACK>
 cudaError_t launch_rows(const LnP& p, int T, float* part, int* parts, cudaStream_t s) {
     const int groups = T > 32 ? 1 : p.N < 148 * 8 ? 4 : 8, smem = RING * (BACK ? 2 : 1) * NV * T * groups * 16;
     i64 most;
-    if constexpr (BACK) most = resident_blocks(ln_bprop_rows<DT, NV, RING, MIS, MAXT, MINB>, T * groups, smem);
+    if constexpr (BACK) most = resident_blocks(ln_bprop_rows<DT, NV, RING, MIS, MAXT, MINB, false>, T * groups, smem);
     else most = resident_blocks(ln_fprop_rows<DT, NV, RING, MIS, MAXT, MINB>, T * groups, smem);
     if (!most) return cudaErrorInvalidConfiguration;
     i64 grid = (p.N + groups - 1) / groups;
@@ -407,7 +450,7 @@ cudaError_t launch_rows(const LnP& p, int T, float* part, int* parts, cudaStream
     if (MIS) grid = grid < 8 ? 8 : grid / 8 * 8;
     if constexpr (BACK) {
         *parts = (int)grid;
-        ln_bprop_rows<DT, NV, RING, MIS, MAXT, MINB><<<(unsigned)grid, T * groups, smem, s>>>(p, part, T);
+        ln_bprop_rows<DT, NV, RING, MIS, MAXT, MINB, false><<<(unsigned)grid, T * groups, smem, s>>>(p, part, T);
     } else {
         ln_fprop_rows<DT, NV, RING, MIS, MAXT, MINB><<<(unsigned)grid, T * groups, smem, s>>>(p, T);
     }
@@ -429,7 +472,7 @@ template <int DT, bool MIS, bool BACK> cudaError_t launch_width(const LnP& p, fl
         if (width(1) <= 64) return launch_rows<DT, 1, 3, MIS, 512, 1, BACK>(p, width(1), part, parts, s);
         if (width(2) <= 512) return launch_rows<DT, 2, 3, MIS, 512, 1, BACK>(p, width(2), part, parts, s);
         if constexpr (V == 4) if (width(4) <= 512) return launch_rows<DT, 4, 3, MIS, 512, 1, BACK>(p, width(4), part, parts, s);
-        return launch_rows<DT, 16 / V, 1, MIS, 1024, 1, BACK>(p, width(16 / V), part, parts, s);
+        return launch_pairs<DT, 16 / V, 3, MIS, 512>(p, width(32 / V), part, parts, s);
     }
 }
 template <bool BACK> cudaError_t launch_type(const LnP& p, bool mis, float* part, int* parts, cudaStream_t s) {

@@ -718,3 +718,13 @@ def test_costs_items_next_to_each_other(b200, v, n, dtype):
     for inplace in (False, True):
         got = run_policy(b200, z, act, old, new_ref, adv, w, dtype, "cols", inplace=inplace)
         compare(got, ref.policy(z, act, old, new_ref, adv, w, 0.2, 0.28, 0.05, dtype))
+
+
+@pytest.mark.parametrize("f,n", [(16384, 170), (9001, 333), (12000, 75), (16377, 90)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: np.dtype(d).name)
+@pytest.mark.parametrize("inplace", [False, True])
+def test_layer_norm_wide_items(b200, f, n, dtype, inplace):
+    """More wide items than pairs of blocks are resident, at and off 16-byte boundaries."""
+    x, gamma, beta, e = ln_inputs(f, n, dtype, np.float32)
+    got = run_ln(b200, x, gamma, beta, e, dtype, np.float32, "rows", inplace=inplace)
+    compare(got, want_ln(x, gamma, beta, e, got, dtype, np.float32))
