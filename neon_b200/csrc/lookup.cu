@@ -47,43 +47,57 @@ __global__ void __launch_bounds__(256) lut_fprop_any(const __grid_constant__ Lut
 // Features of a result next to each other, and of the table: 16-byte vectors of the result, each from
 // one or two vectors of the table's row (which may lie differently to the boundaries).  T threads
 // per position, four positions at a time, so that four independent gathers are under way per thread.
+// Bound by HBM, most of all by the writes: 2048 x 65536 bf16 takes 63 us, 83 % of the copy rate.  Off
+// the boundaries, by instructions: 2047 x 65536 takes 96 us, 134 with branches between the gathers.
 template <int DT, bool MIS>
 __global__ void __launch_bounds__(256) lut_fprop_rows(const __grid_constant__ LutP p, int T) {
     constexpr int V = 16 / dt_size<DT>::value, U = 4;
-    const int F = (int)p.F, me = threadIdx.x % T, per = 256 / T;
-    const i64 n0 = ((i64)blockIdx.x * per + threadIdx.x / T) * U;
-    if (threadIdx.x >= per * T) return;
+    const int F = (int)p.F, me = threadIdx.x % T;
+    const i64 n0 = ((i64)blockIdx.x * (blockDim.x / T) + threadIdx.x / T) * U;
     int id[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) id[u] = n0 + u < p.N ? reinterpret_cast<const int*>(p.ids)[n0 + u] : -1;
     const f32x2 scale = pair(p.scale, p.scale);
+    int mis[U];                                         // of the results' rows
+#pragma unroll
+    for (int u = 0; u < U; ++u) mis[u] = MIS ? (int)((p.out / dt_size<DT>::value + (u64)((n0 + u) * p.o1)) % V) : 0;
     for (int k = me; k * V < F + (MIS ? V - 1 : 0); k += T) {
-        u32 w[U][4];
+        u32 w[U][MIS ? 8 : 4];
         int f[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            f[u] = k * V;
-            if constexpr (MIS) f[u] -= (int)((p.out / dt_size<DT>::value + (u64)((n0 + u) * p.o1)) % V);
-            w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;
-            if (id[u] < 0 || id[u] >= p.V || f[u] >= F) continue;
-            if constexpr (MIS) get_part<DT, V>(p.w, id[u] * p.w0, f[u], F, w[u]);
-            else ld_w<DT, V, true>(p.w, id[u] * p.w0 + f[u], w[u]);
+            f[u] = k * V - mis[u];
+            if constexpr (MIS) {                        // (no branches: the table has a row 0)
+                const bool in = id[u] >= 0 && id[u] < p.V;
+                get_two<DT, V>(p.w, in ? id[u] * p.w0 : 0, f[u] < F ? f[u] : F - 1, F, w[u]);
+            } else if (id[u] >= 0 && id[u] < p.V) {
+                ld_w<DT, V, true>(p.w, id[u] * p.w0 + f[u], w[u]);
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (n0 + u >= p.N) break;
+            if (n0 + u >= p.N || f[u] >= F) continue;
             if (id[u] >= 0 && id[u] < p.V) {
+                if constexpr (MIS) {
+                    u32 x[4];
+                    join_two(w[u], off_boundary<DT>(p.w, id[u] * p.w0, f[u]), x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[u][i] = x[i];
+                }
 #pragma unroll
                 for (int i = 0; i < V / 2; ++i) set2<DT>(w[u], i, mul2(get2<DT>(w[u], i), scale));
+            } else {
+                w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;
             }
-            if constexpr (MIS) { if (f[u] < F) put_part<DT, V>(p.out, (n0 + u) * p.o1, f[u], F, w[u]); }
+            if constexpr (MIS) put_part<DT, V>(p.out, (n0 + u) * p.o1, f[u], F, w[u]);
             else st_raw<16>(reinterpret_cast<char*>(p.out) + ((n0 + u) * p.o1 + f[u]) * dt_size<DT>::value, w[u]);
         }
     }
 }
 
 // Positions of the result next to each other (neon's order): a tile of 64 positions x 64 features
-// is gathered along the features and written along the positions, turned in shared memory.
+// is gathered along the features and written along the positions, turned in shared memory.  2048 x
+// 32768 bf16 takes 60 us, 46 % of the copy rate, bound by the way through shared memory.
 template <int DT>
 __global__ void __launch_bounds__(256) lut_fprop_cols(const __grid_constant__ LutP p, int wide) {
     constexpr int S = dt_size<DT>::value, V = 16 / S, P = 64 * S / 4 + 1;      // words per feature, one spare
@@ -135,10 +149,13 @@ template <int DT> cudaError_t launch_fprop(const LutP& p, cudaStream_t s) {
     if (table && (p.o0 == 1 || p.F == 1)) {
         const bool mis = !(aligned && p.out % 16 == 0 && p.o1 % V == 0);
         const i64 nvec = (p.F + (mis ? V - 1 : 0) + V - 1) / V;
-        const int T = nvec >= 256 ? 256 : nvec <= 32 ? 32 : (int)(nvec + 31) / 32 * 32, per = 256 / T * 4;
-        const unsigned grid = (unsigned)((p.N + per - 1) / per);
-        if (mis) lut_fprop_rows<DT, true><<<grid, 256, 0, s>>>(p, T);
-        else lut_fprop_rows<DT, false><<<grid, 256, 0, s>>>(p, T);
+        int T = 256;                                    // the most threads that leave the fewest without a vector
+        for (int t = 224; t >= 32; t -= 32)
+            if ((nvec + t - 1) / t * t < (nvec + T - 1) / T * T) T = t;
+        const int per = 256 / T;
+        const unsigned grid = (unsigned)((p.N + per * 4 - 1) / (per * 4));
+        if (mis) lut_fprop_rows<DT, true><<<grid, per * T, 0, s>>>(p, T);
+        else lut_fprop_rows<DT, false><<<grid, per * T, 0, s>>>(p, T);
     } else if (p.o1 == 1 || p.N == 1) {
         lut_fprop_cols<DT><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)((p.F + 63) / 64)), 256, 0, s>>>(p, table && aligned);
     } else {
@@ -336,6 +353,25 @@ template <int V> DEV void put_dw(const SumP& p, i64 v, int f, const float* sum) 
     for (int i = 0; i < V; ++i) if (f + i < p.F) st_any(p.w, at + i * p.w1, p.wdt, r[i]);
 }
 
+// The same by a warp, whose lanes hold V features each from f0 on of rows that need not consist of
+// whole vectors: through shared memory, so that neighbouring lanes write neighbouring elements.
+template <int V> DEV void put_dw_warp(const SumP& p, i64 v, int f0, const float* sum, float* buf) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < V; ++i) buf[lane * (V + 1) + i] = sum[i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int k = i * 32 + lane;
+        if (f0 + k >= p.F) break;
+        const i64 at = v * p.w0 + f0 + k;
+        float r = p.alpha * buf[k / V * (V + 1) + k % V];
+        if (p.beta != 0.f) r += p.beta * ld_any(p.w, at, p.wdt);
+        st_any(p.w, at, p.wdt, r);
+    }
+    __syncwarp();
+}
+
 // Clears (or scales) the rows of words that have no position: a warp takes 32 words and a part of
 // their features at a time.  Rows that start off a 16-byte boundary are cleared in whole vectors too.
 template <int DT> DEV void clear_part(u64 base, i64 row, int from, int to) {
@@ -366,19 +402,25 @@ DEV void fill_words(const SumP& p, i64 warp, i64 warps) {
 }
 
 // The first `sum_blocks` blocks: a thread adds up V features of the places of one chunk, in their
-// order; neighbouring threads take neighbouring features.  Eight places are under way at a time, and
-// the numbers of the next eight are read meanwhile.  V > 1: the error's features are next to each
-// other; `aligned`: its positions start on 16-byte boundaries.
+// order; neighbouring threads take neighbouring features.  Eight places are under way at a time (four
+// if MIS), and the numbers of the next ones are read meanwhile.  V > 1: the error's features are next
+// to each other; MIS: its positions need not start on 16-byte boundaries.
 // The other blocks see to the words without a position.
-template <int DT, int V>
-__global__ void __launch_bounds__(256) lut_chunks(const __grid_constant__ SumP p, i64 chunks, int nvec, int aligned, unsigned sum_blocks) {
+//
+// What bounds the gradient: latency, at the two blocks per SM that eight vectors per thread leave, and
+// the sort's launches.  50257 x 1024 f32 from 131072 positions of bf16 takes 126 us, of them 40 for the
+// sort, 1.7 times the copy rate's; 50257 x 1023 from 65536 positions 128, 190 with branches between
+// the loads and rows written element by element.
+template <int DT, int V, bool MIS>
+__global__ void __launch_bounds__(256) lut_chunks(const __grid_constant__ SumP p, i64 chunks, int nvec, int turned, unsigned sum_blocks) {
     grid_enter();
     const int F = (int)p.F;
     if (blockIdx.x >= sum_blocks) {
         fill_words(p, (i64)(blockIdx.x - sum_blocks) * 8 + (threadIdx.x >> 5), (i64)(gridDim.x - sum_blocks) * 8);
         return;
     }
-    constexpr int U = 8, W = V == 1 ? 1 : 4;
+    constexpr int U = MIS ? 4 : 8, W = V == 1 ? 1 : MIS ? 8 : 4;
+    __shared__ float turn[V > 1 ? 8 * 32 * (V + 1) : 1];
     const i64 id = (i64)blockIdx.x * 256 + threadIdx.x, chunk = id / nvec;
     if (chunk >= chunks) return;
     const int f = (int)(id - chunk * nvec) * V;
@@ -394,26 +436,37 @@ __global__ void __launch_bounds__(256) lut_chunks(const __grid_constant__ SumP p
     bool from_before = lo > 0 && keys[-1] == v;
     const bool goes_on = lo + many < used && keys[many] == keys[many - 1];      // the last word of the chunk
 #pragma unroll
-    for (int u = 0; u < U; ++u) if (u < many) { key[u] = keys[u]; pos[u] = poss[u]; }
+    for (int u = 0; u < U; ++u) if (MIS || u < many) { const int i = MIS ? min(u, many - 1) : u; key[u] = keys[i]; pos[u] = poss[i]; }
     for (int i0 = 0; i0 < many; i0 += U) {
         u32 w[U][W];
-        int now[U];
+        int now[U], off[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             now[u] = key[u];
-            if (i0 + u >= many) continue;
             const i64 at = pos[u] * p.e1;
+            if constexpr (MIS) {                       // (no branches)
+                off[u] = off_boundary<DT>(p.e, at, f);
+                get_two<DT, V>(p.e, at, f < F ? f : F - 1, F, w[u]);
+                continue;
+            }
+            if (i0 + u >= many || f >= F) continue;
             if constexpr (V == 1) ld_w<DT, 1, true>(p.e, at + f * p.e0, w[u]);
-            else if (aligned) ld_w<DT, V, true>(p.e, at + f, w[u]);
-            else get_part<DT, V>(p.e, at, f, F, w[u]);
+            else ld_w<DT, V, true>(p.e, at + f, w[u]);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) if (i0 + U + u < many) { key[u] = keys[i0 + U + u]; pos[u] = poss[i0 + U + u]; }
+        for (int u = 0; u < U; ++u)
+            if (MIS || i0 + U + u < many) { const int i = MIS ? min(i0 + U + u, many - 1) : i0 + U + u; key[u] = keys[i]; pos[u] = poss[i]; }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (i0 + u >= many) break;
             float e[V];
-            cvt_in<DT, V>(w[u], e);
+            if constexpr (MIS) {
+                u32 x[4];
+                join_two(w[u], off[u], x);
+                cvt_in<DT, V>(x, e);
+            } else {
+                cvt_in<DT, V>(w[u], e);
+            }
 #pragma unroll
             for (int i = 0; i < V; ++i) sum[i] += e[i];
             const bool last = i0 + u + 1 == many;
@@ -423,6 +476,8 @@ __global__ void __launch_bounds__(256) lut_chunks(const __grid_constant__ SumP p
                 float* to = p.part + (chunk * 2 + (from_before ? 0 : 1)) * F + f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) if (f + i < F) to[i] = sum[i];
+            } else if (V > 1 && turned) {
+                put_dw_warp<V>(p, v, f - (int)(threadIdx.x & 31) * V, sum, turn + (threadIdx.x >> 5) * 32 * (V + 1));
             } else {
                 put_dw<V>(p, v, f, sum);
             }
@@ -505,20 +560,26 @@ __global__ void __launch_bounds__(256) lut_cross(const __grid_constant__ SumP p,
     }
 }
 
-template <int DT, int V> cudaError_t launch_chunks(SumP p, i64 chunks, bool aligned, cudaStream_t s) {
-    const i64 nvec = (p.F + V - 1) / V, sums = (chunks * nvec + 255) / 256;
+template <int DT, int V, bool MIS> cudaError_t launch_chunks(SumP p, i64 chunks, cudaStream_t s) {
+    // rows of dW that are not whole vectors are written by whole warps, if not too many lanes are
+    // left without a feature then (50257 x 1023 f32, 65536 positions of bf16: 128 us, else 190)
+    i64 nvec = (p.F + V - 1) / V;
+    const bool turned = V > 1 && !p.wide && p.w1 == 1 && (nvec + 31) / 32 * 32 * 2 <= nvec * 3;
+    if (turned) nvec = (nvec + 31) / 32 * 32;
+    const i64 sums = (chunks * nvec + 255) / 256;
     // rows of few words are cut, down to 512 features, so that there is a warp for every 16 SM slots
     const i64 groups = ((i64)p.V + 31) / 32;
     p.parts = (int)std::min<i64>((148 * 32 + groups - 1) / groups, (p.F + 511) / 512);
     i64 fill = p.beta == 1.f ? 0 : (groups * p.parts + 7) / 8;
     if (fill > 148 * 16) fill = 148 * 16;
     if (!(sums + fill)) return cudaSuccess;
-    return launch_dependent(lut_chunks<DT, V>, dim3((unsigned)(sums + fill)), 256, 0, s, p, chunks, (int)nvec, (int)aligned, (unsigned)sums);
+    return launch_dependent(lut_chunks<DT, V, MIS>, dim3((unsigned)(sums + fill)), 256, 0, s, p, chunks, (int)nvec, (int)turned, (unsigned)sums);
 }
 template <int DT> cudaError_t launch_sums(const SumP& p, i64 chunks, cudaStream_t s) {
     constexpr int V = 16 / dt_size<DT>::value;
-    if (p.e0 != 1 && p.F != 1) return launch_chunks<DT, 1>(p, chunks, false, s);
-    return launch_chunks<DT, V>(p, chunks, p.e % 16 == 0 && p.e1 % V == 0 && p.F % V == 0, s);
+    if (p.e0 != 1 && p.F != 1) return launch_chunks<DT, 1, false>(p, chunks, s);
+    if (p.e % 16 == 0 && p.e1 % V == 0 && p.F % V == 0) return launch_chunks<DT, V, false>(p, chunks, s);
+    return launch_chunks<DT, V, true>(p, chunks, s);
 }
 
 // Where the pieces of the gradient's scratch lie.

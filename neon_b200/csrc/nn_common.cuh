@@ -150,29 +150,30 @@ template <int DT, int V> DEV void put_part(u64 base, i64 item, int f, int F, con
     }
 }
 
-// V elements from f on of an item that starts anywhere: one aligned vector, or two and a shift.
-// Only 16-byte vectors that hold an element of [0, F) are read; other elements come out undefined.
-template <int DT, int V> DEV void get_part(u64 base, i64 item, int f, int F, u32* w) {
+// V elements from f on, f < F, of an item that starts anywhere: the one or two aligned vectors that
+// hold them, in two steps so that several can be under way.  Only 16-byte vectors that hold an element
+// of [0, F) are read, one of them twice where the other holds none; other elements come out undefined.
+template <int DT, int V> DEV void get_two(u64 base, i64 item, int f, int F, u32* x) {
     constexpr int S = dt_size<DT>::value;
     const u64 at = base + (u64)((item + f) * S);
     const int m = (int)(at & 15u) / S;                  // elements behind a boundary
-    const char* from = reinterpret_cast<const char*>(at - m * S);
-    if (m == 0) { ld_raw<16, false>(from, w); return; }
-    u32 x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (f - m + V > 0) ld_raw<16, false>(from, x);
-    if (f - m + V < F) ld_raw<16, false>(from + 16, x + 4);
-    const int words = m * S / 4;
-    if (words & 2) {
+    const u64 from = at - (u64)(m * S), next = from + 16;
+    const bool first = f - m + V > 0, second = m && f - m + V < F;
+    ld_raw<16, false>(reinterpret_cast<const char*>(first ? from : next), x);
+    ld_raw<16, false>(reinterpret_cast<const char*>(second ? next : first ? from : next), x + 4);
+}
+template <int DT> DEV int off_boundary(u64 base, i64 item, int f) { return (int)((base + (u64)((item + f) * dt_size<DT>::value)) & 15u); }
+DEV void join_two(const u32* x, int off, u32* w) {     // off: bytes behind a boundary
+    const int words = off / 4;
+    const u32 bits = off & 2 ? 16 : 0;
 #pragma unroll
-        for (int i = 0; i < 6; ++i) x[i] = x[i + 2];
+    for (int i = 0; i < 4; ++i) {
+        u32 lo = x[i], hi = x[i + 1];
+#pragma unroll
+        for (int k = 1; k < 4; ++k)
+            if (words == k) { lo = x[i + k]; hi = x[(i + k + 1) & 7]; }
+        w[i] = __funnelshift_r(lo, hi, bits);
     }
-    if (words & 1) {
-#pragma unroll
-        for (int i = 0; i < 5; ++i) x[i] = x[i + 1];
-    }
-    const u32 bits = S == 2 && (m & 1) ? 16 : 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(x[i], x[i + 1], bits);
 }
 
 DEV float warp_sum(float v) {

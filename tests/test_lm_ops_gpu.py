@@ -728,3 +728,10 @@ def test_layer_norm_wide_items(b200, f, n, dtype, inplace):
     x, gamma, beta, e = ln_inputs(f, n, dtype, np.float32)
     got = run_ln(b200, x, gamma, beta, e, dtype, np.float32, "rows", inplace=inplace)
     compare(got, want_ln(x, gamma, beta, e, got, dtype, np.float32))
+
+
+@pytest.mark.parametrize("v,f,n", [(700, 1001, 900), (90, 301, 3000), (40, 333, 200), (2000, 2047, 37), (300, 176, 20000)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: np.dtype(d).name)
+def test_lookup_widths_off_the_boundaries(b200, v, f, n, dtype):
+    """Rows that are written by whole warps, some of whose lanes have no feature."""
+    test_lookup_sizes_and_orders(b200, v, f, n, dtype)
