@@ -368,27 +368,32 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bprop_rows(const __grid_constan
         }
 }
 
-// The sum of the blocks' shares: 8 columns of [grad_gamma | grad_beta] per block (one sector of
-// every share), 128 rows of threads, each over its shares in their order.
-__global__ void __launch_bounds__(1024) ln_sum_parts(const float* part, int parts, i64 F, u64 ggamma, u64 gbeta, int pdt) {
-    __shared__ float s[32][8];
-    const i64 c = (i64)blockIdx.x * 8 + (threadIdx.x & 7);
+// The sum of the blocks' shares: COLS columns of [grad_gamma | grad_beta] per block, ROWS rows of
+// threads, each over its shares in their order: 8 x 128 (one sector of every share), or 32 x 8 where
+// there are few shares (25 of 13925 features: 4 us instead of 18).
+template <int COLS, int ROWS>
+__global__ void __launch_bounds__(COLS * ROWS) ln_sum_parts(const float* part, int parts, i64 F, u64 ggamma, u64 gbeta, int pdt) {
+    grid_enter();
+    constexpr int WARPS = COLS * ROWS / 32;
+    __shared__ float s[WARPS][COLS + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const i64 c = (i64)blockIdx.x * COLS + threadIdx.x % COLS;
     float a = 0.f;
     if (c < 2 * F) {
 #pragma unroll 4
-        for (int b = threadIdx.x >> 3; b < parts; b += 128) a += part[(i64)b * 2 * F + c];
+        for (int b = threadIdx.x / COLS; b < parts; b += ROWS) a += part[(i64)b * 2 * F + c];
     }
-    a += __shfl_xor_sync(0xffffffffu, a, 8);
-    a += __shfl_xor_sync(0xffffffffu, a, 16);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane < 8) s[warp][lane] = a;
+#pragma unroll
+    for (int o = COLS; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if (lane < COLS) s[warp][lane] = a;
     __syncthreads();
-    if (warp >= 8) return;
-    a = warp_sum(s[lane][warp]);
-    const i64 out = (i64)blockIdx.x * 8 + warp;
-    if (lane == 0 && out < 2 * F) {
-        const u64 to = out < F ? ggamma : gbeta;
-        if (to) st_any(to, out < F ? out : out - F, pdt, a);
+    for (int i = warp; i < COLS; i += WARPS) {
+        a = warp_sum(lane < WARPS ? s[lane][i] : 0.f);
+        const i64 out = (i64)blockIdx.x * COLS + i;
+        if (lane == 0 && out < 2 * F) {
+            const u64 to = out < F ? ggamma : gbeta;
+            if (to) st_any(to, out < F ? out : out - F, pdt, a);
+        }
     }
 }
 
@@ -1176,8 +1181,10 @@ extern "C" b200_status b200_ln_bprop(const b200_matrix* delta, const b200_matrix
             err = launch_cols_type<true>(p, wide, at, part, &parts, count, s);
         }
         if (part && err == cudaSuccess) {
-            ln_sum_parts<<<(unsigned)((2 * features + 7) / 8), 1024, 0, s>>>(part, parts, features, grad_gamma, grad_beta, param_dtype);
-            err = cudaGetLastError();
+            err = parts <= 64 ? launch_dependent(ln_sum_parts<32, 8>, dim3((unsigned)((2 * features + 31) / 32)), 256, 0, s, part, parts,
+                                                 features, grad_gamma, grad_beta, param_dtype)
+                              : launch_dependent(ln_sum_parts<8, 128>, dim3((unsigned)((2 * features + 7) / 8)), 1024, 0, s, part, parts,
+                                                 features, grad_gamma, grad_beta, param_dtype);
             ++count;
         }
     } else {
