@@ -858,7 +858,7 @@ template <bool POLICY, int DT, int V> cudaError_t launch_cols(const CostP& all, 
         p.part = reinterpret_cast<float2*>(scratch);
         p.item = reinterpret_cast<float4*>(scratch + 8 * kSplits * slice);
         p.grad = reinterpret_cast<float*>(scratch + (8 * kSplits + 16) * slice);
-        p.splits = (int)cut(room / across < kSplits ? room / across : kSplits);
+        p.splits = (int)cut(room / across < kSplits ? room / across : (i64)kSplits);
         cudaError_t e = launch_dependent(cost_cols_stats<DT, V>, dim3((unsigned)across, (unsigned)p.splits), kColThreads, 0, s, p);
         if (e == cudaSuccess) e = launch_dependent(cost_cols_items<POLICY>, dim3((unsigned)c.N), 32, POLICY ? 0 : 12 * ((c.K + 3) / 4 * 4), s, p);
         launches += 2;
@@ -916,12 +916,18 @@ template <bool POLICY> cudaError_t launch_any(const CostP& p, cudaStream_t s) {
 
 // How many threads a row gets, and with them how many rows are under way: small blocks keep more
 // rows of an SM at different points of their way, but a row stays in L2 between its two walks only
-// if the rows under way do: the smallest block with which they hold no more than 50 MB, or any if
-// all logits together hold no more than 66.  Measured, us, blocks per SM in brackets: 32768 words
-// bf16 x 4096 (64 KB a row), 128 threads (8) 127, 256 (3) 99; 50257 bf16 x 2048, 256 (3) 82, 256 (4)
-// 89, 512 (2) 102; 32768 f32 x 4096, 256 (3) 228, 512 (2) 210; 131072 bf16 x 4096, 512 (2) 489, 1024
-// (1) 412; 32003 f16 x 1000, 128 (8) 30, 256 (4) 37.  Rows of up to 8 KB are a warp's: 4001 bf16 x
-// 16384, 32 threads 54, 128 85.
+// if the rows under way do: the smallest block with which they hold no more than 50 MB (f32: 25, since
+// its walks have half the instructions per byte and so lean more on L2), or any if all logits together
+// hold no more than 66.  Measured, us, blocks per SM in brackets:
+//     32768 bf16 x 4096 (64 KB a row)    128 threads (8) 127    256 (3) 99
+//     50257 bf16 x 2048                  256 (3) 82    256 (4) 89    512 (2) 102
+//     65536 bf16 x 4096                  256 (3) 238   512 (2) 193   1024 (1) 231
+//     131072 bf16 x 4096                 512 (2) 489   1024 (1) 412
+//     10000 f32 x 8192                   128 (8) 134   256 (3) 126   512 (2) 161
+//     16384 f32 x 8192                   256 (3) 199   512 (2) 181   1024 (1) 248
+//     32768 f32 x 4096                   256 (3) 232   512 (2) 212   1024 (1) 203
+//     32003 f16 x 1000                   128 (8) 30    256 (4) 37
+// Rows of up to 8 KB are a warp's: 4001 bf16 x 16384, 32 threads 54, 128 85.
 template <bool POLICY, int DT, int RING, int T, int MINB> cudaError_t launch_rows_of(const CostP& p, cudaStream_t s) {
     const int smem = RING * 4 * T * 16 + (POLICY ? 0 : 24 * ((p.K + 3) / 4 * 4));
     const i64 most = resident_blocks(cost_rows<POLICY, DT, RING, T, MINB>, T, smem);
@@ -931,7 +937,7 @@ template <bool POLICY, int DT, int RING, int T, int MINB> cudaError_t launch_row
 }
 template <bool POLICY, int DT> cudaError_t launch_rows(const CostP& p, cudaStream_t s) {
     const i64 bytes = (i64)p.V * dt_size<DT>::value;
-    auto fits = [&](int per_sm) { return p.N * bytes <= 66 * 1000 * 1000 || 148 * per_sm * bytes <= 50 * 1000 * 1000; };
+    auto fits = [&](int per_sm) { return p.N * bytes <= 66 * 1000 * 1000 || 148 * per_sm * bytes <= (DT == F32 ? 25 : 50) * 1000 * 1000; };
     if (bytes <= 8 * 1024) return launch_rows_of<POLICY, DT, 3, 32, 24>(p, s);
     if (fits(8)) return launch_rows_of<POLICY, DT, 2, 128, 8>(p, s);
     if (fits(3)) return launch_rows_of<POLICY, DT, 3, 256, 3>(p, s);
