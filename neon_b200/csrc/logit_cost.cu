@@ -572,20 +572,27 @@ template <int DT, int V> struct Pairs {
     DEV f32x2 get(int l) const { return get2<DT>(w, l); }
 };
 // A single item's words first, first + step, ... below end (rows that are not whole 16-byte
-// vectors): eight under way, two in a pair.
+// vectors): eight under way, two in a pair; at `from` is the first, `dist` bytes before the next.
 enum { kSingle = 8 };
-template <int DT> DEV void single_words(u64 base, i64 pitch, i64 n, int first, int step, int end, float* z) {
+template <int DT> DEV void single_words(u64 from, i64 dist, int first, int step, int end, float* z) {
+    if (first + (kSingle - 1) * step < end) {
 #pragma unroll
-    for (int u = 0; u < kSingle; ++u) z[u] = first + u * step < end ? ld_any(base, (i64)(first + u * step) * pitch + n, DT) : -INFINITY;
+        for (int u = 0; u < kSingle; ++u) z[u] = ld_any(from + u * dist, 0, DT);
+    } else {
+#pragma unroll
+        for (int u = 0; u < kSingle; ++u) z[u] = first + u * step < end ? ld_any(from + u * dist, 0, DT) : -INFINITY;
+    }
 }
 template <int DT> DEV void single_stats(const ColsP& p, i64 n, int first, int step, int end, float& m, float& sum) {
     const float c = p.c.c;
     const f32x2 c2 = pair(c, c);
     f32x2 s = 0, less = 0;
     m = -INFINITY;
-    for (int v0 = first; v0 < end; v0 += kSingle * step) {
+    const i64 dist = step * p.c.z0 * dt_size<DT>::value;
+    u64 from = p.c.z + (u64)((first * p.c.z0 + n) * dt_size<DT>::value);
+    for (int v0 = first; v0 < end; v0 += kSingle * step, from += kSingle * dist) {
         float z[kSingle];
-        single_words<DT>(p.c.z, p.c.z0, n, v0, step, end, z);
+        single_words<DT>(from, dist, v0, step, end, z);
         float a = z[0];
 #pragma unroll
         for (int u = 1; u < kSingle; ++u) a = fmaxf(a, z[u]);
@@ -607,18 +614,22 @@ template <int DT> DEV void single_stats(const ColsP& p, i64 n, int first, int st
 template <int DT> DEV void single_delta(const ColsP& p, i64 n, int first, int step, int end) {
     const float4 it = p.item[n];
     const f32x2 c2 = pair(p.c.c, p.c.c), less = pair(-it.x, -it.x), scale = pair(it.y, it.y);
-    for (int v0 = first; v0 < end; v0 += kSingle * step) {
+    const u32 alive = it.z != 0.f ? 0u : ~0u;          // bits of the results
+    const i64 dist = step * p.c.z0 * dt_size<DT>::value, out = step * p.c.d0 * dt_size<DT>::value;
+    u64 from = p.c.z + (u64)((first * p.c.z0 + n) * dt_size<DT>::value), to = p.c.d + (u64)((first * p.c.d0 + n) * dt_size<DT>::value);
+    for (int v0 = first; v0 < end; v0 += kSingle * step, from += kSingle * dist, to += kSingle * out) {
         float z[kSingle];
-        single_words<DT>(p.c.z, p.c.z0, n, v0, step, end, z);
+        single_words<DT>(from, dist, v0, step, end, z);
 #pragma unroll
         for (int u = 0; u < kSingle; u += 2) {
             float x, y;
             split(mul2(add2(pair(z[u], z[u + 1]), less), c2), x, y);
-            split(mul2(scale, pair(ex2_approx(x), ex2_approx(y))), x, y);
-            const i64 v = v0 + u * step;
-            if (v < end) st_any(p.c.d, v * p.c.d0 + n, DT, it.z != 0.f ? 0.f : x);
-            if (v + step < end) st_any(p.c.d, (v + step) * p.c.d0 + n, DT, it.z != 0.f ? 0.f : y);
+            split(mul2(scale, pair(ex2_approx(x), ex2_approx(y))), z[u], z[u + 1]);
         }
+        const bool whole = v0 + (kSingle - 1) * step < end;
+#pragma unroll
+        for (int u = 0; u < kSingle; ++u)
+            if (whole || v0 + u * step < end) st_any(to + u * out, 0, DT, __uint_as_float(__float_as_uint(z[u]) & alive));
     }
 }
 
