@@ -503,7 +503,7 @@ template <bool BACK> cudaError_t launch_type(const LnP& p, bool mis, float* part
 // stripe's phases in turn; the loops have constant distances for that (backwards 179 -> 152 us at
 // 1024 x 65536 bf16) and the next stripe is under way meanwhile (152 -> 134 us; forwards 70 us, 59 %
 // of the copy rate against 47 %; backwards at 1001 x 4096 f32 21 us).  Rows that are not whole
-// 16-byte vectors go item by item: 81 and 199 us at 1001 x 32767 bf16, four items a thread, against
+// 16-byte vectors go item by item: 81 and 197 us at 1001 x 32767 bf16, four items a thread, against
 // 103 and 317 us with one.
 //
 // A thread's place in its stripe: its V items, next to each other from n on, or, where the rows do
@@ -1035,6 +1035,8 @@ template <int DT, int V, bool BACK> cudaError_t launch_cols(const LnP& p, char* 
         if (c.held && c.lanes == 4) return launch_cols_one<DT, V, BACK, true, 4>(p, c, part, parts, s);
         if (c.held && c.lanes == 2) return launch_cols_one<DT, V, BACK, true, 2>(p, c, part, parts, s);
     }
+    if constexpr (V < 0)
+        if (c.lanes == 32) return launch_cols_one<DT, V, BACK, false, 32>(p, c, part, parts, s);
     return launch_cols_one<DT, V, BACK, false, 0>(p, c, part, parts, s);
 }
 template <bool BACK> cudaError_t launch_cols_type(const LnP& p, bool wide, char* scratch, float* part, int* parts, int& launches, cudaStream_t s) {
