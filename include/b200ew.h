@@ -229,7 +229,8 @@ b200_status b200_log2_hist(uint64_t in, int32_t dtype, uint64_t count, uint64_t 
  * next to each other) can be handed in.  Vectors of one value per feature or per item are
  * contiguous; an address of 0 leaves an optional one out.  An output may be the input of the same
  * shape itself where that is said; any other sharing of memory is refused (B200_ERR_INVALID).
- * Element types of matrices: f32, f16, bf16, with fp32 arithmetic and rounding to nearest.
+ * Element types of matrices: f32, f16, bf16, with fp32 arithmetic and rounding to nearest.  At most
+ * 2^30 features (lookup: 65535 * 32) or words of logits.
  * `scratch` is 256-byte aligned device memory of at least the size the matching *_scratch_bytes
  * function gives; it is overwritten, and calls that share it must be ordered on the GPU.
  * `launches` (may be null) receives the number of kernels launched. */
