@@ -426,7 +426,8 @@ __global__ void __launch_bounds__(T, MINB) cost_rows(const __grid_constant__ Cos
         }
         const bool skip = skipped<POLICY>(p, w_item, a_item);
         Item it = {0.f, 0.f, 1};
-        const int mis = mis_of(n), kfirst = mis >> LV, nvec = (p.V + mis + V - 1) >> LV, whole = (p.V + mis) >> LV;
+        const int mis = mis_of(n), nvec = (p.V + mis + V - 1) >> LV;
+        const int full = (mis + V - 1) >> LV, whole = (p.V + mis) >> LV;       // vectors [full, whole) are all the row's
         const i64 drow = n * p.d1;
         float at_word = 0.f;
         Entries e;
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(T, MINB) cost_rows(const __grid_constant__ Cos
                         const int k = k0 + u * T + tid;
                         u32 w[1][4];
                         ld_raw<16, false>(here, w[0]);
-                        if (k <= kfirst || k >= nvec - 1) mask_end<DT>(w[0], k * V - mis, p.V);
+                        if (k < full || k >= whole) mask_end<DT>(w[0], k * V - mis, p.V);
                         take<DT, 1>(r, w, p.c);
                     }
                 }
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(T, MINB) cost_rows(const __grid_constant__ Cos
                             ld_raw<16, false>(here, w);
                             give<DT>(w, it, p.c);
                         }
-                        if (k <= kfirst || k >= nvec - 1) put_part<DT, V>(p.d, drow, k * V - mis, p.V, w);
+                        if (k < full || k >= whole) put_part<DT, V>(p.d, drow, k * V - mis, p.V, w);
                         else st_raw<16>(to + u * JUMP, w);
                     }
                 }

@@ -18,7 +18,8 @@ are, handed over as the transposed view of an (items, features) tensor::
 Arithmetic is fp32; results are rounded to the tensor's type once, to nearest (a tensor whose
 ``rounding`` asks for stochastic rounding is refused as a result).  Work is issued on
 ``be.stream`` and uses the backend's scratch, as statements do; nothing is allocated, so a
-call can be recorded with ``be.capture``.
+call can be recorded with ``be.capture``.  A backend's calls and recorded graphs share that
+scratch: they are to follow one another on one stream.
 """
 
 from . import runtime as rt
